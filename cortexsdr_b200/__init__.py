@@ -26,12 +26,13 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import (DTYPE_BF16, DTYPE_F32, FEATURE_MAJOR, TOKEN_MAJOR, DecoderConfig, PayloadInfo,
-                   SegmentHeader)
+from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, FEATURE_MAJOR, TOKEN_MAJOR, DecoderConfig, KVBatchStruct,
+                   PayloadInfo, SegmentHeader)
 
 __all__ = ["CompressionError", "Context", "Segment", "Dictionary", "HierarchicalSDRStrategy",
            "SDRModelLoader", "SDRInferenceEngine", "HSDAReader", "Decoder", "default_context",
-           "HSDR_STRATEGY_ID", "NcclComm", "nccl_unique_id"]
+           "HSDR_STRATEGY_ID", "NcclComm", "nccl_unique_id", "KVBatch", "KVCache", "Q4Weight",
+           "token_logprobs_device"]
 
 HSDR_STRATEGY_ID = 5
 
@@ -740,6 +741,107 @@ class NcclComm:
             self.close()
         except Exception:
             pass
+
+
+class KVBatch:
+    """A ragged batch of new tokens over a paged cache (csdr_kv_batch). Device pointers to int32 arrays: `first_ptr` (n_seqs + 1
+    row numbers), `length_ptr` (n_seqs, tokens with the new ones), `pages_ptr` (n_seqs x pages_per_seq). The arrays
+    are read when a call runs: they may change between calls and between replays of a graph."""
+
+    def __init__(self, n_seqs: int, n_tokens: int, first_ptr: int, length_ptr: int, pages_ptr: int, pages_per_seq: int):
+        self._s = KVBatchStruct(n_seqs, n_tokens, pages_per_seq, first_ptr, length_ptr, pages_ptr)
+        self._ref = C.addressof(self._s)
+
+
+class KVCache:
+    """Paged key/value cache held in 4 bits. dtype arguments: DTYPE_F32, DTYPE_BF16 or DTYPE_F16; pointers are device
+    addresses (e.g. torch tensors' data_ptr()); strides in elements between tokens, 0: dense rows. All calls are
+    asynchronous on the context's stream."""
+
+    def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, *, layers: int = 1, rope_theta: float = 1e6,
+                 ctx: Context | None = None):
+        self.ctx = ctx or default_context()
+        h = C.c_void_p()
+        _check(self.ctx._lib.csdr_kv_cache_create(self.ctx._h, layers, pages, page_tokens, kv_heads, head_dim, rope_theta, C.byref(h)))
+        self._h = h
+        self.ctx._adopt(self)
+
+    @property
+    def nbytes(self) -> int:
+        n = C.c_size_t()
+        _check(self.ctx._lib.csdr_kv_cache_bytes(self._h, C.byref(n)))
+        return n.value
+
+    def append(self, batch: KVBatch, k_ptr: int, v_ptr: int, dtype: int, *, kv_stride: int = 0, rotate: bool = True, q_ptr: int = 0,
+               q_stride: int = 0, q_heads: int = 0, q_out_ptr: int = 0, q_out_stride: int = 0, layer: int = 0):
+        """Store the new tokens' keys and values; rotate: keys, and queries where given, turn by their position."""
+        _check(self.ctx._lib.csdr_kv_cache_append_device_async(
+            self._h, layer, batch._ref, k_ptr, v_ptr, kv_stride, dtype, 1 if rotate else 0, q_ptr or None, q_stride, q_heads,
+            q_out_ptr or None, q_out_stride))
+
+    def read(self, batch: KVBatch, k_ptr: int, v_ptr: int, *, layer: int = 0):
+        """The values that the batch's new tokens are held as, fp32 (n_tokens, kv_heads, head_dim)."""
+        _check(self.ctx._lib.csdr_kv_cache_read_device_async(self._h, layer, batch._ref, k_ptr, v_ptr))
+
+    def attention(self, batch: KVBatch, q_ptr: int, dtype: int, q_heads: int, out_ptr: int, *, q_stride: int = 0, out_stride: int = 0,
+                  scale: float = 0.0, layer: int = 0):
+        """Causal grouped-query attention of the new tokens over their sequences; scale 0: 1 / sqrt(head_dim)."""
+        _check(self.ctx._lib.csdr_kv_cache_attention_device_async(self._h, layer, batch._ref, q_ptr, q_stride, dtype, q_heads, scale,
+                                                                  out_ptr, out_stride))
+
+    def close(self):
+        if getattr(self, "_h", None) and self.ctx._h:
+            self.ctx._lib.csdr_kv_cache_destroy(self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Q4Weight:
+    """Device image of a weight stored in 4 bits ("q4_0" or "q4_k" blocks, as archives hold them)."""
+
+    def __init__(self, ctx: Context, handle, rows: int, cols: int):
+        self.ctx, self._h, self.rows, self.cols = ctx, handle, rows, cols
+        self._close_rank = 0
+        ctx._adopt(self)
+
+    @classmethod
+    def from_payload(cls, payload, format: str, rows: int, cols: int, ctx: Context | None = None) -> "Q4Weight":
+        ctx = ctx or default_context()
+        p = _bytes(payload)
+        h = C.c_void_p()
+        _check(ctx._lib.csdr_q4_create(ctx._h, format.encode(), p.ctypes.data_as(C.c_void_p), p.size, rows, cols, C.byref(h)))
+        return cls(ctx, h, rows, cols)
+
+    def matmul_device(self, x_ptr: int, x_dtype: int, x_layout: int, batch: int, y_ptr: int, y_layout: int, bias_ptr: int = 0):
+        """Asynchronous product on raw device pointers, fp32 out (Segment.matmul_device; x may be fp16 too)."""
+        _check(self.ctx._lib.csdr_q4_matmul_device_async(self.ctx._h, self._h, x_ptr, x_dtype, x_layout, batch, y_ptr, y_layout,
+                                                         bias_ptr or None))
+
+    def close(self):
+        if getattr(self, "_h", None) and self.ctx._h:
+            self.ctx._lib.csdr_q4_destroy(self._h)
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def token_logprobs_device(logits_ptr: int, dtype: int, rows: int, vocab: int, targets_ptr: int, logprobs_ptr: int, entropy_ptr: int = 0,
+                          top: int = 0, top_ids_ptr: int = 0, top_logprobs_ptr: int = 0, *, stride: int = 0,
+                          ctx: Context | None = None):
+    """Log probabilities of given tokens, entropy and top alternatives of rows of logits, on device pointers (0: not wanted)."""
+    ctx = ctx or default_context()
+    _check(ctx._lib.csdr_token_logprobs_device_async(ctx._h, logits_ptr, dtype, stride, rows, vocab, targets_ptr or None,
+                                                     logprobs_ptr or None, entropy_ptr or None, top, top_ids_ptr or None,
+                                                     top_logprobs_ptr or None))
 
 
 class Decoder:

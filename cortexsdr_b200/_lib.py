@@ -25,7 +25,7 @@ ERR_BUFFER = -10
 ERR_CODE_RANGE = -11
 ERR_LIMIT = -12
 
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 FEATURE_MAJOR, TOKEN_MAJOR = 0, 1
 
 
@@ -62,6 +62,11 @@ class DecoderConfig(C.Structure):
                 ("vocab", C.c_uint32), ("max_seq", C.c_uint32), ("max_batch", C.c_uint32),
                 ("rms_eps", C.c_float), ("rope_theta", C.c_float), ("tp_rank", C.c_uint32),
                 ("tp_size", C.c_uint32), ("nccl_comm", C.c_void_p), ("kv_dtype", C.c_uint32)]
+
+
+class KVBatchStruct(C.Structure):
+    _fields_ = [("n_seqs", C.c_uint32), ("n_tokens", C.c_uint32), ("pages_per_seq", C.c_uint32),
+                ("first_dev", C.c_void_p), ("length_dev", C.c_void_p), ("pages_dev", C.c_void_p)]
 
 
 _P = C.c_void_p
@@ -148,6 +153,19 @@ SIGNATURES = {
     "csdr_decoder_forward": (C.c_int, [_P, C.c_uint32, C.POINTER(C.c_int32), _SZ, _F, _F]),
     "csdr_decoder_step": (C.c_int, [_P, C.POINTER(C.c_int32), _SZ, C.POINTER(C.c_int32), _F]),
     "csdr_decoder_step_device_async": (C.c_int, [_P, _P, _SZ, _P]),
+    "csdr_kv_cache_create": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float,
+                                       C.POINTER(_P)]),
+    "csdr_kv_cache_destroy": (C.c_int, [_P]),
+    "csdr_kv_cache_bytes": (C.c_int, [_P, C.POINTER(_SZ)]),
+    "csdr_kv_cache_append_device_async": (C.c_int, [_P, C.c_uint32, _P, _P, _P, _SZ, C.c_int, C.c_int, _P, _SZ,
+                                                    C.c_uint32, _P, _SZ]),
+    "csdr_kv_cache_read_device_async": (C.c_int, [_P, C.c_uint32, _P, _P, _P]),
+    "csdr_kv_cache_attention_device_async": (C.c_int, [_P, C.c_uint32, _P, _P, _SZ, C.c_int, C.c_uint32, C.c_float,
+                                                       _P, _SZ]),
+    "csdr_q4_create": (C.c_int, [_P, C.c_char_p, _P, _SZ, C.c_uint32, C.c_uint32, C.POINTER(_P)]),
+    "csdr_q4_destroy": (C.c_int, [_P]),
+    "csdr_q4_matmul_device_async": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, _SZ, _P, C.c_int, _P]),
+    "csdr_token_logprobs_device_async": (C.c_int, [_P, _P, C.c_int, _SZ, _SZ, _SZ, _P, _P, _P, C.c_uint32, _P, _P]),
     "csdr_nccl_unique_id": (C.c_int, [_P]),
     "csdr_nccl_comm_create": (C.c_int, [_P, _P, C.c_int, C.c_int, C.POINTER(_P)]),
     "csdr_nccl_comm_destroy": (C.c_int, [_P]),

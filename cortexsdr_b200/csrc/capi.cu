@@ -102,7 +102,8 @@ const char* kernel_class_name(int cls) {
     static const char* names[KC_COUNT] = {"hsdr_unpack", "hsdr_dx", "hsdr_gather", "hsdr_tile_project",
                                           "hsdr_tile_gather", "hsdr_edge", "dense_rows", "hsdr_decode_rows",
                                           "dequant", "hsdr_gemm_tcgen05", "decoder_op", "hsdr_gemv_fused", "attention",
-                                          "hsdr_gemv_queue", "hsdr_encode"};
+                                          "hsdr_gemv_queue", "hsdr_encode", "kv_cache", "kv_attention", "q4_matmul",
+                                          "token_logprobs"};
     return (cls >= 0 && cls < KC_COUNT) ? names[cls] : "?";
 }
 

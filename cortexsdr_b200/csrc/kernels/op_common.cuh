@@ -1,0 +1,64 @@
+// What the operator kernels (kv_cache.cu, q4_matmul.cu, logprobs.cu) share.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "../internal.hpp"
+
+namespace csdr {
+
+// Lets the kernel behind on the stream start its own prologue, then waits until everything before on the
+// stream has completed and is visible: no global memory is touched before.
+__device__ __forceinline__ void op_enter() {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// The kernel must begin with op_enter(). cluster: CTAs of a cluster along x (1: none).
+template <typename... KArgs, typename... Args>
+void launch_op(csdr_context* ctx, void (*kern)(KArgs...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = ctx->pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    CSDR_CUDA(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
+}
+
+__device__ __forceinline__ float op_widen(float v) { return v; }
+__device__ __forceinline__ float op_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float op_widen(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T op_narrow(float v);
+template <>
+__device__ __forceinline__ float op_narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 op_narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half op_narrow<__half>(float v) { return __float2half_rn(v); }
+
+// Calls f with a null pointer of the element type that a CSDR_DTYPE_* stands for.
+template <typename F>
+void with_dtype(int dtype, F&& f) {
+    switch (dtype) {
+        case CSDR_DTYPE_F32: f(static_cast<float*>(nullptr)); break;
+        case CSDR_DTYPE_BF16: f(static_cast<__nv_bfloat16*>(nullptr)); break;
+        case CSDR_DTYPE_F16: f(static_cast<__half*>(nullptr)); break;
+        default: throw Error(CSDR_ERR_INVALID_ARG, "unknown dtype");
+    }
+}
+
+}  // namespace csdr

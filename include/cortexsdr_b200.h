@@ -55,7 +55,7 @@ enum {
 };
 
 enum { CSDR_DTYPE_F32 = 0, CSDR_DTYPE_BF16 = 1,
-       CSDR_DTYPE_F16 = 2 /* KV-cache element type only; activations are fp32 or bf16 */ };
+       CSDR_DTYPE_F16 = 2 /* KV caches and the operators that say so; elsewhere activations are fp32 or bf16 */ };
 enum { CSDR_LAYOUT_FEATURE_MAJOR = 0, CSDR_LAYOUT_TOKEN_MAJOR = 1 };
 enum { CSDR_KIND_HSDR = 0, CSDR_KIND_HSDC = 1 };
 
@@ -65,6 +65,8 @@ typedef struct csdr_dictionary csdr_dictionary; /* device image of a shared dict
 typedef struct csdr_archive csdr_archive;       /* an opened .sdr */
 typedef struct csdr_hsda csdr_hsda;             /* an opened .hsda */
 typedef struct csdr_decoder csdr_decoder;       /* device-resident decoder-layer driver */
+typedef struct csdr_kv_cache csdr_kv_cache;     /* paged key/value cache held in 4 bits */
+typedef struct csdr_q4_weight csdr_q4_weight;   /* device image of a weight stored in 4 bits */
 
 /* Fields of the payload header (HSDRHeader, strategies/HierarchicalSDRStrategy.cpp:49-66;
  * HSDRCodesHeader, :675-692) plus the byte offsets of the streams behind it. */
@@ -483,6 +485,83 @@ CSDR_API int csdr_decoder_step(csdr_decoder* d, const int32_t* tokens, size_t ba
 /* Same step, nothing copied to the host: tokens_dev in, next_dev out (device int32). */
 CSDR_API int csdr_decoder_step_device_async(csdr_decoder* d, const int32_t* tokens_dev,
                                             size_t batch, int32_t* next_dev);
+
+/* ---- paged key/value cache held in 4 bits (no counterpart in the reference) ----
+ * Keys and values of a layer in pages of page_tokens tokens (a power of two, 16 to 4096), shared by any
+ * number of sequences through page tables. Each group of 64 values of a head is held as 4-bit codes with
+ * an fp16 minimum and an fp16 step: minimum + step * code, step = (max - min) / 15 (4.5 bits a value with
+ * head_dim 64, 128 or 256; 0.28 of an fp16 cache). A group that holds a value that is not finite reads
+ * back as NaN; values past 65504 saturate. rope_theta > 0: the rotary embedding that
+ * csdr_kv_cache_append_device_async applies on request. */
+CSDR_API int csdr_kv_cache_create(csdr_context* ctx, uint32_t n_layers, uint32_t n_pages,
+                                  uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim,
+                                  float rope_theta, csdr_kv_cache** out);
+CSDR_API int csdr_kv_cache_destroy(csdr_kv_cache* cache);
+CSDR_API int csdr_kv_cache_bytes(const csdr_kv_cache* cache, size_t* bytes);
+
+/* A ragged batch of new tokens, all arrays on the device. Sequence s has rows first_dev[s] to
+ * first_dev[s + 1] - 1 of the operands (n_seqs + 1 entries, not falling; no rows: an idle sequence) and
+ * length_dev[s] tokens with these new ones at its end; its token p lies in page
+ * pages_dev[s * pages_per_seq + p / page_tokens]. Rows that belong to no sequence (before the first or behind
+ * the last; n_tokens says how many rows the operands have) are left as they were. A token whose page is
+ * negative or not below n_pages, or whose position is negative or behind the table, has no place: it is
+ * not stored, and attention does not see it. */
+typedef struct {
+    uint32_t n_seqs, n_tokens, pages_per_seq;
+    const int32_t* first_dev;
+    const int32_t* length_dev;
+    const int32_t* pages_dev;
+} csdr_kv_batch;
+
+/* Stores the new tokens' keys and values (n_tokens x kv_heads x head_dim; kv_stride elements between the
+ * rows of either, 0: dense; dtype: CSDR_DTYPE_F32, _BF16 or _F16). rotate != 0: keys, and queries where given
+ * (q_dev, q_stride, q_heads -> q_out_dev, q_out_stride; q_out may be q itself), are rotated by their position
+ * as the decoder rotates them (adjacent pairs, api/cortex_sdk.cpp:1363-1423), angles in 64 bits; else
+ * queries are copied. Tokens must have slots of their own. Asynchronous on the cache's context. */
+CSDR_API int csdr_kv_cache_append_device_async(csdr_kv_cache* cache, uint32_t layer,
+                                               const csdr_kv_batch* batch, const void* k_dev,
+                                               const void* v_dev, size_t kv_stride, int dtype, int rotate,
+                                               const void* q_dev, size_t q_stride, uint32_t q_heads,
+                                               void* q_out_dev, size_t q_out_stride);
+/* The values that the batch's new tokens are held as (fp32, n_tokens x kv_heads x head_dim); zeros for a
+ * token without a place. A batch whose new tokens are all of a sequence's tokens reads it whole. */
+CSDR_API int csdr_kv_cache_read_device_async(csdr_kv_cache* cache, uint32_t layer,
+                                             const csdr_kv_batch* batch, float* k_dev, float* v_dev);
+/* Causal grouped-query attention of the new tokens (already stored) over their sequences' cached tokens:
+ * out = softmax(scale * q k^T) v (multi_head_attention, kernels/attention_kernels.cpp:26-113), a new token
+ * seeing every token up to its own position. q and out: n_tokens x q_heads x head_dim of `dtype`, strides
+ * as above; out must not overlap q; scale 0: 1 / sqrt(head_dim). A token that sees nothing gets zeros.
+ * Scores, weights and sums in fp32. Calls on one cache share its workspace: they run one after
+ * the other, graphs that were captured from them too. */
+CSDR_API int csdr_kv_cache_attention_device_async(csdr_kv_cache* cache, uint32_t layer,
+                                                  const csdr_kv_batch* batch, const void* q_dev,
+                                                  size_t q_stride, int dtype, uint32_t q_heads, float scale,
+                                                  void* out_dev, size_t out_stride);
+
+/* ---- products with weights stored in 4 bits ----
+ * format "q4_0" or "q4_k": the blocks of a stored-raw tensor as decodeSupportedGGUFQuantized reads them
+ * (SparseInferenceEngine.cpp:276-469; csdr_dequantize_inference gives the same matrix). rows x cols, cols on
+ * whole blocks (32 or 256). The weight is laid out once and stays packed. */
+CSDR_API int csdr_q4_create(csdr_context* ctx, const char* format, const void* payload, size_t nbytes,
+                            uint32_t rows, uint32_t cols, csdr_q4_weight** out);
+CSDR_API int csdr_q4_destroy(csdr_q4_weight* weight);
+/* y = W x (+ bias), fp32 out; dtypes (CSDR_DTYPE_F16 too) and layouts as csdr_matmul_device_async. Products and sums
+ * are those of fp32 activations. Asynchronous on the context's stream. */
+CSDR_API int csdr_q4_matmul_device_async(csdr_context* ctx, const csdr_q4_weight* weight,
+                                         const void* x_dev, int x_dtype, int x_layout, size_t batch,
+                                         float* y_dev, int y_layout, const float* bias_dev);
+
+/* ---- log probabilities of given tokens ----
+ * logits: rows x vocab of `dtype`, `stride` elements between rows (0: vocab). Each may be NULL:
+ * logprobs_dev[r] = log softmax(row r)[targets_dev[r]] (a target outside the vocabulary: NaN);
+ * entropy_dev[r] = -sum p log p. top > 0 (at most 32): the top alternatives' ids and log
+ * probabilities, rows x top, largest first, equal logits by index. A row without a softmax (a NaN or +infinity,
+ * or nothing above -infinity) answers NaN, ids -1. Asynchronous on the context's stream. */
+CSDR_API int csdr_token_logprobs_device_async(csdr_context* ctx, const void* logits_dev, int dtype,
+                                              size_t stride, size_t rows, size_t vocab,
+                                              const int32_t* targets_dev, float* logprobs_dev,
+                                              float* entropy_dev, uint32_t top, int32_t* top_ids_dev,
+                                              float* top_logprobs_dev);
 
 /* ---- NCCL plumbing for tensor parallelism (rank 0 makes the id, the host program
  * broadcasts it, every rank initialises) ---- */

@@ -1,0 +1,425 @@
+"""Paged 4-bit key/value cache: what is stored, and attention over it, against 64-bit restatements."""
+import numpy as np
+import pytest
+import torch
+
+import cortexsdr_b200 as cs
+from cortexsdr_b200 import _lib
+from tests import operator_refs as ref
+
+pytestmark = pytest.mark.gpu
+THETA = 1e6
+DTYPES = {"f32": (torch.float32, 0), "bf16": (torch.bfloat16, 1), "f16": (torch.float16, 2)}
+
+
+class Case:
+    """A ragged batch over a paged cache, with what each sequence holds."""
+
+    def __init__(self, ctx, lengths, fresh, kvh, hd, page, seed=0, dtype="f32", spare=0, tail=0, layers=1, ptr_pages=None):
+        self.rng = np.random.default_rng(seed)
+        self.ctx, self.lengths, self.fresh, self.kvh, self.hd, self.page, self.tail = ctx, lengths, fresh, kvh, hd, page, tail
+        self.tdtype, self.dtype = DTYPES[dtype]
+        n = len(lengths)
+        counts = [-(-max(a, 0) // page) for a in lengths]
+        self.per = max(1, max(counts)) + spare
+        self.n_pages = max(1, sum(counts))
+        order = self.rng.permutation(self.n_pages)
+        self.pages = np.full((n, self.per), -1, np.int32)
+        at = 0
+        for s, c in enumerate(counts):
+            self.pages[s, :c] = order[at:at + c]
+            at += c
+        self.cache = cs.KVCache(self.n_pages, page, kvh, hd, layers=layers, rope_theta=THETA, ctx=ctx)
+        self.k = [self.values((max(a, 0), kvh, hd)) for a in lengths]
+        self.v = [self.values((max(a, 0), kvh, hd)) for a in lengths]
+
+    def values(self, shape):
+        x = self.rng.normal(0, 1, shape) * (1 + 3 * (self.rng.random(shape[-2:]) < 0.05))
+        return torch.tensor(x, dtype=torch.float32).to(self.tdtype)
+
+    def batch(self, lengths, fresh, tail=0):
+        first = np.concatenate([[0], np.cumsum(fresh)]).astype(np.int32)
+        dev = [torch.tensor(a, dtype=torch.int32, device="cuda") for a in (first, lengths, self.pages)]
+        b = cs.KVBatch(len(lengths), int(first[-1]) + tail, *[t.data_ptr() for t in dev], self.per)
+        b.keep = dev
+        return b
+
+    def rows(self, parts, tail=0, fill=0.0):
+        x = torch.cat([p for p in parts if p.shape[0]] + [torch.full((tail, *parts[0].shape[1:]), fill, dtype=parts[0].dtype)])
+        return x.cuda().contiguous()
+
+    def store(self, rotate=False, layer=0):
+        """Everything into the cache, each sequence's tokens in two calls."""
+        for lo, hi in ((0, 2), (2, 3)):
+            a = [n * lo // 3 for n in self.lengths]
+            e = [n * hi // 3 for n in self.lengths]
+            b = self.batch(e, [y - x for x, y in zip(a, e)])
+            k, v = (self.rows([t[x:y] for t, x, y in zip(src, a, e)]) for src in (self.k, self.v))
+            torch.cuda.synchronize()
+            self.cache.append(b, k.data_ptr(), v.data_ptr(), self.dtype, rotate=rotate, layer=layer)
+            self.ctx.synchronize()
+
+    def held(self, rotated=False):
+        def f(t, turn):
+            x = t.to(torch.float64).numpy()
+            return ref.held(ref.rotate(x, np.arange(len(x)), THETA) if turn else x) if len(x) else x
+        return [f(t, rotated) for t in self.k], [f(t, False) for t in self.v]
+
+    def attend(self, q, qh, layer=0, **kw):
+        out = torch.full_like(q, 7.0)
+        torch.cuda.synchronize()
+        self.cache.attention(self.batch(self.lengths, self.fresh, self.tail), q.data_ptr(), self.dtype, qh, out.data_ptr(), layer=layer, **kw)
+        self.ctx.synchronize()
+        return out
+
+
+def close(out, want, tdtype, largest):
+    """fp32 arithmetic: a score's error is at most sum |q k| scale 2^-21 (two 11-bit halves of q, fp32 sums), here
+    under 64 * 16 * 2^-21 / 8 < 1e-4 of a weight for the loudest rows, an output that times the largest value; and
+    half a step of the output's type."""
+    half = 2.0 ** -24 if tdtype == torch.float32 else torch.finfo(tdtype).eps / 2
+    bound = half * np.abs(want) + 1e-4 * largest
+    err = np.abs(out.to(torch.float64).cpu().numpy() - want)
+    assert (err <= bound).all(), f"off by up to {np.nanmax(err - bound)} past the bound"
+    if tdtype == torch.float32:
+        # the errors of many terms do not all point one way: over all rows, fp32's own
+        assert np.linalg.norm(err) <= 4e-6 * np.linalg.norm(want) + 1e-30
+
+
+SHAPES = [
+    # lengths, new tokens, kv heads, query heads, head_dim, page
+    ([1], [1], 1, 1, 64, 16),
+    ([17], [1], 2, 14, 64, 16),
+    ([512], [1], 2, 14, 64, 64),
+    ([5, 64, 65, 1, 200], [1, 1, 1, 1, 1], 4, 4, 128, 64),
+    ([1024, 3, 700], [1, 1, 1], 8, 32, 128, 64),
+    ([130, 33], [1, 1], 2, 32, 256, 32),
+    ([5000], [1], 1, 8, 128, 128),
+    ([9, 100, 40], [9, 0, 40], 2, 6, 128, 16),
+    ([300, 77], [100, 77], 2, 8, 64, 32),
+    ([1000], [333], 1, 16, 128, 64),
+    ([70, 129], [70, 65], 3, 15, 256, 16),
+    ([2048, 513], [3, 17], 2, 8, 128, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,kvh,page", [(64, 3, 16), (128, 2, 64), (256, 1, 32)])
+def test_append_holds_what_the_definition_says(ctx, hd, kvh, page, dtype):
+    c = Case(ctx, [7, 0, 90, 33], [7, 0, 90, 33], kvh, hd, page, seed=hd, dtype=dtype)
+    qh = 5
+    q = [c.values((n, qh, hd)) for n in c.lengths]
+    b = c.batch(c.lengths, c.fresh)
+    dq, dk, dv = c.rows(q), c.rows(c.k), c.rows(c.v)
+    q_out = torch.empty_like(dq)
+    k_out, v_out = (torch.empty(dk.shape, dtype=torch.float32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    c.cache.append(b, dk.data_ptr(), dv.data_ptr(), c.dtype, q_ptr=dq.data_ptr(), q_heads=qh, q_out_ptr=q_out.data_ptr())
+    c.cache.read(b, k_out.data_ptr(), v_out.data_ptr())
+    ctx.synchronize()
+    k, v = c.held(rotated=True)
+    np.testing.assert_array_equal(k_out.cpu().numpy(), np.concatenate(k).astype(np.float32))
+    np.testing.assert_array_equal(v_out.cpu().numpy(), np.concatenate(v).astype(np.float32))
+    want = np.concatenate([ref.rotate(t.to(torch.float64).numpy(), np.arange(len(t)), THETA) for t in q])
+    half = torch.finfo(c.tdtype).eps / 2
+    assert (np.abs(q_out.to(torch.float64).cpu().numpy() - want) <= 1.01 * half * np.abs(want) + 1e-6).all()
+
+
+def test_append_at_far_positions(ctx):
+    n, far = 5, 100_000
+    c = Case(ctx, [far + n], [n], 1, 128, 64, seed=3)
+    k, v = c.values((n, 1, 128)).cuda(), c.values((n, 1, 128)).cuda()
+    b = c.batch([far + n], [n])
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    torch.cuda.synchronize()
+    c.cache.append(b, k.data_ptr(), v.data_ptr(), 0)
+    c.cache.read(b, ko.data_ptr(), vo.data_ptr())
+    ctx.synchronize()
+    want = ref.held(ref.rotate(k.cpu().numpy(), far + np.arange(n), THETA))
+    np.testing.assert_array_equal(ko.cpu().numpy(), want.astype(np.float32))
+
+
+def test_append_takes_strided_rows_and_queries_in_place(ctx):
+    c = Case(ctx, [40, 21], [40, 21], 2, 128, 16, seed=4, dtype="bf16")
+    qh, t = 4, 61
+    rows = c.values((t, qh + 4 + 3, 128)).cuda()       # q | k | v | padding
+    keep = rows.clone()
+    b = c.batch(c.lengths, c.fresh)
+    ko, vo = (torch.empty(t, 2, 128, device="cuda") for _ in range(2))
+    stride, es = rows.stride(0), 2
+    torch.cuda.synchronize()
+    c.cache.append(b, rows.data_ptr() + qh * 128 * es, rows.data_ptr() + (qh + 2) * 128 * es, 1, kv_stride=stride, q_ptr=rows.data_ptr(),
+                   q_stride=stride, q_heads=qh, q_out_ptr=rows.data_ptr(), q_out_stride=stride)
+    c.cache.read(b, ko.data_ptr(), vo.data_ptr())
+    ctx.synchronize()
+    pos = np.concatenate([np.arange(40), np.arange(21)])
+    x = keep.to(torch.float64).cpu().numpy()
+    np.testing.assert_array_equal(ko.cpu().numpy(), ref.held(ref.rotate(x[:, qh:qh + 2], pos, THETA)).astype(np.float32))
+    np.testing.assert_array_equal(vo.cpu().numpy(), ref.held(x[:, qh + 2:qh + 4]).astype(np.float32))
+    want = ref.rotate(x[:, :qh], pos, THETA)
+    assert (np.abs(rows[:, :qh].to(torch.float64).cpu().numpy() - want) <= 2.0 ** -8 * 1.01 * np.abs(want) + 1e-6).all()
+    assert torch.equal(rows[:, qh:], keep[:, qh:])
+
+
+def test_append_odd_element_offsets(ctx):
+    # operands that start between 16-byte boundaries, rows of an odd number of elements
+    for dtype in ("f32", "f16"):
+        c = Case(ctx, [19], [19], 1, 64, 16, seed=5, dtype=dtype)
+        room = torch.zeros(19 * 201 + 1, dtype=c.tdtype, device="cuda")
+        rows = room[1:].view(19, 201)
+        rows[:, :128] = c.values((19, 2, 64)).view(19, 128).cuda()
+        b = c.batch(c.lengths, c.fresh)
+        ko, vo = (torch.empty(19, 1, 64, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+        es = room.element_size()
+        c.cache.append(b, rows.data_ptr(), rows.data_ptr() + 64 * es, c.dtype, kv_stride=201, rotate=False)
+        c.cache.read(b, ko.data_ptr(), vo.data_ptr())
+        ctx.synchronize()
+        x = rows.to(torch.float64).cpu().numpy()
+        np.testing.assert_array_equal(ko.cpu().numpy()[:, 0], ref.held(x[:, :64]).astype(np.float32))
+        np.testing.assert_array_equal(vo.cpu().numpy()[:, 0], ref.held(x[:, 64:128]).astype(np.float32))
+
+
+def test_append_borders(ctx):
+    # constant groups, ties between codes, saturation, and values that are not finite
+    c = Case(ctx, [6], [6], 1, 64, 16)
+    k = np.zeros((6, 1, 64), np.float32)
+    k[0] = 1.25
+    k[1, 0] = np.arange(64) % 31 / 2.0                    # step 1: halves are ties
+    k[2, 0, 3] = 1e6
+    k[3, 0, 5] = np.nan
+    k[4, 0, 7] = -np.inf
+    k[5, 0] = np.linspace(-3e-7, 3e-7, 64)                # the step is a subnormal fp16 or nothing
+    dk = torch.tensor(k).cuda()
+    ko, vo = torch.empty_like(dk), torch.empty_like(dk)
+    b = c.batch([6], [6])
+    torch.cuda.synchronize()
+    c.cache.append(b, dk.data_ptr(), dk.data_ptr(), 0, rotate=False)
+    c.cache.read(b, ko.data_ptr(), vo.data_ptr())
+    ctx.synchronize()
+    np.testing.assert_array_equal(vo.cpu().numpy(), ref.held(k).astype(np.float32))
+    np.testing.assert_array_equal(ko.cpu().numpy(), vo.cpu().numpy())
+
+
+def test_append_touches_its_slots_only(ctx):
+    # idle sequences, rows behind the last, tokens without a place: nothing else changes
+    c = Case(ctx, [20, 33, 16], [20, 33, 16], 2, 64, 16, seed=6)
+    c.store()
+    whole = c.batch(c.lengths, c.lengths)
+    before = [torch.empty(sum(c.lengths), 2, 64, device="cuda") for _ in range(2)]
+    c.cache.read(whole, *[t.data_ptr() for t in before])
+    ctx.synchronize()
+    good = c.pages.copy()
+    c.pages[1, 2] = -1                       # sequence 1: position 32 has no place
+    c.pages[2, 0] = c.n_pages                # sequence 2: no such page
+    b = c.batch([20, 33, 16], [0, 2, 3], tail=4)
+    k, v = c.values((9, 2, 64)).cuda(), c.values((9, 2, 64)).cuda()
+    ko, vo = torch.full_like(k, 5.0), torch.full_like(v, 5.0)
+    torch.cuda.synchronize()
+    c.cache.append(b, k.data_ptr(), v.data_ptr(), 0, rotate=False)
+    c.cache.read(b, ko.data_ptr(), vo.data_ptr())
+    c.pages = good
+    after = [torch.empty_like(t) for t in before]
+    c.cache.read(whole, *[t.data_ptr() for t in after])
+    ctx.synchronize()
+    for old, new, src in zip(before, after, (k, v)):
+        want = old.cpu().numpy()
+        want[20 + 31] = ref.held(src[:1].cpu().numpy())[0]       # position 31 of sequence 1
+        np.testing.assert_array_equal(new.cpu().numpy(), want)
+    assert (ko[5:] == 5).all() and (vo[5:] == 5).all()           # rows of no sequence
+    assert (ko[1:5] == 0).all()                                  # rows without a place
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention_matches_the_definition(ctx, shape, dtype):
+    lengths, fresh, kvh, qh, hd, page = shape
+    c = Case(ctx, lengths, fresh, kvh, hd, page, seed=len(lengths) + qh, dtype=dtype, spare=2, tail=3)
+    c.store()
+    q = [c.values((n, qh, hd)) * 0.7 for n in fresh]
+    out = c.attend(c.rows(q, c.tail), qh)
+    k, v = c.held()
+    at = 0
+    for s, n in enumerate(fresh):
+        if n:
+            want = ref.attention(q[s].to(torch.float64).numpy(), k[s], v[s], lengths[s] - n + np.arange(n), hd ** -0.5)
+            close(out[at:at + n], want, c.tdtype, np.abs(v[s]).max())
+        at += n
+    assert (out[at:] == 7).all()             # rows behind the last sequence
+
+
+def test_attention_sees_what_has_a_place(ctx):
+    # a page that is not there inside a sequence, a length past the table, a length that is less than the new rows
+    c = Case(ctx, [100, 64, 2, 0], [1, 1, 5, 3], 2, 64, 16, seed=8)
+    c.store()
+    k, v = c.held()
+    qh = 6
+    q = [c.values((n, qh, 64)) for n in c.fresh]
+    c.pages[0, 2], c.pages[0, 4] = -1, c.n_pages + 5
+    c.lengths = [100, 64 + 3 * 16 * c.per, 2, 0]
+    out = c.attend(c.rows(q), qh).cpu().numpy()
+    keep = np.r_[0:32, 48:64, 80:100]
+    np.testing.assert_allclose(out[:1], ref.attention(q[0].numpy(), k[0][keep], v[0][keep], [len(keep) - 1], 0.125), rtol=0, atol=2e-5)
+    np.testing.assert_allclose(out[1:2], ref.attention(q[1].numpy(), k[1], v[1], [63], 0.125), rtol=0, atol=2e-5)
+    want = ref.attention(q[2].numpy(), k[2], v[2], [-3, -2, -1, 0, 1], 0.125)
+    np.testing.assert_allclose(out[2:7], want, rtol=0, atol=2e-5)
+    assert (out[2:5] == 0).all() and (out[7:] == 0).all()
+
+
+def test_attention_does_not_see_later_tokens(ctx):
+    # NaN and loud values behind a sequence's end, in the same pages
+    c = Case(ctx, [64], [64], 1, 128, 64, seed=9)
+    c.k[0][37:] = float("nan")
+    c.v[0][37:] = float("nan")
+    c.k[0][37, 0, :64] = 6e4
+    c.store()
+    k, v = c.held()
+    for n, length in ((1, 37), (5, 37), (37, 37)):
+        c.lengths, c.fresh = [length], [n]
+        q = [c.values((n, 8, 128))]
+        out = c.attend(c.rows(q), 8)
+        close(out, ref.attention(q[0].numpy(), k[0], v[0], length - n + np.arange(n), 128 ** -0.5), torch.float32, np.abs(v[0][:37]).max())
+    c.lengths, c.fresh = [40], [4]
+    out = c.attend(c.rows([c.values((4, 8, 128))]), 8)
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1:]).all()
+
+
+@pytest.mark.parametrize("vscale,qscale", [(1e-6, 1.0), (1e-3, 30.0), (2000.0, 1e-4), (1.0, 0.0)])
+def test_attention_keeps_its_precision_at_any_magnitude(ctx, vscale, qscale):
+    c = Case(ctx, [700], [2], 2, 128, 64, seed=10)
+    c.v[0] = c.v[0] * vscale
+    c.v[0][300:320] = c.v[0][300:320] * 20          # steps grow on the way
+    c.store()
+    q = [c.values((2, 8, 128)) * qscale]
+    out = c.attend(c.rows(q), 8).to(torch.float64).cpu().numpy()
+    k, v = c.held()
+    want = ref.attention(q[0].numpy(), k[0], v[0], [698, 699], 128 ** -0.5)
+    # sharp rows (|q| 30): a score of ~500 carries 2^-21 of itself
+    tol = 4e-6 if qscale < 10 else 1e-3
+    assert np.linalg.norm(out - want) <= tol * np.linalg.norm(want)
+
+
+def test_attention_strides_scale_and_layers(ctx):
+    c = Case(ctx, [90, 20], [3, 1], 2, 64, 16, seed=11, layers=3)
+    c.store(layer=2)
+    qh = 4
+    rows = c.values((4, qh + 2, 64)).cuda()
+    out = torch.full((4, qh + 1, 64), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    c.cache.attention(c.batch(c.lengths, c.fresh), rows.data_ptr(), 0, qh, out.data_ptr(), q_stride=(qh + 2) * 64, out_stride=(qh + 1) * 64,
+                      scale=0.3, layer=2)
+    ctx.synchronize()
+    k, v = c.held()
+    q = rows[:, :qh].cpu().numpy()
+    want = np.concatenate([ref.attention(q[:3], k[0], v[0], [87, 88, 89], 0.3), ref.attention(q[3:], k[1], v[1], [19], 0.3)])
+    close(out[:, :qh], want, torch.float32, 16.0)
+    assert (out[:, qh:] == 7).all()
+    zeros = c.attend(rows[:, :qh].contiguous(), qh, layer=0)       # nothing was stored there: zero keys and values
+    assert (zeros == 0).all()
+
+
+def test_attention_repeats_itself_and_follows_a_stream(ctx):
+    lengths = [3000, 11, 700, 64] * 5
+    c = Case(ctx, lengths, [1] * 20, 2, 128, 64, seed=12)
+    c.store()
+    q = c.rows([c.values((1, 16, 128)) for _ in lengths])
+    a, b = c.attend(q, 16), c.attend(q, 16)
+    assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    other = cs.Context(0, side.cuda_stream)
+    d = Case(other, lengths, [1] * 20, 2, 128, 64, seed=12)
+    d.store()
+    batch, out = d.batch(lengths, [1] * 20), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        x = torch.empty_like(q)
+        x.copy_(q)                           # the operator's input is made on its stream
+        d.cache.attention(batch, x.data_ptr(), 0, 16, out.data_ptr())
+        y = out * 2
+    side.synchronize()
+    assert torch.equal(y, a * 2)
+    d.cache.close()
+    other.close()
+
+
+def test_graph_replays_with_new_lengths(ctx):
+    side = torch.cuda.Stream()
+    own = cs.Context(0, side.cuda_stream)
+    c = Case(own, [150, 90], [1, 1], 2, 128, 16, seed=13)
+    qh = 8
+    b = c.batch([1, 1], [1, 1])
+    kv = [torch.empty(2, 2, 128, device="cuda") for _ in range(2)]
+    q, qr, out = (torch.empty(2, qh, 128, device="cuda") for _ in range(3))
+    torch.cuda.synchronize()
+
+    def step():
+        c.cache.append(b, kv[0].data_ptr(), kv[1].data_ptr(), 0, q_ptr=q.data_ptr(), q_heads=qh, q_out_ptr=qr.data_ptr())
+        c.cache.attention(b, qr.data_ptr(), 0, qh, out.data_ptr())
+
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            step()
+    queries = [c.values((150, qh, 128)), c.values((90, qh, 128))]
+    got = []
+    for i in range(150):
+        at = [i, min(i, 89)]
+        with torch.cuda.stream(side):
+            b.keep[1].copy_(torch.tensor([a + 1 for a in at], dtype=torch.int32))
+            for s in range(2):
+                kv[0][s].copy_(c.k[s][at[s]])
+                kv[1][s].copy_(c.v[s][at[s]])
+                q[s].copy_(queries[s][at[s]])
+            g.replay()
+            got.append(out.cpu())
+    k, v = c.held(rotated=True)
+    for s, n in ((0, 150), (1, 90)):
+        qq = ref.rotate(queries[s].numpy(), np.arange(n), THETA)
+        want = ref.attention(qq, k[s], v[s], np.arange(n), 128 ** -0.5)
+        close(torch.stack([got[i][s] for i in range(n)]), want, torch.float32, 16.0)
+    del g
+    c.cache.close()
+    own.close()
+
+
+def test_refusals(ctx, lib):
+    with pytest.raises(ValueError, match="power of two"):
+        cs.KVCache(4, 24, 1, 64, ctx=ctx)
+    with pytest.raises(cs.CompressionError, match="head_dim"):
+        cs.KVCache(4, 16, 1, 96, ctx=ctx)
+    with pytest.raises(ValueError, match="zero"):
+        cs.KVCache(0, 16, 1, 64, ctx=ctx)
+    with pytest.raises(ValueError, match="finite"):
+        cs.KVCache(4, 16, 1, 64, rope_theta=float("nan"), ctx=ctx)
+    c = Case(ctx, [16], [16], 2, 64, 16)
+    b = c.batch([16], [16])
+    x = torch.zeros(16, 4, 64, device="cuda")
+    p = x.data_ptr()
+    plain = cs.KVCache(1, 16, 2, 64, rope_theta=0.0, ctx=ctx)
+    with pytest.raises(ValueError, match="rotation"):
+        plain.append(b, p, p, 0)
+    for call, what in [
+        (lambda: c.cache.append(b, p, p, 3), "dtype"),
+        (lambda: c.cache.append(b, p, p, 0, layer=1), "layer"),
+        (lambda: c.cache.append(b, 0, p, 0), "null"),
+        (lambda: c.cache.append(b, p, p, 0, kv_stride=127), "stride"),
+        (lambda: c.cache.append(b, p, p, 0, q_ptr=p, q_heads=4), "q_out"),
+        (lambda: c.cache.append(b, p, p, 0, q_ptr=p, q_out_ptr=p), "head count"),
+        (lambda: c.cache.attention(b, p, 0, 3, p), "multiple"),
+        (lambda: c.cache.attention(b, p, 0, 0, p), "multiple"),
+        (lambda: c.cache.attention(b, p, 0, 4, 0), "null"),
+        (lambda: c.cache.attention(b, p, 0, 4, p, scale=float("inf")), "scale"),
+        (lambda: c.cache.attention(b, p, 7, 4, p), "dtype"),
+        (lambda: c.cache.read(b, p, 0), "null"),
+        (lambda: c.cache.read(cs.KVBatch(1, 16, 0, 0, 0, 1), p, p), "null array"),
+        (lambda: c.cache.read(cs.KVBatch(1, 16, p, p, p, 0), p, p), "range"),
+    ]:
+        with pytest.raises(ValueError, match=what):
+            call()
+    before = ctx.launch_count
+    c.cache.append(cs.KVBatch(0, 0, 0, 0, 0, 1), 0, 0, 0)          # nothing to do
+    c.cache.attention(cs.KVBatch(1, 0, 0, 0, 0, 1), 0, 0, 4, 0)
+    assert ctx.launch_count == before
+    assert lib.csdr_kv_cache_read_device_async(None, 0, b._ref, p, p) == _lib.ERR_INVALID_ARG

@@ -1,0 +1,169 @@
+"""Products with weights stored in 4 bits against the matrix their blocks stand for, in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import cortexsdr_b200 as cs
+from tests import operator_refs as ref
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"f32": (torch.float32, 0), "bf16": (torch.bfloat16, 1), "f16": (torch.float16, 2)}
+
+
+def run(w, x, layout, rows, ctx, bias=None, y_layout=None):
+    tdtype = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[x.dtype]
+    batch = x.shape[0]
+    y_layout = layout if y_layout is None else y_layout
+    xd = (x if layout else x.t()).contiguous().cuda()
+    y = torch.full((batch, rows) if y_layout else (rows, batch), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    w.matmul_device(xd.data_ptr(), tdtype, layout, batch, y.data_ptr(), y_layout, bias.data_ptr() if bias is not None else 0)
+    ctx.synchronize()
+    return (y if y_layout else y.t()).to(torch.float64).cpu().numpy()
+
+
+def check(y, x, dense):
+    """Each product of fp32 values carries at most 2^-22 (two 11-bit halves of x) + 2^-23 (the step), sums fp32: 2^-19
+    of sum |x w| covers widths to 2^14 summed in any order with room; on the whole fp32's own error."""
+    x = x.to(torch.float64).numpy()
+    want, room = x @ dense.T, np.abs(x) @ np.abs(dense).T
+    assert (np.abs(y - want) <= 2.0 ** -19 * room + 1e-30).all()
+    assert np.linalg.norm(y - want) <= 2e-6 * np.linalg.norm(want) + 1e-30
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,batch", [(1, 32, 1), (16, 128, 1), (17, 160, 2), (100, 896, 1), (333, 1056, 3), (64, 4096, 4),
+                                             (130, 2080, 5), (48, 96, 8), (1000, 512, 16), (33, 1280, 17), (50, 352, 40), (20, 64, 130)])
+def test_q4_0(ctx, rows, cols, batch, dtype):
+    rng = np.random.default_rng(rows)
+    payload, dense = ref.q4_weight(rng, rows, cols, "q4_0")
+    w = cs.Q4Weight.from_payload(payload, "q4_0", rows, cols, ctx)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32).to(DTYPES[dtype][0])
+    for layout in (0, 1):
+        check(run(w, x, layout, rows, ctx), x, dense)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,batch", [(1, 256, 1), (40, 256, 2), (129, 1024, 1), (31, 2304, 7), (512, 768, 16), (70, 512, 33),
+                                             (24, 4096, 3), (3, 11008, 9)])
+def test_q4_k(ctx, rows, cols, batch, dtype):
+    rng = np.random.default_rng(rows + 1)
+    payload, dense = ref.q4_weight(rng, rows, cols, "q4_k")
+    w = cs.Q4Weight.from_payload(payload, "q4_k", rows, cols, ctx)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32).to(DTYPES[dtype][0])
+    for layout in (0, 1):
+        check(run(w, x, layout, rows, ctx), x, dense)
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+def test_the_matrix_is_what_dequantisation_gives(ctx, fmt):
+    # one column at a time: the product is the stored weight itself, to fp32
+    rng = np.random.default_rng(5)
+    payload, dense = ref.q4_weight(rng, 37, 512, fmt)
+    w = cs.Q4Weight.from_payload(payload, fmt, 37, 512, ctx)
+    wide = cs.dequantize_inference(payload, fmt, ctx=ctx).astype(np.float64).reshape(37, 512)
+    for c0 in range(0, 512, 64):
+        eye = torch.zeros(64, 512)
+        eye[torch.arange(64), c0 + torch.arange(64)] = 1.0
+        y = run(w, eye, 1, 37, ctx)
+        # q4_k: minimum and step times code are one rounding each, as large as the larger of them
+        bound = 2.0 ** -22 * (np.abs(dense[:, c0:c0 + 64]).T + (0.2 if fmt == "q4_k" else 0.0))
+        assert (np.abs(y - wide[:, c0:c0 + 64].T) <= bound).all()
+
+
+def test_bias_layouts_and_untouched_rows(ctx):
+    rng = np.random.default_rng(6)
+    rows, cols, batch = 45, 224, 5
+    payload, dense = ref.q4_weight(rng, rows, cols, "q4_0")
+    w = cs.Q4Weight.from_payload(payload, "q4_0", rows, cols, ctx)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32)
+    bias = torch.tensor(rng.normal(0, 1, rows), dtype=torch.float32).cuda()
+    want = x.to(torch.float64).numpy() @ dense.T + bias.cpu().numpy()
+    for lx in (0, 1):
+        for ly in (0, 1):
+            np.testing.assert_allclose(run(w, x, lx, rows, ctx, bias, ly), want, rtol=0, atol=1e-5)
+    # the buffer around the result stays as it was, and operands need not start on 16 bytes
+    room = torch.full((rows * batch + 2,), 7.0, device="cuda")
+    xr = torch.zeros(batch * cols + 1, device="cuda")
+    xr[1:] = x.reshape(-1).cuda()
+    torch.cuda.synchronize()
+    w.matmul_device(xr.data_ptr() + 4, 0, 1, batch, room.data_ptr() + 4, 1)
+    ctx.synchronize()
+    assert room[0] == 7 and room[-1] == 7
+    np.testing.assert_allclose(room[1:-1].view(batch, rows).cpu().numpy(), want - bias.cpu().numpy(), rtol=0, atol=1e-5)
+
+
+@pytest.mark.parametrize("scale", [1e-20, 1e-6, 1e5, 1e20])
+def test_activations_of_any_magnitude(ctx, scale):
+    rng = np.random.default_rng(7)
+    payload, dense = ref.q4_weight(rng, 64, 768, "q4_k")
+    w = cs.Q4Weight.from_payload(payload, "q4_k", 64, 768, ctx)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = (torch.tensor(rng.normal(0, 1, (3, 768))) * scale).to(dtype)
+        x[1] = x[1] * 1e-3                   # rows of one call differ in magnitude
+        check(run(w, x, 1, 64, ctx), x, dense)
+    x = torch.zeros(2, 768)
+    assert (run(w, x, 1, 64, ctx) == 0).all()
+
+
+def test_what_is_not_finite_stays_with_its_token(ctx):
+    rng = np.random.default_rng(8)
+    payload, dense = ref.q4_weight(rng, 40, 512, "q4_0")
+    w = cs.Q4Weight.from_payload(payload, "q4_0", 40, 512, ctx)
+    x = torch.tensor(rng.normal(0, 1, (6, 512)), dtype=torch.float32)
+    clean = run(w, x, 1, 40, ctx)
+    x[2, 7], x[4, 300] = float("nan"), float("inf")
+    y = run(w, x, 1, 40, ctx)
+    keep = [0, 1, 3, 5]
+    np.testing.assert_array_equal(y[keep], clean[keep])
+    assert not np.isfinite(y[2]).any() and not np.isfinite(y[4][dense[:, 300] != 0]).any()
+
+
+def test_repeats_itself_and_captures(ctx):
+    rng = np.random.default_rng(9)
+    payload, dense = ref.q4_weight(rng, 4096, 4096, "q4_k")
+    side = torch.cuda.Stream()
+    own = cs.Context(0, side.cuda_stream)
+    w = cs.Q4Weight.from_payload(payload, "q4_k", 4096, 4096, own)
+    x = torch.tensor(rng.normal(0, 1, (2, 4096)), dtype=torch.float32).cuda()
+    y = torch.zeros(2, 4096, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        w.matmul_device(x.data_ptr(), 0, 1, 2, y.data_ptr(), 1)
+        side.synchronize()
+        first = y.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            w.matmul_device(x.data_ptr(), 0, 1, 2, y.data_ptr(), 1)
+        y.zero_()
+        g.replay()
+    side.synchronize()
+    assert torch.equal(y, first)
+    check(y.to(torch.float64).cpu().numpy(), x.cpu(), dense)
+    del g
+    w.close()
+    own.close()
+
+
+def test_refusals(ctx):
+    payload, _ = ref.q4_weight(np.random.default_rng(0), 4, 256, "q4_0")
+    make = lambda *a: cs.Q4Weight.from_payload(*a, ctx)
+    with pytest.raises(cs.CompressionError, match="format"):
+        make(payload, "q8_0", 4, 256)
+    with pytest.raises(cs.CompressionError, match="whole blocks"):
+        make(payload, "q4_0", 4, 250)
+    with pytest.raises(cs.CompressionError, match="size"):
+        make(payload, "q4_0", 5, 256)
+    with pytest.raises(cs.CompressionError, match="size"):
+        make(payload.reshape(-1)[:-1], "q4_0", 4, 256)
+    with pytest.raises(ValueError, match="range"):
+        make(payload, "q4_0", 0, 256)
+    w = make(payload, "q4_0", 4, 256)
+    x, y = torch.zeros(256, device="cuda"), torch.zeros(4, device="cuda")
+    for args, what in [((0, 0, 1, 1, y.data_ptr(), 1), "null"), ((x.data_ptr(), 5, 1, 1, y.data_ptr(), 1), "dtype"),
+                       ((x.data_ptr(), 0, 2, 1, y.data_ptr(), 1), "layout"), ((x.data_ptr(), 0, 1, 1, 0, 1), "null")]:
+        with pytest.raises(ValueError, match=what):
+            w.matmul_device(*args)
+    before = ctx.launch_count
+    w.matmul_device(x.data_ptr(), 0, 1, 0, y.data_ptr(), 1)
+    assert ctx.launch_count == before
