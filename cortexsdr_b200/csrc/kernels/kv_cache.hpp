@@ -57,7 +57,10 @@ struct KvAttend {
     uint32_t q_heads;
     float scale;
 };
-void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAttend& a);
+void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAttend& a,
+                         void* workspace);
+// Zeroed once by whoever makes it; launches leave the counters at its front at zero.
+size_t kv_attention_workspace(const csdr_context* ctx, uint32_t head_dim);
 
 }  // namespace csdr
 
@@ -66,7 +69,7 @@ struct csdr_kv_cache {
     uint32_t n_layers = 0, n_pages = 0, page_tokens = 0, kv_heads = 0, head_dim = 0;
     size_t layer_bytes = 0;
     csdr::KvView view;          // of layer 0
-    csdr::DevPtr data, freq;
+    csdr::DevPtr data, freq, workspace;
     csdr::KvView layer(uint32_t l) const {
         csdr::KvView v = view;
         v.base += static_cast<size_t>(l) * layer_bytes;

@@ -73,6 +73,8 @@ int csdr_kv_cache_create(csdr_context* ctx, uint32_t n_layers, uint32_t n_pages,
         c->data = std::make_shared<DeviceBuffer>(c->layer_bytes * n_layers, ctx->device);
         c->view.base = static_cast<uint8_t*>(c->data->ptr);
         CSDR_CUDA(cudaMemsetAsync(c->data->ptr, 0, c->data->bytes, ctx->stream));
+        c->workspace = std::make_shared<DeviceBuffer>(kv_attention_workspace(ctx, head_dim), ctx->device);
+        CSDR_CUDA(cudaMemsetAsync(c->workspace->ptr, 0, c->workspace->bytes, ctx->stream));
         if (rope_theta > 0.0f) {
             std::vector<double> freq(head_dim / 2);
             for (uint32_t i = 0; i < head_dim / 2; ++i) freq[i] = std::pow(static_cast<double>(rope_theta), -2.0 * i / head_dim);
@@ -156,7 +158,7 @@ int csdr_kv_cache_attention_device_async(csdr_kv_cache* c, uint32_t layer, const
         a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(c->head_dim));
         if (!b.n_tokens || !b.n_seqs) return;
         if (!q_dev || !out_dev) throw Error(CSDR_ERR_INVALID_ARG, "null argument");
-        launch_kv_attention(c->ctx, c->layer(layer), c->head_dim, b, dtype, a);
+        launch_kv_attention(c->ctx, c->layer(layer), c->head_dim, b, dtype, a, c->workspace->ptr);
     });
 }
 
