@@ -1,23 +1,25 @@
 // Causal grouped-query attention over the paged 4-bit cache (kv_cache.hpp).
 //   o = sum_t softmax_t(scale q . k_t) v_t,   k_t = minimum + step * code, over the tokens up to the row's own
 //
-// A decode step reads every cached byte once and does 4 head_dim flops a byte for each query head of a group:
-// the CUDA cores could not keep up with grouped heads, and widening codes is the other half of the work. So both products run
-// on mma.m16n8k16 with the codes themselves (-8 .. 7, exact in fp16) as the second operand:
-//   scores   sum over groups of step * (q . (code - 8)) + (minimum + 8 step) * (sum of q)
-//   output   sum over groups of (p step) . (code - 8) + sum p (minimum + 8 step)
-// Eight query rows fill the sixteen rows of a fragment: rows 0-7 are the fp16 roundings of q (or of p step), rows 8-15
-// what the rounding left, so that products carry 22 bits and the sums are fp32's; the two halves of a result
-// sit in one lane. A row's q is scaled by a power of two to use fp16's range, p step likewise by the
-// largest step met. tcgen05 would want the codes widened into shared memory first, which costs more than the
-// products here (16 of 320 issue slots a block are mma).
+// A decode step reads every cached byte once and does 4 head_dim flops a byte for each query head of a group: the
+// CUDA cores could not keep up with grouped heads, and they have the codes to widen. So both products run on
+// mma.m16n8k16 with the codes themselves as an operand: a code's bits, where they lie in a 16-bit word, are a
+// subnormal fp16 (code 2^-18), which the matrix units multiply exactly; widening is an AND a pair, and some shifts.
+//   scores   sum over groups of step * (q . code) + minimum * (sum of q)         q: 16 rows, eight fp16 roundings
+//            of query rows and eight of what the roundings left
+//   output   sum over groups of (p step) . (code - 8) + sum p (minimum + 8 step)   transposed, p step: 8 columns
+// Rounding and rest carry 22 bits, sums are fp32's. A row's q is scaled by a power of two to use fp16's range, p step
+// likewise by the largest step met. The 8 comes off in every piece (by one more product, of p step with eights): the
+// matrix units cut sums off instead of rounding them, and sums of one sign drift (1e-5 of an output over 5000 keys).
+// tcgen05 would want the codes widened into shared memory first, which costs more than the products here.
 //
-// Work is cut evenly, whatever the lengths: units are (sequence, tile of query rows, kv head), their length in 64 keys
+// Work is cut evenly, whatever the lengths: units are (sequence, tile of query rows, kv head), their length in 128 keys
 // is known on the device, and CTA c of G takes the c-th G-th of all of it. A unit that is cut leaves partial
 // (maximum, sum, output) pieces; the last CTA to arrive at it joins them, in the order of the keys. Nothing depends on the
 // host knowing lengths, so a captured call follows its sequences as they grow.
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "kv_cache.hpp"
 #include "op_common.cuh"
@@ -26,7 +28,10 @@ namespace csdr {
 
 namespace {
 
-constexpr uint32_t kWarps = 4, kThreads = kWarps * 32, kBlockKeys = 64;
+constexpr uint32_t kWarps = 4, kThreads = kWarps * 32, kPiece = 32, kBlockKeys = kWarps * kPiece;
+constexpr float kSlack = 6.0f;
+template <int HD>
+constexpr uint32_t kPitch = HD + 4;      // of a row of outputs with its maximum and sum
 constexpr uint32_t kMostPerSm = 4;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -54,6 +59,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// With nothing to add to.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 __device__ __forceinline__ float power_of_two(int n) { return __int_as_float((n + 127) << 23); }   // -126 <= n <= 127
 
 __device__ __forceinline__ float ex2(float x) {
@@ -62,37 +74,59 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Eight codes of a word, less 8, as four fp16 pairs, bits (4n, 4n + 16) into pair n: the code's bits below a
-// leading one give 1024 + code (or 1024 + 16 code), the rest is one packed operation. Less 8, because the matrix units
-// cut their sums off instead of rounding them: what has one sign drifts (1e-5 of an output over 5000 keys).
-__device__ __forceinline__ uint32_t pair_or(uint32_t w, uint32_t mask) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, 0x64006400, 0xEA;" : "=r"(r) : "r"(w), "r"(mask));   // (w & mask) | 0x6400'6400
+// Eight codes of a word as four pairs of subnormal fp16 (code n of either half into pair n), see kv_cache.hpp for the bits.
+// FINE: all times 2^-18. Else pairs 1 and 3 are left four bits lower, times 2^-22: two operations less, but the matrix
+// units line sums up by exponents, where a subnormal counts as the smallest normal number, so four bits of the sums
+// go (2e-6 of an output against 3e-7) - for results that are rounded to 16 bits.
+template <bool FINE>
+__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t (&r)[4]) {
+    const uint32_t v = __byte_perm(w, 0u, 0x2301);
+    r[0] = w & 0x03C003C0u;
+    r[1] = FINE ? w << 4 & 0x03C003C0u : w & 0x003C003Cu;
+    r[2] = v & 0x03C003C0u;
+    r[3] = FINE ? w >> 4 & 0x03C003C0u : v & 0x003C003Cu;
+}
+constexpr int kCodeShift = 18;
+constexpr uint32_t kEights = 0x02000200u;      // code 8, twice
+
+// Pairs of fp32 values, one packed operation each.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
     return r;
 }
-__device__ __forceinline__ uint32_t low_code(uint32_t r) {
-    const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x6408)));   // r - 1032
-    return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
 }
-__device__ __forceinline__ uint32_t high_code(uint32_t r) {
-    const __half2 v = __hfma2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x2C00)), __half2half2(__ushort_as_half(0xD480)));
-    return *reinterpret_cast<const uint32_t*>(&v);   // r / 16 - 72
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
 }
-__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t (&r)[4]) {
-    const uint32_t v = w >> 8;
-    r[0] = low_code(pair_or(w, 0x000F000Fu));
-    r[1] = high_code(pair_or(w, 0x00F000F0u));
-    r[2] = low_code(pair_or(v, 0x000F000Fu));
-    r[3] = high_code(pair_or(v, 0x00F000F0u));
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
+__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
 // Two fp32 values as a pair of fp16 roundings and a pair of what they left.
-__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
+__device__ __forceinline__ void split(f32x2 v, uint32_t& hi, uint32_t& lo) {
+    const float2 x = unpack2(v);
+    const __half2 h = __floats2half2_rn(x.x, x.y);
     const float2 back = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - back.x, y - back.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
+    const float2 rest = unpack2(fma2(pack2(back.x, back.y), pack2(-1.0f, -1.0f), v));
+    hi = bits_of(h);
+    lo = bits_of(__floats2half2_rn(rest.x, rest.y));
 }
 
 struct AttnParams {
@@ -101,7 +135,7 @@ struct AttnParams {
     KvAttend a;
     uint32_t group;          // query heads of a kv head
     uint32_t vec;            // q rows start on 16 bytes
-    float* part;             // [CTA][2][rows][HD + 2]
+    float* part;             // [CTA][2][rows][HD + 4]
     uint32_t* counters;      // [CTA]: arrivals at the unit that starts in a CTA's share and is cut
     int* status;
     uint32_t spin;
@@ -113,7 +147,7 @@ struct Seq {
     int64_t cap;             // keys that its table can hold
     uint32_t row0, n_new, tiles;
     uint32_t pair_weight, mid_weight;
-    // blocks of 64 keys that a tile of rows sees; at least one, so that rows that see nothing are written too
+    // blocks of 128 keys that a tile of rows sees; at least one, so that rows that see nothing are written too
     template <uint32_t TILE>
     __device__ __forceinline__ int64_t keys(uint32_t tile, uint32_t group) const {
         const uint32_t last = min(n_new - 1u, static_cast<uint32_t>((static_cast<uint64_t>(TILE) * (tile + 1u) - 1u) / group));
@@ -147,16 +181,21 @@ struct Seq {
     __device__ __forceinline__ uint64_t head_weight() const { return static_cast<uint64_t>(tiles / 2u) * pair_weight + mid_weight; }
 };
 
-// One warp's eight query rows: fragments, running maxima and sums, outputs.
+// One warp's eight query rows: fragments, running maxima and sums, outputs. Lane (g, t) = (lane / 4, lane % 4) has the
+// scores of row g for keys 2t, 2t + 1 of every eight, and the outputs of rows 2t, 2t + 1 for values 64 u + 8 g .. + 7.
 template <typename T, int HD>
 struct Rows {
-    static constexpr uint32_t W = HD / 32, G = HD / 64, NT = HD / 8;
+    static constexpr uint32_t W = HD / 32, G = HD / 64;
+    static constexpr bool kOnce = std::is_same<T, __nv_bfloat16>::value, kFine = std::is_same<T, float>::value;
+    static constexpr float kOdd = kFine ? 1.0f : 16.0f;      // odd pairs of codes count one in kOdd
     static constexpr bool kShared = HD > 128;      // q fragments in shared memory: the registers go to the outputs
+    static constexpr uint32_t kMetaBytes = 2u * G * 16u * 16u;      // of a piece, widened
     uint32_t q[kShared ? 1 : W * 2][4];
-    float o[NT][4];
-    float om[G], sum_q[G];
-    float factor, m, l, escale;
-    uint32_t vmax;
+    float o[G][4][4];    // tile n of a group: values 8 g + n (rows 2t, 2t + 1), 8 g + 4 + n (rows 2t, 2t + 1)
+    f32x2 om[G], l;      // over even and odd keys
+    float sum_q[G];
+    float factor, m, escale;
+    uint32_t vmax;      // the largest step of the values so far, as bits
     int32_t limit;      // keys that this lane's row sees
     int32_t least;      // the fewest that one of the warp's rows sees, the most
     int32_t most;
@@ -198,24 +237,28 @@ struct Rows {
             }
         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-        // 2^e above the largest |q|: q 2^(15 - e) < 2^15, exact but for the last bits of what is 2^-24 of the largest
-        const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -100), 128) : 15;
-        const float up = power_of_two(15 - e), k = p.a.scale * 1.4426950408889634f;
-        factor = k * power_of_two(e - 15);
+        // 2^e above the largest |q|: q 2^(top - e) < 2^15 (and sixteen times that), exact but for the last bits of what is
+        // 2^-20 of the largest
+        constexpr int kTop = kFine ? 15 : 11;
+        const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : kTop;
+        // the scale's sign goes with q: the largest score / factor is the largest score
+        const float up = copysignf(power_of_two(kTop - e), p.a.scale);
+        factor = fabsf(p.a.scale) * 1.4426950408889634f * power_of_two(min(e - kTop + kCodeShift, 127));
 #pragma unroll
         for (uint32_t g = 0; g < G; ++g) sum_q[g] = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < W; ++w) {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) {
-                sum_q[w / 2u] += x[w][i];
                 x[w][i] *= up;
+                sum_q[w / 2u] += x[w][i];
             }
 #pragma unroll
             for (uint32_t h = 0; h < 2u; ++h) {
+                // values 2h, 2h + 4 meet even pairs of codes, 2h + 1, 2h + 5 odd ones
                 uint32_t f[4];
-                split(x[w][2 * h], x[w][2 * h + 4], f[0], f[1]);
-                split(x[w][2 * h + 1], x[w][2 * h + 5], f[2], f[3]);
+                split(pack2(x[w][2 * h], x[w][2 * h + 4]), f[0], f[1]);
+                split(pack2(x[w][2 * h + 1] * kOdd, x[w][2 * h + 5] * kOdd), f[2], f[3]);
                 if constexpr (kShared) {
                     shared[(w * 2u + h) * 32u + lane] = make_uint4(f[0], f[1], f[2], f[3]);
                 } else {
@@ -228,187 +271,259 @@ struct Rows {
         for (uint32_t g = 0; g < G; ++g) {
             sum_q[g] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[g], 1);
             sum_q[g] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[g], 2);
-            sum_q[g] *= k;
-            om[g] = 0.0f;
+            sum_q[g] *= power_of_two(-kCodeShift);
+            om[g] = pack2(0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t n = 0; n < 4u; ++n)
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; ++j) o[g][n][j] = 0.0f;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < NT; ++i)
-#pragma unroll
-            for (uint32_t j = 0; j < 4u; ++j) o[i][j] = 0.0f;
         m = -FLT_MAX;
-        l = 0.0f;
+        l = pack2(0.0f, 0.0f);
         escale = 1.0f;
         vmax = 0;
         if constexpr (kShared) __syncwarp();
     }
 
-    // Sixteen keys from `tok0` on, in shared memory at `block`.
-    __device__ __forceinline__ void keys16(const uint8_t* block, int32_t tok0, bool valid, uint32_t lane, const uint4* shared) {
-        const uint32_t g = lane >> 2, t = lane & 3u;
-        float sc[4];
-#pragma unroll
-        for (uint32_t nt = 0; nt < 2u; ++nt) {
-            uint32_t w[W];
-            const uint8_t* row = block + (8u * nt + g) * (HD / 2) + t * (HD / 8);
-            if constexpr (W == 2) {
-                const uint2 v = *reinterpret_cast<const uint2*>(row);
-                w[0] = v.x;
-                w[1] = v.y;
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < W; i += 4u) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(row + 4u * i);
-                    w[i] = v.x;
-                    w[i + 1] = v.y;
-                    w[i + 2] = v.z;
-                    w[i + 3] = v.w;
-                }
-            }
-            uint32_t meta[2 * G];
-            load_meta(block + 16u * HD + (8u * nt + 2u * t) * G * 4u, meta);
-            float s0 = 0.0f, s1 = 0.0f, n0 = 0.0f, n1 = 0.0f;
-#pragma unroll
-            for (uint32_t gq = 0; gq < G; ++gq) {
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (uint32_t i = 0; i < 2u; ++i) {
-                    uint32_t r[4];
-                    widen_codes(w[2u * gq + i], r);
-#pragma unroll
-                    for (uint32_t h = 0; h < 2u; ++h) {
-                        if constexpr (kShared) {
-                            const uint4 f = shared[((2u * gq + i) * 2u + h) * 32u + lane];
-                            mma16816(acc, f.x, f.y, f.z, f.w, r[2 * h], r[2 * h + 1]);
-                        } else {
-                            const uint32_t* f = q[(2u * gq + i) * 2u + h];
-                            mma16816(acc, f[0], f[1], f[2], f[3], r[2 * h], r[2 * h + 1]);
-                        }
-                    }
-                }
-                const float2 m0 = __half22float2(*reinterpret_cast<const __half2*>(&meta[gq]));
-                const float2 m1 = __half22float2(*reinterpret_cast<const __half2*>(&meta[G + gq]));
-                s0 = fmaf(m0.x, acc[0] + acc[2], s0);
-                s1 = fmaf(m1.x, acc[1] + acc[3], s1);
-                n0 = fmaf(fmaf(8.0f, m0.x, m0.y), sum_q[gq], n0);
-                n1 = fmaf(fmaf(8.0f, m1.x, m1.y), sum_q[gq], n1);
-            }
-            sc[2 * nt] = fmaf(s0, factor, n0);
-            sc[2 * nt + 1] = fmaf(s1, factor, n1);
-        }
-        uint32_t vm[2][2 * G];
-        load_meta(block + 17u * HD + (2u * t) * G * 4u, vm[0]);
-        load_meta(block + 17u * HD + (8u + 2u * t) * G * 4u, vm[1]);
-        if (!valid || tok0 + 16 > least) {
-            // keys that a row does not see weigh nothing, whatever lies there
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                const int32_t tok = tok0 + static_cast<int32_t>(8u * (i >> 1) + 2u * t + (i & 1u));
-                if (!valid || tok >= limit) {
-                    sc[i] = -INFINITY;
-#pragma unroll
-                    for (uint32_t gq = 0; gq < G; ++gq) vm[i >> 1][(i & 1u) * G + gq] = 0u;
-                }
-            }
-        }
-        float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        uint32_t big = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 2u; ++i)
-#pragma unroll
-            for (uint32_t j = 0; j < 2u * G; ++j) big = __vmaxu2(big, vm[i][j] & 0xFFFFu);
-        big = __reduce_max_sync(0xFFFFFFFFu, big);
-        if (__any_sync(0xFFFFFFFFu, top > m) || big > vmax) {
-            const float next = fmaxf(m, top), f = ex2(m - next);
-            m = next;
-            l *= f;
-#pragma unroll
-            for (uint32_t gq = 0; gq < G; ++gq) om[gq] *= f;
-            float both = f;
-            if (big > vmax) {
-                // p step 2^(14 - exponent of the largest step) < 2^15
-                vmax = big;
-                const float st = __half2float(__ushort_as_half(static_cast<unsigned short>(big)));
-                const float next_scale = power_of_two(14 - ilogbf(st));
-                both = f * (next_scale / escale);
-                escale = next_scale;
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < NT; ++i)
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) o[i][j] *= both;
-        }
-        float p[4], pe[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            p[i] = ex2(sc[i] - m);
-            pe[i] = p[i] * escale;
-        }
-        l += (p[0] + p[1]) + (p[2] + p[3]);
-        const uint8_t* v0 = block + 8u * HD + t * HD + g * (HD / 8);
-        const uint8_t* v1 = v0 + 4u * HD;
-#pragma unroll
-        for (uint32_t u = 0; u < G; ++u) {
-            float2 s[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                s[i] = __half22float2(*reinterpret_cast<const __half2*>(&vm[i >> 1][(i & 1u) * G + u]));
-                om[u] = fmaf(p[i], fmaf(8.0f, s[i].x, s[i].y), om[u]);
-            }
-            uint32_t a0, a1, a2, a3;
-            split(pe[0] * s[0].x, pe[1] * s[1].x, a0, a1);
-            split(pe[2] * s[2].x, pe[3] * s[3].x, a2, a3);
-            const uint2 w0 = *reinterpret_cast<const uint2*>(v0 + 8u * u), w1 = *reinterpret_cast<const uint2*>(v1 + 8u * u);
-#pragma unroll
-            for (uint32_t x = 0; x < 2u; ++x) {
-                uint32_t r0[4], r1[4];
-                widen_codes(x ? w0.y : w0.x, r0);
-                widen_codes(x ? w1.y : w1.x, r1);
-#pragma unroll
-                for (uint32_t n = 0; n < 4u; ++n) mma16816(o[u * 8u + x * 4u + n], a0, a1, a2, a3, r0[n], r1[n]);
-            }
-        }
-    }
-    static __device__ __forceinline__ void load_meta(const uint8_t* from, uint32_t (&m)[2 * G]) {
-        if constexpr (G == 1) {
-            const uint2 v = *reinterpret_cast<const uint2*>(from);
-            m[0] = v.x;
-            m[1] = v.y;
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 2u * G; i += 4u) {
-                const uint4 v = *reinterpret_cast<const uint4*>(from + 4u * i);
-                m[i] = v.x;
-                m[i + 1] = v.y;
-                m[i + 2] = v.z;
-                m[i + 3] = v.w;
-            }
-        }
+    // A value of row 2t and of row 2t + 1, from the lanes that have the rows.
+    static __device__ __forceinline__ float2 of_columns(float v, uint32_t lane) {
+        const uint32_t from = 8u * (lane & 3u);
+        return make_float2(__shfl_sync(0xFFFFFFFFu, v, from), __shfl_sync(0xFFFFFFFFu, v, from + 4u));
     }
 
-    // Row g's (maximum, sum) and its output before the division, to `to`: [row][HD + 2].
-    __device__ __forceinline__ void store(float* to, uint32_t lane) {
+    // 32 keys from `tok0` on, in shared memory at `block` (two blocks of sixteen); bit i of `there`: block i has a page.
+    // `meta`: the warp's, for steps and minima as pairs of fp32 over neighbouring tokens.
+    __device__ __forceinline__ void keys32(const uint8_t* block, int32_t tok0, uint32_t there, uint32_t lane, const uint4* shared, uint8_t* meta) {
         const uint32_t g = lane >> 2, t = lane & 3u;
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-        float* row = to + g * (HD + 2u);
-        const float down = 1.0f / escale;
+        const bool edge = there != 3u || tok0 + 32 > least;
+        // ---- steps and minima: a lane widens a pair of tokens of the keys' groups (lanes 0-15) or of the values' ----
+        uint32_t big = 0;
+        {
+            const uint32_t pr = lane & 15u, of_values = lane >> 4;
+            const uint8_t* from = block + (pr >> 3) * (18u * HD) + (16u + of_values) * HD + (pr & 7u) * 8u;
+            const float mid = of_values ? 8.0f : 0.0f;
 #pragma unroll
-        for (uint32_t u = 0; u < G; ++u) {
-            om[u] += __shfl_xor_sync(0xFFFFFFFFu, om[u], 1);
-            om[u] += __shfl_xor_sync(0xFFFFFFFFu, om[u], 2);
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) {
-                const float(&c)[4] = o[u * 8u + i];
-                row[64u * u + 16u * t + i] = fmaf(c[0] + c[2], down, om[u]);
-                row[64u * u + 16u * t + 8u + i] = fmaf(c[1] + c[3], down, om[u]);
+            for (uint32_t u = 0; u < G; ++u) {
+                uint2 w = *reinterpret_cast<const uint2*>(from + 64u * u);
+                if (edge && of_values) {     // nothing of what lies behind the last key that is seen
+                    const int32_t tok = tok0 + static_cast<int32_t>(2u * pr);
+                    const bool gone = !(there >> (pr >> 3) & 1u);
+                    if (gone || tok >= most) w.x = 0u;
+                    if (gone || tok + 1 >= most) w.y = 0u;
+                }
+                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+                const float2 c = unpack2(fma2(pack2(mid, mid), pack2(a.y, b.y), pack2(a.x, b.x)));
+                *reinterpret_cast<float4*>(meta + ((of_values * G + u) * 16u + pr) * 16u) = make_float4(a.y, b.y, c.x, c.y);
+                if (of_values) big = max(big, max(__float_as_uint(a.y), __float_as_uint(b.y)));
             }
         }
-        if (t == 0) {
-            row[HD] = m;
-            row[HD + 1] = l;
+        __syncwarp();
+        // ---- scores ----
+        f32x2 sc[4];             // scores / factor
+#pragma unroll
+        for (uint32_t gq = 0; gq < G; ++gq) {
+            float acc[4][4];
+            uint2 w[4];
+#pragma unroll
+            for (uint32_t nt = 0; nt < 4u; ++nt)
+                w[nt] = *reinterpret_cast<const uint2*>(block + (nt >> 1) * (18u * HD) + (8u * (nt & 1u) + g) * (HD / 2) + t * (HD / 8) + 8u * gq);
+#pragma unroll
+            for (uint32_t i = 0; i < 2u; ++i) {
+                uint32_t f[2][4];
+#pragma unroll
+                for (uint32_t h = 0; h < 2u; ++h) {
+                    if constexpr (kShared) {
+                        const uint4 v = shared[((2u * gq + i) * 2u + h) * 32u + lane];
+                        f[h][0] = v.x;
+                        f[h][1] = v.y;
+                        f[h][2] = v.z;
+                        f[h][3] = v.w;
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; ++j) f[h][j] = q[(2u * gq + i) * 2u + h][j];
+                    }
+                }
+#pragma unroll
+                for (uint32_t nt = 0; nt < 4u; ++nt) {
+                    uint32_t r[4];
+                    widen_codes<kFine>(i ? w[nt].y : w[nt].x, r);
+                    if (i == 0u) mma16816_first(acc[nt], f[0][0], f[0][1], f[0][2], f[0][3], r[0], r[1]);
+                    else mma16816(acc[nt], f[0][0], f[0][1], f[0][2], f[0][3], r[0], r[1]);
+                    mma16816(acc[nt], f[1][0], f[1][1], f[1][2], f[1][3], r[2], r[3]);
+                }
+            }
+            const f32x2 sq = pack2(sum_q[gq], sum_q[gq]);
+#pragma unroll
+            for (uint32_t nt = 0; nt < 4u; ++nt) {
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(meta + (gq * 16u + 4u * nt + t) * 16u);     // steps, minima
+                const f32x2 low = gq ? fma2(v.y, sq, sc[nt]) : mul2(v.y, sq);
+                sc[nt] = fma2(v.x, add2(pack2(acc[nt][0], acc[nt][1]), pack2(acc[nt][2], acc[nt][3])), low);
+            }
         }
+        if (edge) {
+            // keys that a row does not see weigh nothing, whatever lies there
+#pragma unroll
+            for (uint32_t nt = 0; nt < 4u; ++nt) {
+                float2 v = unpack2(sc[nt]);
+                const int32_t tok = tok0 + static_cast<int32_t>(8u * nt + 2u * t);
+                const bool gone = !(there >> (nt >> 1) & 1u);
+                if (gone || tok >= limit) v.x = -INFINITY;
+                if (gone || tok + 1 >= limit) v.y = -INFINITY;
+                sc[nt] = pack2(v.x, v.y);
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t nt = 0; nt < 4u; ++nt) {
+            const float2 v = unpack2(sc[nt]);
+            top = fmaxf(top, fmaxf(v.x, v.y));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2)) * factor;
+        // The maximum follows in steps: weights may reach 2^kSlack before outputs are scaled anew
+        if (__any_sync(0xFFFFFFFFu, top > m + kSlack || big > vmax)) {
+            const float next = fmaxf(m, top), f = ex2(m - next);
+            m = next;
+            l = mul2(l, pack2(f, f));
+#pragma unroll
+            for (uint32_t u = 0; u < G; ++u) om[u] = mul2(om[u], pack2(f, f));
+            float down = 1.0f;
+            big = __reduce_max_sync(0xFFFFFFFFu, big);
+            if (big > vmax) {
+                // weight * step < 2^(kSlack + 1 + exponent of the largest step) -> below 2^15
+                vmax = big;
+                const float next_scale = power_of_two(14 - static_cast<int>(kSlack) - ilogbf(__uint_as_float(big)));
+                down = next_scale / escale;
+                escale = next_scale;
+            }
+            const float2 fc = of_columns(f, lane);
+            const f32x2 both = pack2(fc.x * down, fc.y * down);
+#pragma unroll
+            for (uint32_t u = 0; u < G; ++u)
+#pragma unroll
+                for (uint32_t n = 0; n < 4u; ++n) scale_tile(o[u][n], both);
+        }
+        f32x2 p[4], pe[4];
+        const f32x2 fac = pack2(factor, factor), less = pack2(-m, -m), es = pack2(escale, escale);
+#pragma unroll
+        for (uint32_t nt = 0; nt < 4u; ++nt) {
+            const float2 v = unpack2(fma2(sc[nt], fac, less));
+            p[nt] = pack2(ex2(v.x), ex2(v.y));
+            pe[nt] = mul2(p[nt], es);
+            l = add2(l, p[nt]);
+        }
+        // ---- outputs ----
+#pragma unroll
+        for (uint32_t u = 0; u < G; ++u) {
+            uint32_t hi[4], lo[4];
+            float eight[4];
+#pragma unroll
+            for (uint32_t nt = 0; nt < 4u; ++nt) {
+                ulonglong2 v = *reinterpret_cast<const ulonglong2*>(meta + ((G + u) * 16u + 4u * nt + t) * 16u);     // steps, minima + 8 steps
+                if (edge) {
+                    const int32_t tok = tok0 + static_cast<int32_t>(8u * nt + 2u * t);
+                    float2 st = unpack2(v.x), mn = unpack2(v.y);
+                    if (tok >= limit) st.x = mn.x = 0.0f;
+                    if (tok + 1 >= limit) st.y = mn.y = 0.0f;
+                    v.x = pack2(st.x, st.y);
+                    v.y = pack2(mn.x, mn.y);
+                }
+                om[u] = fma2(p[nt], v.y, om[u]);
+                const f32x2 w = mul2(pe[nt], v.x);
+                if constexpr (kOnce) {       // bf16 outputs round eight times as coarsely as fp16 weights
+                    const float2 x = unpack2(w);
+                    hi[nt] = bits_of(__floats2half2_rn(x.x, x.y));
+                } else {
+                    split(w, hi[nt], lo[nt]);
+                }
+            }
+            mma16816_first(eight, kEights, kEights, kEights, kEights, hi[0], hi[1]);
+            mma16816(eight, kEights, kEights, kEights, kEights, hi[2], hi[3]);
+            if constexpr (!kOnce) {
+                mma16816(eight, kEights, kEights, kEights, kEights, lo[0], lo[1]);
+                mma16816(eight, kEights, kEights, kEights, kEights, lo[2], lo[3]);
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < 2u; ++b) {
+                const uint8_t* v0 = block + b * (18u * HD) + 8u * HD + t * HD + g * (HD / 8) + 8u * u;
+                const uint2 w0 = *reinterpret_cast<const uint2*>(v0), w1 = *reinterpret_cast<const uint2*>(v0 + 4u * HD);
+                uint32_t r0[4], r1[4], r2[4], r3[4];
+                widen_codes<kFine>(w0.x, r0);
+                widen_codes<kFine>(w0.y, r1);
+                widen_codes<kFine>(w1.x, r2);
+                widen_codes<kFine>(w1.y, r3);
+#pragma unroll
+                for (uint32_t n = 0; n < 4u; ++n) {
+                    mma16816(o[u][n], r0[n], r1[n], r2[n], r3[n], hi[2u * b], hi[2u * b + 1u]);
+                    if constexpr (!kOnce) mma16816(o[u][n], r0[n], r1[n], r2[n], r3[n], lo[2u * b], lo[2u * b + 1u]);
+                }
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < 4u; ++n) {
+                const float times = n & 1u ? -1.0f / kOdd : -1.0f;
+                const f32x2 e = pack2(eight[0], eight[1]), k = pack2(times, times);
+                add_tile(o[u][n], e, k);
+            }
+        }
+    }
+    static __device__ __forceinline__ void scale_tile(float (&c)[4], f32x2 f) {
+        const float2 a = unpack2(mul2(pack2(c[0], c[1]), f)), b = unpack2(mul2(pack2(c[2], c[3]), f));
+        c[0] = a.x;
+        c[1] = a.y;
+        c[2] = b.x;
+        c[3] = b.y;
+    }
+    static __device__ __forceinline__ void add_tile(float (&c)[4], f32x2 e, f32x2 k) {
+        const float2 a = unpack2(fma2(e, k, pack2(c[0], c[1]))), b = unpack2(fma2(e, k, pack2(c[2], c[3])));
+        c[0] = a.x;
+        c[1] = a.y;
+        c[2] = b.x;
+        c[3] = b.y;
+    }
+
+    // Calls out(row, value of the head, eight values) with the outputs before the division, for rows 2t and 2t + 1, and
+    // row(row, maximum, sum) once for each row.
+    template <typename Out, typename Row>
+    __device__ __forceinline__ void finish(uint32_t lane, Out&& out, Row&& row) {
+        const uint32_t g = lane >> 2, t = lane & 3u;
+        auto all = [](f32x2 v) {
+            const float2 e = unpack2(v);
+            float x = e.x + e.y;
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+            return x + __shfl_xor_sync(0xFFFFFFFFu, x, 2);
+        };
+        const float sum = all(l), down = power_of_two(kCodeShift) / escale;
+        const float2 sums = of_columns(sum, lane);
+        if (t == 0) row(g, m, sum);
+#pragma unroll
+        for (uint32_t u = 0; u < G; ++u) {
+            const float2 mins = of_columns(all(om[u]), lane);
+            float v[2][8];
+#pragma unroll
+            for (uint32_t n = 0; n < 4u; ++n) {
+                const float d = n & 1u ? down * kOdd : down;
+                v[0][n] = fmaf(o[u][n][0], d, mins.x);
+                v[1][n] = fmaf(o[u][n][1], d, mins.y);
+                v[0][4 + n] = fmaf(o[u][n][2], d, mins.x);
+                v[1][4 + n] = fmaf(o[u][n][3], d, mins.y);
+            }
+            out(2u * t, 64u * u + 8u * g, v[0], sums.x);
+            out(2u * t + 1u, 64u * u + 8u * g, v[1], sums.y);
+        }
+    }
+    // Row r's output before the division, maximum and sum, to `to`: [row][HD + 4].
+    __device__ __forceinline__ void store(float* to, uint32_t lane) {
+        finish(
+            lane,
+            [&](uint32_t r, uint32_t d, const float(&v)[8], float) {
+                float4* at = reinterpret_cast<float4*>(to + r * kPitch<HD> + d);
+                at[0] = make_float4(v[0], v[1], v[2], v[3]);
+                at[1] = make_float4(v[4], v[5], v[6], v[7]);
+            },
+            [&](uint32_t r, float top, float sum) {
+                to[r * kPitch<HD> + HD] = top;
+                to[r * kPitch<HD> + HD + 1] = sum;
+            });
     }
 };
 
@@ -430,27 +545,37 @@ __device__ __forceinline__ float join(uint32_t n, uint32_t d, F&& get, float& m,
     return o;
 }
 
+// Stages of 32 keys that a warp (KEYS) or the CTA keeps on their way.
+template <int HD, bool KEYS>
+__host__ __device__ constexpr uint32_t stages() { return !KEYS || HD == 64 ? 4u : 2u; }
+template <int HD, bool KEYS>
+constexpr size_t smem_bytes() {
+    return (KEYS ? kWarps : 1u) * stages<HD, KEYS>() * 36u * HD + kWarps * (2u * (HD / 64u) * 256u + (HD > 128 ? HD / 16u * 512u : 0u));
+}
+
 // KEYS: the four warps share a tile of eight rows and take sixteen keys of a block each (a decode step);
 // else each has eight rows of a tile of 32 of its own and all see the same keys (prompts).
 template <typename T, int HD, bool KEYS>
-__global__ void __launch_bounds__(kThreads, HD > 128 ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, HD > 128 ? 2 : HD > 64 ? 3 : 4)
 kv_attention_kernel(AttnParams p) {
-    constexpr uint32_t TILE = KEYS ? 8u : 32u, SB = 18u * HD;
-    constexpr uint32_t kStages = KEYS ? 4u : 3u, kStageBytes = KEYS ? SB : 4u * SB;
+    constexpr uint32_t TILE = KEYS ? 8u : 32u, SB = 18u * HD;      // SB: a block of sixteen tokens
+    using Warp = Rows<T, HD>;
+    constexpr uint32_t kStages = stages<HD, KEYS>(), kStageBytes = 2u * SB;
     extern __shared__ __align__(128) uint8_t smem[];
-    // stages (of each warp, or of all); then for each warp its rows to be joined (KEYS) and, before them in the
-    // same place, its q fragments (head_dim 256)
+    // stages (of each warp, or of all); for each warp, widened steps and minima; q fragments (head_dim 256). Rows to be
+    // joined (KEYS) lie where the warp's stages were
     uint8_t* ring = smem;
-    constexpr uint32_t kOwn = 8u * (HD + 2u) * 4u;
-    static_assert(HD <= 128 || kOwn >= HD / 16 * 512u, "a warp's q fragments fit where its rows go");
-    float* rows_s = reinterpret_cast<float*>(smem + (KEYS ? kWarps : 1u) * kStages * kStageBytes);
+    uint8_t* meta_s = smem + (KEYS ? kWarps : 1u) * kStages * kStageBytes;
     __shared__ uint64_t bars[kWarps * kStages];
     __shared__ uint64_t scan[kWarps];
     __shared__ uint64_t found_at;
     __shared__ uint32_t found, flag, longest;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    uint4* my_q = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(rows_s) + warp * kOwn);
+    uint8_t* my_meta = meta_s + warp * Warp::kMetaBytes;
+    uint4* my_q = reinterpret_cast<uint4*>(meta_s + kWarps * Warp::kMetaBytes + warp * (HD / 16u) * 512u);
     uint8_t* my_ring = ring + (KEYS ? warp * kStages * kStageBytes : 0u);
+    static_assert(!KEYS || kStages * kStageBytes >= 8u * kPitch<HD> * 4u, "a warp's rows fit into its stages");
+    auto rows_of = [&](uint32_t w) { return reinterpret_cast<float*>(ring + w * kStages * kStageBytes); };
     const uint32_t my_bar = smem_u32(&bars[KEYS ? warp * kStages : 0u]);
     if (tid == 0) {
         for (uint32_t i = 0; i < kWarps * kStages; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&bars[i])));
@@ -489,7 +614,7 @@ kv_attention_kernel(AttnParams p) {
     }
     if (!total) return;
     // Joining n pieces costs a CTA about a ninth of a block's time each: no unit is cut finer than both together take.
-    const uint64_t least_blocks = 1u + static_cast<uint32_t>(sqrtf(static_cast<float>(longest) / 9.0f));
+    const uint64_t least_blocks = 1u + static_cast<uint32_t>(sqrtf(static_cast<float>(longest) / 16.0f));
     const uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), max(total / least_blocks, static_cast<uint64_t>(1)));
     if (blockIdx.x >= ctas) return;
     const uint64_t x0 = blockIdx.x * total / ctas, x1 = (blockIdx.x + 1u) * total / ctas;
@@ -516,7 +641,21 @@ kv_attention_kernel(AttnParams p) {
     sq.load<TILE>(p, s);
     uint32_t turn = 0;       // stages filled so far
     bool live = true;
-    Rows<T, HD> rows;
+    Warp rows;
+
+    // Two blocks of sixteen tokens, one copy where they lie one behind the other; a block without a page is left out.
+    auto fetch = [&](uint8_t* to, uint32_t bar, uint32_t sub, int32_t pg0, int32_t pg1, uint32_t kvh) {
+        const uint32_t mask = (1u << p.kv.page_shift) - 1u, bytes = ((pg0 >= 0 ? 1u : 0u) + (pg1 >= 0 ? 1u : 0u)) * SB;
+        const bool one = pg0 == pg1 && pg0 >= 0 && p.kv.page_shift > 4u;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+        auto copy = [&](uint32_t at, int32_t page, uint32_t token, uint32_t size) {
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to) + at),
+                         "l"(p.kv.base + p.kv.block_at(static_cast<uint32_t>(page), kvh, token & mask)), "r"(size), "r"(bar)
+                         : "memory");
+        };
+        if (pg0 >= 0) copy(0u, pg0, sub * 16u, one ? 2u * SB : SB);
+        if (pg1 >= 0 && !one) copy(SB, pg1, sub * 16u + 16u, SB);
+    };
 
     while (x < x1 && live) {
         // ---- the unit that holds place x ----
@@ -561,33 +700,24 @@ kv_attention_kernel(AttnParams p) {
 
         rows.load(p, sq, kvh, tile * TILE + (KEYS ? 0u : warp * 8u), lane, my_q);
 
-        // ---- its keys from block b0 to b1 ----
+        // ---- its keys from block b0 to b1, in pieces of 32 ----
+        const uint32_t subs = static_cast<uint32_t>(keys + 15) / 16u;      // blocks of sixteen that exist
         if constexpr (KEYS) {
-            // a warp's i-th piece is keys (4 (b0 + i) + warp) * 16 and on; its page, 32 pieces at a time
+            // a warp's i-th piece is number 4 (b0 + i) + warp; the pages of sixteen pieces at a time, a lane a block
             const uint32_t first = 4u * b0 + warp;
-            const int32_t left = (keys + 15) / 16 - static_cast<int32_t>(first);
-            const uint32_t n = left <= 0 ? 0u : min(b1 - b0, (static_cast<uint32_t>(left) + 3u) / 4u);
+            const uint32_t n = 2u * first >= subs ? 0u : min(b1 - b0, (subs - 2u * first + 7u) / 8u);
             int32_t page_of = -1;
-            uint32_t there = 0;      // by stage: the piece has a page
+            uint32_t there = 0;      // two bits a stage: the piece's blocks have pages
             auto issue = [&](uint32_t i) {
-                if ((i & 31u) == 0u) {
-                    const uint32_t j = i + lane;
-                    page_of = j < n ? __ldg(table + ((first + 4u * j) >> (p.kv.page_shift - 4u))) : -1;
+                if ((i & 15u) == 0u) {
+                    const uint32_t sub = 2u * (first + 4u * (i + (lane >> 1))) + (lane & 1u);
+                    page_of = sub < subs ? __ldg(table + (sub >> (p.kv.page_shift - 4u))) : -1;
+                    if (static_cast<uint32_t>(page_of) >= p.kv.n_pages) page_of = -1;
                 }
-                const int32_t page = __shfl_sync(0xFFFFFFFFu, page_of, i & 31u);
-                const bool ok = page >= 0 && static_cast<uint32_t>(page) < p.kv.n_pages;
-                const uint32_t st = turn % kStages;
-                there = ok ? there | 1u << st : there & ~(1u << st);
-                if (lane == 0) {
-                    const uint32_t at = ((first + 4u * i) * 16u) & ((1u << p.kv.page_shift) - 1u);
-                    const uint8_t* src = p.kv.base + p.kv.block_at(ok ? page : 0, kvh, at);    // page 0 always is one
-                    const uint32_t bar = my_bar + 8u * st;
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(SB) : "memory");
-                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                     smem_u32(my_ring + st * SB)),
-                                 "l"(src), "r"(SB), "r"(bar)
-                                 : "memory");
-                }
+                const int32_t pg0 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u)), pg1 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u) + 1u);
+                const uint32_t st = turn % kStages, have = (pg0 >= 0 ? 1u : 0u) | (pg1 >= 0 ? 2u : 0u);
+                there = (there & ~(3u << 2u * st)) | have << 2u * st;
+                if (lane == 0) fetch(my_ring + st * kStageBytes, my_bar + 8u * st, 2u * (first + 4u * i), pg0, pg1, kvh);
                 ++turn;
             };
             const uint32_t turn0 = turn;
@@ -596,53 +726,34 @@ kv_attention_kernel(AttnParams p) {
                 const uint32_t k = turn0 + i, st = k % kStages;
                 live = live && __all_sync(0xFFFFFFFFu, mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin));
                 if (!live) break;
-                rows.keys16(my_ring + st * SB, static_cast<int32_t>((first + 4u * i) * 16u), there >> st & 1u, lane, my_q);
+                rows.keys32(my_ring + st * kStageBytes, static_cast<int32_t>((first + 4u * i) * kPiece), there >> 2u * st & 3u, lane, my_q, my_meta);
                 __syncwarp();
                 if (i + kStages < n) issue(i + kStages);
             }
             __syncwarp();
-            rows.store(rows_s + warp * 8u * (HD + 2u), lane);
+            rows.store(rows_of(warp), lane);
         } else {
-            // all warps: block by block, thread 0 copies; sixteen keys without a page are left out by everyone
-            const uint32_t n = b1 - b0;
+            // all warps see every piece; thread 0 copies, everyone asks for the pages
+            const uint32_t first = 4u * b0, n = min(4u * (b1 - b0), (max(subs, 2u * first) - 2u * first + 1u) / 2u);
             auto page_at = [&](uint32_t sub) -> int32_t {
-                const int32_t page = static_cast<int32_t>(sub * 16u) < keys ? __ldg(table + (sub >> (p.kv.page_shift - 4u))) : -1;
-                return page >= 0 && static_cast<uint32_t>(page) < p.kv.n_pages ? page : -1;
+                const int32_t page = sub < subs ? __ldg(table + (sub >> (p.kv.page_shift - 4u))) : -1;
+                return static_cast<uint32_t>(page) < p.kv.n_pages ? page : -1;
             };
-            auto issue = [&](uint32_t i, uint32_t k) {
-                const uint32_t st = k % kStages, bar = my_bar + 8u * st;
-                int32_t page[4];
-                uint32_t count = 0;
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) {
-                    page[j] = page_at(4u * (b0 + i) + j);
-                    count += page[j] >= 0;
-                }
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count * SB) : "memory");
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) {
-                    if (page[j] < 0) continue;
-                    const uint32_t at = ((4u * (b0 + i) + j) * 16u) & ((1u << p.kv.page_shift) - 1u);
-                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                     smem_u32(my_ring + st * kStageBytes + j * SB)),
-                                 "l"(p.kv.base + p.kv.block_at(page[j], kvh, at)), "r"(SB), "r"(bar)
-                                 : "memory");
-                }
+            auto issue = [&](uint32_t i) {
+                const uint32_t st = (turn + i) % kStages, sub = 2u * (first + i);
+                fetch(my_ring + st * kStageBytes, my_bar + 8u * st, sub, page_at(sub), page_at(sub + 1u), kvh);
             };
             if (tid == 0)
-                for (uint32_t i = 0; i < min(n, kStages); ++i) issue(i, turn + i);
+                for (uint32_t i = 0; i < min(n, kStages); ++i) issue(i);
             for (uint32_t i = 0; i < n; ++i) {
-                const uint32_t k = turn + i, st = k % kStages;
+                const uint32_t k = turn + i, st = k % kStages, sub = 2u * (first + i);
                 live = live && __all_sync(0xFFFFFFFFu, mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin));
-                if (live) {
-                    for (uint32_t j = 0; j < 4u; ++j) {
-                        const int32_t tok = static_cast<int32_t>((4u * (b0 + i) + j) * 16u);
-                        if (tok < rows.most) rows.keys16(my_ring + st * kStageBytes + j * SB, tok, page_at(4u * (b0 + i) + j) >= 0, lane, my_q);
-                    }
-                }
+                const int32_t tok = static_cast<int32_t>(16u * sub);
+                if (live && tok < rows.most)
+                    rows.keys32(my_ring + st * kStageBytes, tok, (page_at(sub) >= 0 ? 1u : 0u) | (page_at(sub + 1u) >= 0 ? 2u : 0u), lane, my_q, my_meta);
                 live = __syncthreads_and(live);
                 if (!live) break;
-                if (tid == 0 && i + kStages < n) issue(i + kStages, k + kStages);
+                if (tid == 0 && i + kStages < n) issue(i + kStages);
             }
             turn += n;
         }
@@ -653,7 +764,7 @@ kv_attention_kernel(AttnParams p) {
 
         // ---- out, or a piece of it ----
         const bool whole = b0 == 0u && b1 == n_blocks;
-        float* slot = p.part + (static_cast<size_t>(blockIdx.x) * 2u + (start >= x0 ? 1u : 0u)) * TILE * (HD + 2u);
+        float* slot = p.part + (static_cast<size_t>(blockIdx.x) * 2u + (start >= x0 ? 1u : 0u)) * TILE * kPitch<HD>;
         auto write = [&](uint32_t r, uint32_t d, float o, float l, bool seen) {
             const uint32_t rr = tile * TILE + r, tok = rr / p.group, head = kvh * p.group + rr % p.group;
             if (tok >= sq.n_new) return;
@@ -664,37 +775,29 @@ kv_attention_kernel(AttnParams p) {
             for (uint32_t e = tid; e < 8u * HD; e += kThreads) {
                 const uint32_t r = e / HD, d = e % HD;
                 float m, l;
-                const float o = join<HD>(kWarps, d, [&](uint32_t i, uint32_t j) { return rows_s[(i * 8u + r) * (HD + 2u) + j]; }, m, l);
+                const float o = join<HD>(kWarps, d, [&](uint32_t i, uint32_t j) { return rows_of(i)[r * kPitch<HD> + j]; }, m, l);
                 if (whole) {
                     write(r, d, o, l, l != 0.0f);
                 } else {
-                    slot[r * (HD + 2u) + d] = o;
+                    slot[r * kPitch<HD> + d] = o;
                     if (d == 0) {
-                        slot[r * (HD + 2u) + HD] = m;
-                        slot[r * (HD + 2u) + HD + 1u] = l;
+                        slot[r * kPitch<HD> + HD] = m;
+                        slot[r * kPitch<HD> + HD + 1u] = l;
                     }
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the stages are copied into again
             __syncthreads();
         } else if (!whole) {
-            rows.store(slot + warp * 8u * (HD + 2u), lane);
+            rows.store(slot + warp * 8u * kPitch<HD>, lane);
         } else {
-            // straight from the registers: lane (g, t) has sixteen neighbouring values of every group
-            const uint32_t g = lane >> 2, t = lane & 3u;
-            rows.l += __shfl_xor_sync(0xFFFFFFFFu, rows.l, 1);
-            rows.l += __shfl_xor_sync(0xFFFFFFFFu, rows.l, 2);
-            const float down = 1.0f / rows.escale;
+            rows.finish(
+                lane,
+                [&](uint32_t r, uint32_t d, const float(&v)[8], float sum) {
 #pragma unroll
-            for (uint32_t u = 0; u < HD / 64; ++u) {
-                rows.om[u] += __shfl_xor_sync(0xFFFFFFFFu, rows.om[u], 1);
-                rows.om[u] += __shfl_xor_sync(0xFFFFFFFFu, rows.om[u], 2);
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) {
-                    const float(&c)[4] = rows.o[u * 8u + i];
-                    write(warp * 8u + g, 64u * u + 16u * t + i, fmaf(c[0] + c[2], down, rows.om[u]), rows.l, rows.l != 0.0f);
-                    write(warp * 8u + g, 64u * u + 16u * t + 8u + i, fmaf(c[1] + c[3], down, rows.om[u]), rows.l, rows.l != 0.0f);
-                }
-            }
+                    for (uint32_t i = 0; i < 8u; ++i) write(warp * 8u + r, d + i, v[i], sum, sum != 0.0f);
+                },
+                [](uint32_t, float, float) {});
         }
         if (!whole) {
             // CTA c has place v if floor(c total / ctas) <= v < floor((c + 1) total / ctas)
@@ -716,7 +819,7 @@ kv_attention_kernel(AttnParams p) {
                     const float o = join<HD>(
                         c1 - c0 + 1u, d,
                         [&](uint32_t i, uint32_t j) {   // past L1: other CTAs wrote these
-                            return __ldcg(p.part + ((static_cast<size_t>(c0 + i) * 2u + (i == 0u ? 1u : 0u)) * TILE + r) * (HD + 2u) + j);
+                            return __ldcg(p.part + ((static_cast<size_t>(c0 + i) * 2u + (i == 0u ? 1u : 0u)) * TILE + r) * kPitch<HD> + j);
                         },
                         m, l);
                     write(r, d, o, l, l != 0.0f);
@@ -731,8 +834,7 @@ kv_attention_kernel(AttnParams p) {
 
 template <typename T, int HD, bool KEYS>
 void launch(csdr_context* ctx, AttnParams& p) {
-    constexpr size_t SB = 18u * HD;
-    constexpr size_t smem = (KEYS ? kWarps * 4u * SB : 3u * 4u * SB) + (KEYS || HD > 128 ? kWarps * 8u * (HD + 2u) * 4u : 0u);
+    constexpr size_t smem = smem_bytes<HD, KEYS>();
     auto kern = kv_attention_kernel<T, HD, KEYS>;
     const void* key = reinterpret_cast<const void*>(kern);
     ctx->opt_in_smem(key, smem);
@@ -756,7 +858,7 @@ void launch_typed(csdr_context* ctx, uint32_t head_dim, bool keys, AttnParams& p
 
 size_t kv_attention_counters(const csdr_context* ctx) { return static_cast<size_t>(ctx->sm_count) * kMostPerSm; }
 size_t kv_attention_workspace(const csdr_context* ctx, uint32_t head_dim) {
-    return kv_attention_counters(ctx) * (4u + 2u * 32u * (head_dim + 2u) * 4u);
+    return kv_attention_counters(ctx) * (4u + 2u * 32u * (head_dim + 4u) * 4u);
 }
 
 void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAttend& a, void* workspace) {

@@ -42,20 +42,20 @@ __device__ __forceinline__ bool locate(const KvView& kv, const KvBatchView& b, u
     return true;
 }
 
-// Lane `lane` holds values E lane .. E lane + E - 1 of a row: where its codes go.
+// Where the half word with values d & ~3 .. + 3 of a token lies.
 template <int HD>
 __device__ __forceinline__ uint32_t key_offset(uint32_t tok, uint32_t d) {
     const uint32_t o = d & 63u;
-    return tok * (HD / 2) + ((o >> 4) * (HD / 32) + 2u * (d >> 6) + ((o & 15u) >> 3)) * 4u + (o & 7u) / 2u;
+    return tok * (HD / 2) + ((o >> 4) * (HD / 32) + 2u * (d >> 6) + ((o & 15u) >> 3)) * 4u + (o & 4u) / 2u;
 }
 template <int HD>
 __device__ __forceinline__ uint32_t value_offset(uint32_t tok, uint32_t d) {
     const uint32_t o = d & 63u;
-    return 8u * HD + (tok >> 1) * HD + (o >> 3) * (HD / 8) + (d >> 6) * 8u + ((o & 7u) >> 2) * 4u + (tok & 1u) * 2u + (o & 3u) / 2u;
+    return 8u * HD + (tok >> 1) * HD + (o >> 3) * (HD / 8) + (d >> 6) * 8u + ((o & 7u) >> 2) * 4u + (tok & 1u) * 2u;
 }
 template <int HD>
 __device__ __forceinline__ uint32_t meta_offset(uint32_t tok, uint32_t d, uint32_t of_values) {
-    return 16u * HD + of_values * HD + (tok * (HD / 64) + (d >> 6)) * 4u;
+    return 16u * HD + of_values * HD + ((d >> 6) * 16u + tok) * 4u;
 }
 
 template <int HD>
@@ -80,26 +80,21 @@ __device__ __forceinline__ void quantise_row(const double (&x)[HD / 32], uint8_t
     const __half mn = fine ? __float2half_rn(static_cast<float>(lo)) : __ushort_as_half(0x7FFF);
     const __half st = fine ? __float2half_rn(static_cast<float>((hi - lo) / 15.0)) : __ushort_as_half(0);
     const double m = __half2float(mn), s = __half2float(st);
-    uint32_t codes = 0;
+    uint32_t c[E];
 #pragma unroll
-    for (uint32_t i = 0; i < E; ++i) {
-        const double c = s > 0.0 ? fmin(fmax(rint((x[i] - m) / s), 0.0), 15.0) : 0.0;
-        codes |= static_cast<uint32_t>(c) << (4u * i);
-    }
+    for (uint32_t i = 0; i < E; ++i) c[i] = s > 0.0 ? static_cast<uint32_t>(fmin(fmax(rint((x[i] - m) / s), 0.0), 15.0)) : 0u;
     const uint32_t d = E * lane;
     uint8_t* to = block + (of_values ? value_offset<HD>(tok, d) : key_offset<HD>(tok, d));
-    if constexpr (E == 2) {
-        *to = static_cast<uint8_t>(codes);
-    } else if constexpr (E == 4) {
-        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(codes);
-    } else if (of_values) {
-        reinterpret_cast<uint16_t*>(to)[0] = static_cast<uint16_t>(codes);
-        reinterpret_cast<uint16_t*>(to)[2] = static_cast<uint16_t>(codes >> 16);
+    if constexpr (E == 2) {       // two lanes share a half word
+        const uint32_t c2 = __shfl_down_sync(0xFFFFFFFFu, c[0], 1), c3 = __shfl_down_sync(0xFFFFFFFFu, c[1], 1);
+        if (!(lane & 1u)) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(pack_codes(c[0], c[1], c2, c3));
     } else {
-        *reinterpret_cast<uint32_t*>(to) = codes;
+#pragma unroll
+        for (uint32_t i = 0; i < E; i += 4u)
+            *reinterpret_cast<uint16_t*>(to + (of_values ? i : i / 2u)) = static_cast<uint16_t>(pack_codes(c[i], c[i + 1], c[i + 2], c[i + 3]));
     }
     if (lane % kLanes == 0) {
-        const __half2 both = __halves2half2(st, mn);
+        const __half2 both = __halves2half2(mn, st);
         *reinterpret_cast<__half2*>(block + meta_offset<HD>(tok, d, of_values)) = both;
     }
 }
@@ -159,22 +154,21 @@ kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restric
     for (uint32_t u = blockIdx.y * kWarps + warp; u < 2u * kv.kv_heads; u += gridDim.y * kWarps) {
         const uint32_t is_v = u >= kv.kv_heads, head = is_v ? u - kv.kv_heads : u;
         float* dst = (is_v ? v : k) + (static_cast<size_t>(t) * kv.kv_heads + head) * HD + d;
-        uint32_t codes = 0;
+        uint32_t codes[E] = {};
         float st = 0.0f, mn = 0.0f;
         if (page >= 0) {
             const uint32_t at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
             const uint8_t* block = kv.base + kv.block_at(page, head, at);
             const uint8_t* from = block + (is_v ? value_offset<HD>(tok, d) : key_offset<HD>(tok, d));
-            if constexpr (E == 2) codes = *from;
-            else if constexpr (E == 4) codes = *reinterpret_cast<const uint16_t*>(from);
-            else if (is_v) codes = reinterpret_cast<const uint16_t*>(from)[0] | static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(from)[2]) << 16;
-            else codes = *reinterpret_cast<const uint32_t*>(from);
+#pragma unroll
+            for (uint32_t i = 0; i < E; ++i)
+                codes[i] = unpack_code(*reinterpret_cast<const uint16_t*>(from + (is_v ? i / 4u * 4u : i / 4u * 2u)), (d + i) & 3u);
             const __half2 both = *reinterpret_cast<const __half2*>(block + meta_offset<HD>(tok, d, is_v));
-            st = __low2float(both);
-            mn = __high2float(both);
+            mn = __low2float(both);
+            st = __high2float(both);
         }
 #pragma unroll
-        for (uint32_t i = 0; i < E; ++i) dst[i] = fmaf(static_cast<float>((codes >> (4u * i)) & 15u), st, mn);
+        for (uint32_t i = 0; i < E; ++i) dst[i] = fmaf(static_cast<float>(codes[i]), st, mn);
     }
 }
 

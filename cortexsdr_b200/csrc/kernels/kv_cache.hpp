@@ -14,12 +14,20 @@ constexpr uint32_t kKvBlock = 16;    // tokens of a block, the unit of the layou
 
 // Where a cache's pages lie. A page holds, for each kv head, its blocks of sixteen tokens one behind the other:
 //   keys     16 x head_dim / 2 bytes, a token's row after another; word (t, w) of a row, t < 4 and
-//            w < head_dim / 32, holds the eight values 64 (w / 2) + 16 t + 8 (w % 2) + n, value n in bits 4n
-//   values   8 pairs of tokens; word (g, u, x) of a pair, g < 8, u < head_dim / 64, x < 2, holds the four
-//            values 64 u + 8 g + 4 x + n of the even token in its low half and of the odd one in its high half
-//   (fp16 step, fp16 minimum) of the keys' groups, [token][group], then of the values'
-// so that a lane of the attention kernel finds what its matrix fragments take in one 128-bit piece
-// each, and a block is one contiguous copy.
+//            w < head_dim / 32, holds the values 64 (w / 2) + 16 t + 8 (w % 2) + 0 .. 3 in its low half, + 4 .. 7 in its high half
+//   values   8 pairs of tokens; word (g, u, x) of a pair, g < 8, u < head_dim / 64, x < 2, holds the
+//            values 64 u + 8 g + 4 x + 0 .. 3 of the even token in its low half and of the odd one in its high half
+//   (fp16 minimum, fp16 step in the upper half) of the keys' groups, [group][token], then of the values'
+// so that a lane of the attention kernel finds what its matrix fragments take in one piece each, and a block is one
+// contiguous copy. The four codes of a half lie where a mask, after a shift by four bits or an exchange of the
+// half's bytes, leaves each of them in bits 6 - 9 (pack_codes).
+__host__ __device__ inline uint32_t pack_codes(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
+    return c0 << 6 | c1 << 2 | (c2 & 3u) << 14 | c2 >> 2 | c3 << 10;
+}
+__host__ __device__ inline uint32_t unpack_code(uint32_t half, uint32_t n) {
+    return n == 0u ? half >> 6 & 15u : n == 1u ? half >> 2 & 15u : n == 2u ? (half >> 14 & 3u) | (half & 3u) << 2 : half >> 10 & 15u;
+}
+
 struct KvView {
     uint8_t* base = nullptr;
     uint32_t n_pages = 0, kv_heads = 0, page_shift = 0;   // tokens of a page: 1 << page_shift
