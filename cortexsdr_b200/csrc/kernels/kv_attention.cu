@@ -32,24 +32,28 @@ constexpr uint32_t kWarps = 4, kThreads = kWarps * 32, kPiece = 32, kBlockKeys =
 constexpr float kSlack = 6.0f;
 template <int HD>
 constexpr uint32_t kPitch = HD + 4;      // of a row of outputs with its maximum and sum
-constexpr uint32_t kMostPerSm = 4;
+constexpr uint32_t kMostPerSm = 5;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"      // callers stop at p.spin, the wait limit
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0u;
+}
+// The whole warp waits, and gives up as one.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
-    for (uint32_t spin = 0; spin < limit; ++spin) {
-        uint32_t done;
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-            "selp.u32 %0, 1, 0, p;\n"
-            "}\n"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
+    if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
+    for (uint32_t spin = 0; spin < limit; ++spin)
+        if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
     return false;
 }
 
@@ -134,12 +138,16 @@ struct AttnParams {
     KvBatchView b;
     KvAttend a;
     uint32_t group;          // query heads of a kv head
-    uint32_t vec;            // q rows start on 16 bytes
+    uint32_t vec, vec_out;   // rows of q, of the result start on 16 bytes
     float* part;             // [CTA][2][rows][HD + 4]
     uint32_t* counters;      // [CTA]: arrivals at the unit that starts in a CTA's share and is cut
     int* status;
     uint32_t spin;
 };
+
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
+    return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
 
 // A sequence as the schedule sees it.
 struct Seq {
@@ -188,7 +196,7 @@ struct Rows {
     static constexpr uint32_t W = HD / 32, G = HD / 64;
     static constexpr bool kOnce = std::is_same<T, __nv_bfloat16>::value, kFine = std::is_same<T, float>::value;
     static constexpr float kOdd = kFine ? 1.0f : 16.0f;      // odd pairs of codes count one in kOdd
-    static constexpr bool kShared = HD > 128;      // q fragments in shared memory: the registers go to the outputs
+    static constexpr bool kShared = HD >= 128;     // q fragments in shared memory: the registers go to the outputs
     static constexpr uint32_t kMetaBytes = 2u * G * 16u * 16u;      // of a piece, widened
     uint32_t q[kShared ? 1 : W * 2][4];
     float o[G][4][4];    // tile n of a group: values 8 g + n (rows 2t, 2t + 1), 8 g + 4 + n (rows 2t, 2t + 1)
@@ -201,7 +209,9 @@ struct Rows {
     int32_t most;
 
     // Lane (g, t): row g of the tile, values 64 (w / 2) + 16 t + 8 (w % 2) + n of words w.
-    __device__ __forceinline__ void load(const AttnParams& p, const Seq& s, uint32_t kvh, uint32_t row, uint32_t lane, uint4* shared) {
+    // Of `parts` warps with the same rows, number `part` writes its part of shared fragments.
+    __device__ __forceinline__ void load(const AttnParams& p, const Seq& s, uint32_t kvh, uint32_t row, uint32_t lane, uint4* shared, uint32_t part,
+                                         uint32_t parts) {
         const uint32_t t = lane & 3u, rr = row + (lane >> 2);
         const uint32_t tok = rr / p.group, head = kvh * p.group + rr % p.group;
         const bool there = tok < s.n_new;
@@ -255,6 +265,7 @@ struct Rows {
             }
 #pragma unroll
             for (uint32_t h = 0; h < 2u; ++h) {
+                if (kShared && w % parts != part) continue;
                 // values 2h, 2h + 4 meet even pairs of codes, 2h + 1, 2h + 5 odd ones
                 uint32_t f[4];
                 split(pack2(x[w][2 * h], x[w][2 * h + 4]), f[0], f[1]);
@@ -282,7 +293,6 @@ struct Rows {
         l = pack2(0.0f, 0.0f);
         escale = 1.0f;
         vmax = 0;
-        if constexpr (kShared) __syncwarp();
     }
 
     // A value of row 2t and of row 2t + 1, from the lanes that have the rows.
@@ -293,9 +303,10 @@ struct Rows {
 
     // 32 keys from `tok0` on, in shared memory at `block` (two blocks of sixteen); bit i of `there`: block i has a page.
     // `meta`: the warp's, for steps and minima as pairs of fp32 over neighbouring tokens.
+    // edge: some row does not see all of them.
+    template <bool edge>
     __device__ __forceinline__ void keys32(const uint8_t* block, int32_t tok0, uint32_t there, uint32_t lane, const uint4* shared, uint8_t* meta) {
         const uint32_t g = lane >> 2, t = lane & 3u;
-        const bool edge = there != 3u || tok0 + 32 > least;
         // ---- steps and minima: a lane widens a pair of tokens of the keys' groups (lanes 0-15) or of the values' ----
         uint32_t big = 0;
         {
@@ -466,6 +477,10 @@ struct Rows {
             }
         }
     }
+    __device__ __forceinline__ void piece(const uint8_t* block, int32_t tok0, uint32_t there, uint32_t lane, const uint4* shared, uint8_t* meta) {
+        if (there != 3u || tok0 + 32 > least) keys32<true>(block, tok0, there, lane, shared, meta);
+        else keys32<false>(block, tok0, there, lane, shared, meta);
+    }
     static __device__ __forceinline__ void scale_tile(float (&c)[4], f32x2 f) {
         const float2 a = unpack2(mul2(pack2(c[0], c[1]), f)), b = unpack2(mul2(pack2(c[2], c[3]), f));
         c[0] = a.x;
@@ -521,28 +536,51 @@ struct Rows {
                 at[1] = make_float4(v[4], v[5], v[6], v[7]);
             },
             [&](uint32_t r, float top, float sum) {
-                to[r * kPitch<HD> + HD] = top;
-                to[r * kPitch<HD> + HD + 1] = sum;
+                *reinterpret_cast<float2*>(to + r * kPitch<HD> + HD) = make_float2(top, sum);
             });
     }
 };
 
-// Adds up n pieces of a row ([HD] outputs, maximum, sum), one element: the joined output, maximum and sum.
-// `get` reads a float of a piece.
+// Joins n pieces of a row (outputs, maximum, sum), eight values of it. `get` reads four floats of a piece.
 template <int HD, typename F>
-__device__ __forceinline__ float join(uint32_t n, uint32_t d, F&& get, float& m, float& l) {
+__device__ __forceinline__ void join(uint32_t n, uint32_t d, F&& get, float (&o)[8], float& m, float& l) {
     m = -FLT_MAX;
-#pragma unroll 4
-    for (uint32_t i = 0; i < n; ++i) m = fmaxf(m, get(i, HD));
-    float o = 0.0f;
     l = 0.0f;
+#pragma unroll
+    for (uint32_t j = 0; j < 8u; ++j) o[j] = 0.0f;
+#pragma unroll 4
+    for (uint32_t i = 0; i < n; ++i) m = fmaxf(m, get(i, HD).x);
 #pragma unroll 4
     for (uint32_t i = 0; i < n; ++i) {
-        const float f = ex2(get(i, HD) - m);
-        l = fmaf(f, get(i, HD + 1), l);
-        o = fmaf(f, get(i, d), o);
+        const float4 st = get(i, HD), a = get(i, d), b = get(i, d + 4u);
+        const float f = ex2(st.x - m);
+        l = fmaf(f, st.y, l);
+        o[0] = fmaf(f, a.x, o[0]);
+        o[1] = fmaf(f, a.y, o[1]);
+        o[2] = fmaf(f, a.z, o[2]);
+        o[3] = fmaf(f, a.w, o[3]);
+        o[4] = fmaf(f, b.x, o[4]);
+        o[5] = fmaf(f, b.y, o[5]);
+        o[6] = fmaf(f, b.z, o[6]);
+        o[7] = fmaf(f, b.w, o[7]);
     }
-    return o;
+}
+
+// Eight results, as one or two 128-bit pieces where rows start on 16 bytes.
+template <typename T>
+__device__ __forceinline__ void store_row(T* to, const float (&v)[8], float by, bool vec) {
+    T r[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) r[i] = op_narrow<T>(v[i] * by);
+    if (vec) {
+        const uint4* from = reinterpret_cast<const uint4*>(r);
+        uint4* at = reinterpret_cast<uint4*>(to);
+        at[0] = from[0];
+        if constexpr (sizeof(T) == 4) at[1] = from[1];
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) to[i] = r[i];
+    }
 }
 
 // Stages of 32 keys that a warp (KEYS) or the CTA keeps on their way.
@@ -550,19 +588,20 @@ template <int HD, bool KEYS>
 __host__ __device__ constexpr uint32_t stages() { return !KEYS || HD == 64 ? 4u : 2u; }
 template <int HD, bool KEYS>
 constexpr size_t smem_bytes() {
-    return (KEYS ? kWarps : 1u) * stages<HD, KEYS>() * 36u * HD + kWarps * (2u * (HD / 64u) * 256u + (HD > 128 ? HD / 16u * 512u : 0u));
+    return (KEYS ? kWarps : 1u) * stages<HD, KEYS>() * 36u * HD + kWarps * 2u * (HD / 64u) * 256u +
+           (HD >= 128 ? (KEYS ? 1u : kWarps) * (HD / 16u) * 512u : 0u);
 }
 
 // KEYS: the four warps share a tile of eight rows and take sixteen keys of a block each (a decode step);
 // else each has eight rows of a tile of 32 of its own and all see the same keys (prompts).
 template <typename T, int HD, bool KEYS>
-__global__ void __launch_bounds__(kThreads, HD > 128 ? 2 : HD > 64 ? 3 : 4)
+__global__ void __launch_bounds__(kThreads, HD > 128 ? 2 : 5)
 kv_attention_kernel(AttnParams p) {
     constexpr uint32_t TILE = KEYS ? 8u : 32u, SB = 18u * HD;      // SB: a block of sixteen tokens
     using Warp = Rows<T, HD>;
     constexpr uint32_t kStages = stages<HD, KEYS>(), kStageBytes = 2u * SB;
     extern __shared__ __align__(128) uint8_t smem[];
-    // stages (of each warp, or of all); for each warp, widened steps and minima; q fragments (head_dim 256). Rows to be
+    // stages (of each warp, or of all); for each warp, widened steps and minima; q fragments (head_dim 128 and 256). Rows to be
     // joined (KEYS) lie where the warp's stages were
     uint8_t* ring = smem;
     uint8_t* meta_s = smem + (KEYS ? kWarps : 1u) * kStages * kStageBytes;
@@ -572,7 +611,7 @@ kv_attention_kernel(AttnParams p) {
     __shared__ uint32_t found, flag, longest;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     uint8_t* my_meta = meta_s + warp * Warp::kMetaBytes;
-    uint4* my_q = reinterpret_cast<uint4*>(meta_s + kWarps * Warp::kMetaBytes + warp * (HD / 16u) * 512u);
+    uint4* my_q = reinterpret_cast<uint4*>(meta_s + kWarps * Warp::kMetaBytes + (KEYS ? 0u : warp) * (HD / 16u) * 512u);
     uint8_t* my_ring = ring + (KEYS ? warp * kStages * kStageBytes : 0u);
     static_assert(!KEYS || kStages * kStageBytes >= 8u * kPitch<HD> * 4u, "a warp's rows fit into its stages");
     auto rows_of = [&](uint32_t w) { return reinterpret_cast<float*>(ring + w * kStages * kStageBytes); };
@@ -615,9 +654,9 @@ kv_attention_kernel(AttnParams p) {
     if (!total) return;
     // Joining n pieces costs a CTA about a ninth of a block's time each: no unit is cut finer than both together take.
     const uint64_t least_blocks = 1u + static_cast<uint32_t>(sqrtf(static_cast<float>(longest) / 16.0f));
-    const uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), max(total / least_blocks, static_cast<uint64_t>(1)));
+    const uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), max(quotient(total, least_blocks), static_cast<uint64_t>(1)));
     if (blockIdx.x >= ctas) return;
-    const uint64_t x0 = blockIdx.x * total / ctas, x1 = (blockIdx.x + 1u) * total / ctas;
+    const uint64_t x0 = quotient(blockIdx.x * total, ctas), x1 = quotient((blockIdx.x + 1u) * total, ctas);
     {
         uint64_t at = before + upto - mine;
         if (x0 >= at && x0 < at + mine) {
@@ -644,17 +683,20 @@ kv_attention_kernel(AttnParams p) {
     Warp rows;
 
     // Two blocks of sixteen tokens, one copy where they lie one behind the other; a block without a page is left out.
-    auto fetch = [&](uint8_t* to, uint32_t bar, uint32_t sub, int32_t pg0, int32_t pg1, uint32_t kvh) {
-        const uint32_t mask = (1u << p.kv.page_shift) - 1u, bytes = ((pg0 >= 0 ? 1u : 0u) + (pg1 >= 0 ? 1u : 0u)) * SB;
-        const bool one = pg0 == pg1 && pg0 >= 0 && p.kv.page_shift > 4u;
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-        auto copy = [&](uint32_t at, int32_t page, uint32_t token, uint32_t size) {
+    const uint32_t in_page = (1u << (p.kv.page_shift - 4u)) - 1u;
+    const size_t page_bytes = p.kv.block_at(1u, 0u, 0u);
+    const uint8_t* head_base = nullptr;      // of the unit's kv head
+    auto fetch = [&](uint8_t* to, uint32_t bar, uint32_t sub, int32_t pg0, int32_t pg1) {
+        const bool one = pg0 == pg1 && in_page != 0u;
+        const uint32_t first = one && pg0 >= 0 ? 2u * SB : pg0 >= 0 ? SB : 0u, second = !one && pg1 >= 0 ? SB : 0u;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(first + second) : "memory");
+        auto copy = [&](uint32_t at, int32_t page, uint32_t block, uint32_t size) {
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to) + at),
-                         "l"(p.kv.base + p.kv.block_at(static_cast<uint32_t>(page), kvh, token & mask)), "r"(size), "r"(bar)
+                         "l"(head_base + static_cast<uint32_t>(page) * page_bytes + (block & in_page) * SB), "r"(size), "r"(bar)
                          : "memory");
         };
-        if (pg0 >= 0) copy(0u, pg0, sub * 16u, one ? 2u * SB : SB);
-        if (pg1 >= 0 && !one) copy(SB, pg1, sub * 16u + 16u, SB);
+        if (first) copy(0u, pg0, sub, first);
+        if (second) copy(SB, pg1, sub + 1u, second);
     };
 
     while (x < x1 && live) {
@@ -666,12 +708,12 @@ kv_attention_kernel(AttnParams p) {
             w = sq.head_weight() * p.kv.kv_heads;
         }
         const uint64_t hw = sq.head_weight(), y = x - seq_at, pairs = static_cast<uint64_t>(sq.tiles / 2u) * sq.pair_weight;
-        const uint32_t kvh = static_cast<uint32_t>(y / hw);
-        const uint64_t z = y % hw;
+        const uint32_t kvh = static_cast<uint32_t>(quotient(y, hw));
+        const uint64_t z = y - kvh * hw;
         uint32_t tile, b0;
         uint64_t next = seq_at + kvh * hw;       // where the next unit starts
         if (z < pairs) {
-            const uint32_t pr = static_cast<uint32_t>(z / sq.pair_weight), o = static_cast<uint32_t>(z % sq.pair_weight);
+            const uint32_t pr = static_cast<uint32_t>(quotient(z, sq.pair_weight)), o = static_cast<uint32_t>(z - static_cast<uint64_t>(pr) * sq.pair_weight);
             const uint32_t n = sq.blocks<TILE>(pr, p.group);
             next += static_cast<uint64_t>(pr) * sq.pair_weight;
             tile = pr;
@@ -696,9 +738,8 @@ kv_attention_kernel(AttnParams p) {
         const uint64_t start = x - b0;
         const uint32_t b1 = static_cast<uint32_t>(min(static_cast<uint64_t>(n_blocks), static_cast<uint64_t>(b0) + (x1 - x)));
         const int32_t keys = static_cast<int32_t>(sq.keys<TILE>(tile, p.group));
+        head_base = p.kv.base + p.kv.block_at(0u, kvh, 0u);
         const int32_t* table = p.b.pages + static_cast<size_t>(s) * p.b.pages_per_seq;
-
-        rows.load(p, sq, kvh, tile * TILE + (KEYS ? 0u : warp * 8u), lane, my_q);
 
         // ---- its keys from block b0 to b1, in pieces of 32 ----
         const uint32_t subs = static_cast<uint32_t>(keys + 15) / 16u;      // blocks of sixteen that exist
@@ -717,16 +758,18 @@ kv_attention_kernel(AttnParams p) {
                 const int32_t pg0 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u)), pg1 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u) + 1u);
                 const uint32_t st = turn % kStages, have = (pg0 >= 0 ? 1u : 0u) | (pg1 >= 0 ? 2u : 0u);
                 there = (there & ~(3u << 2u * st)) | have << 2u * st;
-                if (lane == 0) fetch(my_ring + st * kStageBytes, my_bar + 8u * st, 2u * (first + 4u * i), pg0, pg1, kvh);
+                if (lane == 0) fetch(my_ring + st * kStageBytes, my_bar + 8u * st, 2u * (first + 4u * i), pg0, pg1);
                 ++turn;
             };
             const uint32_t turn0 = turn;
             for (uint32_t i = 0; i < min(n, kStages); ++i) issue(i);
+            rows.load(p, sq, kvh, tile * TILE, lane, my_q, warp, kWarps);
+            if constexpr (Warp::kShared) __syncthreads();
             for (uint32_t i = 0; i < n; ++i) {
                 const uint32_t k = turn0 + i, st = k % kStages;
-                live = live && __all_sync(0xFFFFFFFFu, mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin));
+                live = live && mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
                 if (!live) break;
-                rows.keys32(my_ring + st * kStageBytes, static_cast<int32_t>((first + 4u * i) * kPiece), there >> 2u * st & 3u, lane, my_q, my_meta);
+                rows.piece(my_ring + st * kStageBytes, static_cast<int32_t>((first + 4u * i) * kPiece), there >> 2u * st & 3u, lane, my_q, my_meta);
                 __syncwarp();
                 if (i + kStages < n) issue(i + kStages);
             }
@@ -741,16 +784,18 @@ kv_attention_kernel(AttnParams p) {
             };
             auto issue = [&](uint32_t i) {
                 const uint32_t st = (turn + i) % kStages, sub = 2u * (first + i);
-                fetch(my_ring + st * kStageBytes, my_bar + 8u * st, sub, page_at(sub), page_at(sub + 1u), kvh);
+                fetch(my_ring + st * kStageBytes, my_bar + 8u * st, sub, page_at(sub), page_at(sub + 1u));
             };
             if (tid == 0)
                 for (uint32_t i = 0; i < min(n, kStages); ++i) issue(i);
+            rows.load(p, sq, kvh, tile * TILE + warp * 8u, lane, my_q, 0u, 1u);
+            __syncwarp();
             for (uint32_t i = 0; i < n; ++i) {
                 const uint32_t k = turn + i, st = k % kStages, sub = 2u * (first + i);
-                live = live && __all_sync(0xFFFFFFFFu, mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin));
+                live = live && mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
                 const int32_t tok = static_cast<int32_t>(16u * sub);
                 if (live && tok < rows.most)
-                    rows.keys32(my_ring + st * kStageBytes, tok, (page_at(sub) >= 0 ? 1u : 0u) | (page_at(sub + 1u) >= 0 ? 2u : 0u), lane, my_q, my_meta);
+                    rows.piece(my_ring + st * kStageBytes, tok, (page_at(sub) >= 0 ? 1u : 0u) | (page_at(sub + 1u) >= 0 ? 2u : 0u), lane, my_q, my_meta);
                 live = __syncthreads_and(live);
                 if (!live) break;
                 if (tid == 0 && i + kStages < n) issue(i + kStages);
@@ -765,25 +810,24 @@ kv_attention_kernel(AttnParams p) {
         // ---- out, or a piece of it ----
         const bool whole = b0 == 0u && b1 == n_blocks;
         float* slot = p.part + (static_cast<size_t>(blockIdx.x) * 2u + (start >= x0 ? 1u : 0u)) * TILE * kPitch<HD>;
-        auto write = [&](uint32_t r, uint32_t d, float o, float l, bool seen) {
+        auto write = [&](uint32_t r, uint32_t d, const float(&o)[8], float l) {
             const uint32_t rr = tile * TILE + r, tok = rr / p.group, head = kvh * p.group + rr % p.group;
             if (tok >= sq.n_new) return;
             T* dst = static_cast<T*>(p.a.out) + static_cast<size_t>(sq.row0 + tok) * p.a.out_stride + static_cast<size_t>(head) * HD + d;
-            *dst = op_narrow<T>(seen ? o / l : 0.0f);
+            store_row(dst, o, l != 0.0f ? 1.0f / l : 0.0f, p.vec_out);      // rows that saw nothing: zeros
         };
         if constexpr (KEYS) {
-            for (uint32_t e = tid; e < 8u * HD; e += kThreads) {
-                const uint32_t r = e / HD, d = e % HD;
-                float m, l;
-                const float o = join<HD>(kWarps, d, [&](uint32_t i, uint32_t j) { return rows_of(i)[r * kPitch<HD> + j]; }, m, l);
+            for (uint32_t e = tid; e < HD; e += kThreads) {
+                const uint32_t r = e / (HD / 8u), d = e % (HD / 8u) * 8u;
+                float o[8], m, l;
+                join<HD>(kWarps, d, [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const float4*>(rows_of(i) + r * kPitch<HD> + j); }, o, m, l);
                 if (whole) {
-                    write(r, d, o, l, l != 0.0f);
+                    write(r, d, o, l);
                 } else {
-                    slot[r * kPitch<HD> + d] = o;
-                    if (d == 0) {
-                        slot[r * kPitch<HD> + HD] = m;
-                        slot[r * kPitch<HD> + HD + 1u] = l;
-                    }
+                    float4* to = reinterpret_cast<float4*>(slot + r * kPitch<HD> + d);
+                    to[0] = make_float4(o[0], o[1], o[2], o[3]);
+                    to[1] = make_float4(o[4], o[5], o[6], o[7]);
+                    if (d == 0) *reinterpret_cast<float4*>(slot + r * kPitch<HD> + HD) = make_float4(m, l, 0.0f, 0.0f);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the stages are copied into again
@@ -792,17 +836,12 @@ kv_attention_kernel(AttnParams p) {
             rows.store(slot + warp * 8u * kPitch<HD>, lane);
         } else {
             rows.finish(
-                lane,
-                [&](uint32_t r, uint32_t d, const float(&v)[8], float sum) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) write(warp * 8u + r, d + i, v[i], sum, sum != 0.0f);
-                },
-                [](uint32_t, float, float) {});
+                lane, [&](uint32_t r, uint32_t d, const float(&v)[8], float sum) { write(warp * 8u + r, d, v, sum); }, [](uint32_t, float, float) {});
         }
         if (!whole) {
             // CTA c has place v if floor(c total / ctas) <= v < floor((c + 1) total / ctas)
-            const uint32_t c0 = static_cast<uint32_t>(((start + 1u) * ctas - 1u) / total);
-            const uint32_t c1 = static_cast<uint32_t>(((start + n_blocks) * ctas - 1u) / total);
+            const uint32_t c0 = static_cast<uint32_t>(quotient((start + 1u) * ctas - 1u, total));
+            const uint32_t c1 = static_cast<uint32_t>(quotient((start + n_blocks) * ctas - 1u, total));
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -813,16 +852,17 @@ kv_attention_kernel(AttnParams p) {
             }
             __syncthreads();
             if (flag) {
-                for (uint32_t e = tid; e < TILE * HD; e += kThreads) {
-                    const uint32_t r = e / HD, d = e % HD;
-                    float m, l;
-                    const float o = join<HD>(
+                for (uint32_t e = tid; e < TILE * HD / 8u; e += kThreads) {
+                    const uint32_t r = e / (HD / 8u), d = e % (HD / 8u) * 8u;
+                    float o[8], m, l;
+                    join<HD>(
                         c1 - c0 + 1u, d,
                         [&](uint32_t i, uint32_t j) {   // past L1: other CTAs wrote these
-                            return __ldcg(p.part + ((static_cast<size_t>(c0 + i) * 2u + (i == 0u ? 1u : 0u)) * TILE + r) * kPitch<HD> + j);
+                            return __ldcg(reinterpret_cast<const float4*>(
+                                p.part + ((static_cast<size_t>(c0 + i) * 2u + (i == 0u ? 1u : 0u)) * TILE + r) * kPitch<HD> + j));
                         },
-                        m, l);
-                    write(r, d, o, l, l != 0.0f);
+                        o, m, l);
+                    write(r, d, o, l);
                 }
             }
             __syncthreads();
@@ -873,6 +913,7 @@ void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim,
     p.spin = ctx->spin_limit_barrier;
     const size_t es = dtype == CSDR_DTYPE_F32 ? 4 : 2;
     p.vec = (reinterpret_cast<uintptr_t>(a.q) | a.q_stride * es) % 16u == 0;
+    p.vec_out = (reinterpret_cast<uintptr_t>(a.out) | a.out_stride * es) % 16u == 0;
     // rows of a sequence that share keys: from two tiles of eight on, warps with rows of their own
     const bool keys = static_cast<uint64_t>(b.n_tokens) * p.group < 16u * static_cast<uint64_t>(b.n_seqs);
     LaunchScope ls(ctx, KC_KV_ATTENTION);
