@@ -8,6 +8,7 @@
 // step). A group that holds a value that is not finite reads back as NaN; |x| past 65504 saturates.
 #include <algorithm>
 
+#include "codes4.cuh"
 #include "kv_cache.hpp"
 #include "op_common.cuh"
 

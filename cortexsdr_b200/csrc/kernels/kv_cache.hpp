@@ -19,15 +19,7 @@ constexpr uint32_t kKvBlock = 16;    // tokens of a block, the unit of the layou
 //            values 64 u + 8 g + 4 x + 0 .. 3 of the even token in its low half and of the odd one in its high half
 //   (fp16 minimum, fp16 step in the upper half) of the keys' groups, [group][token], then of the values'
 // so that a lane of the attention kernel finds what its matrix fragments take in one piece each, and a block is one
-// contiguous copy. The four codes of a half lie where a mask, after a shift by four bits or an exchange of the
-// half's bytes, leaves each of them in bits 6 - 9 (pack_codes).
-__host__ __device__ inline uint32_t pack_codes(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3) {
-    return c0 << 6 | c1 << 2 | (c2 & 3u) << 14 | c2 >> 2 | c3 << 10;
-}
-__host__ __device__ inline uint32_t unpack_code(uint32_t half, uint32_t n) {
-    return n == 0u ? half >> 6 & 15u : n == 1u ? half >> 2 & 15u : n == 2u ? (half >> 14 & 3u) | (half & 3u) << 2 : half >> 10 & 15u;
-}
-
+// contiguous copy. Codes of a half: codes4.cuh.
 struct KvView {
     uint8_t* base = nullptr;
     uint32_t n_pages = 0, kv_heads = 0, page_shift = 0;   // tokens of a page: 1 << page_shift
