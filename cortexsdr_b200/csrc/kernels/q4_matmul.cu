@@ -84,6 +84,7 @@ struct Q4Params {
     uint32_t n_blocks;          // of 128 rows
     uint32_t units_rank;        // units of a row tile that a CTA of a cluster takes
     uint32_t units_staged;      // of those, units whose activations fit into shared memory at a time
+    uint32_t x_vec;             // a token's columns lie one behind the other and start on 16 bytes
 };
 
 template <int FMT, int NT, bool SPLIT>
@@ -95,11 +96,28 @@ struct Q4Shape {
     static constexpr uint32_t kSumBytes = 2u * kRowsBlock * kTokens * 4u;      // partial results, twice
 };
 
-__device__ __forceinline__ float load_x(const Q4Args& a, size_t tok, size_t col) {
-    const size_t i = tok * a.x_token + col * a.x_col;
-    if (a.x_dtype == CSDR_DTYPE_F32) return static_cast<const float*>(a.x)[i];
-    if (a.x_dtype == CSDR_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.x)[i]);
-    return __half2float(static_cast<const __half*>(a.x)[i]);
+// Eight neighbouring columns of a token; what lies behind the matrix is zero.
+template <typename T>
+__device__ __forceinline__ void load8(const Q4Params& p, size_t tok, uint32_t col, float (&v)[8]) {
+    const T* x = static_cast<const T*>(p.a.x) + tok * p.a.x_token + static_cast<size_t>(col) * p.a.x_col;
+    if (p.x_vec) {       // columns come in multiples of 32
+        if (col >= p.w.cols) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) v[i] = 0.0f;
+            return;
+        }
+        constexpr uint32_t N = 16u / sizeof(T);
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i += N) {
+            const uint4 q = *reinterpret_cast<const uint4*>(x + i);
+            const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) v[i + j] = op_widen(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) v[i] = col + i < p.w.cols ? op_widen(x[i * p.a.x_col]) : 0.0f;
+    }
 }
 
 // A lane's pieces of a unit: codes (pairs of groups), steps of rows g and g + 8.
@@ -125,11 +143,13 @@ struct Q4Unit {
 __device__ __forceinline__ uint32_t word_of(const uint4& v, uint32_t i) { return i == 0u ? v.x : i == 1u ? v.y : i == 2u ? v.z : v.w; }
 __device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-template <int FMT, int NT, bool SPLIT>
+template <typename T, int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, 2)
 q4_matmul_kernel(Q4Params p) {
+    constexpr bool SPLIT = std::is_same<T, float>::value;
     using S = Q4Shape<FMT, NT, SPLIT>;
     constexpr uint32_t kBytes = q4_unit_bytes(FMT), kAhead = FMT ? 2u : 4u;
+    constexpr bool kScaled = !std::is_same<T, __half>::value;       // fp16 activations are operands as they come
     extern __shared__ __align__(16) uint8_t smem[];
     float* part = reinterpret_cast<float*>(smem);                             // [2][tokens][128 rows]
     uint8_t* xs = smem + S::kSumBytes;                                        // [unit][group][column][t] 16 bytes
@@ -162,25 +182,36 @@ q4_matmul_kernel(Q4Params p) {
     // ---- activations: a power of two for each token brings its largest below 2^15 ----
     for (uint32_t i = tid; i < S::kTokens; i += kThreads) largest[i] = 0u;
     __syncthreads();
-    {
+    if constexpr (kScaled) {
         const uint32_t c0 = u_begin * S::kUnitCols, c1 = min(u_end * S::kUnitCols, p.w.cols);
-        if (p.a.x_col == 1) {
-            for (uint32_t tok = 0; tok < n_tok; ++tok) {
-                float big = 0.0f;
-                for (uint32_t c = c0 + tid; c < c1; c += kThreads) big = fmaxf(big, fabsf(load_x(p.a, tok0 + tok, c)));
-                const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(big));
-                if (lane == 0 && m) atomicMax(&largest[tok], m);
+        if (p.a.x_col == 1) {       // a warp a token
+            for (uint32_t tok = warp; tok < n_tok; tok += kThreads / 32u) {
+                uint32_t big = 0;
+#pragma unroll 4
+                for (uint32_t c = c0 + lane * 8u; c < c1; c += 256u) {
+                    float v[8];
+                    load8<T>(p, tok0 + tok, c, v);
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i) big = max(big, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+                }
+                big = __reduce_max_sync(0xFFFFFFFFu, big);
+                if (lane == 0) largest[tok] = big;
             }
-        } else {
-            for (uint32_t e = tid; e < (c1 > c0 ? c1 - c0 : 0u) * n_tok; e += kThreads) {
-                const uint32_t m = __float_as_uint(fabsf(load_x(p.a, tok0 + e % n_tok, c0 + e / n_tok)));
-                if (m) atomicMax(&largest[e % n_tok], m < 0x7F800001u ? m : 0x7F800000u);
+        } else {                    // neighbouring threads have neighbouring tokens
+            const uint32_t each = kThreads / n_tok, tok = tid % n_tok;
+            const T* x = static_cast<const T*>(p.a.x) + (tok0 + tok) * p.a.x_token;
+            uint32_t big = 0;
+            if (tid / n_tok < each) {
+#pragma unroll 4
+                for (uint32_t c = c0 + tid / n_tok; c < c1; c += each) big = max(big, __float_as_uint(op_widen(x[static_cast<size_t>(c) * p.a.x_col])) & 0x7FFFFFFFu);
+                atomicMax(&largest[tok], big);
             }
         }
     }
     __syncthreads();
     // what is not finite stays as it is; 2^-100 counts as the smallest
     auto exponent = [&](uint32_t tok) {
+        if constexpr (!kScaled) return 14;
         const uint32_t b = largest[tok];
         return b == 0u || b >= 0x7F800000u ? 14 : max(static_cast<int>(b >> 23) - 127, -100);
     };
@@ -190,14 +221,16 @@ q4_matmul_kernel(Q4Params p) {
         for (uint32_t e0 = 0; e0 < items; e0 += kThreads) {
             const uint32_t e = e0 + tid;
             // neighbouring threads: the four pieces of a group, then tokens or groups, whichever lie closer
-            const uint32_t piece = e & 3u, rest = e >> 2, gr = rest / n_tok, tok = rest % n_tok;
+            const uint32_t piece = e & 3u, rest = e >> 2, groups = (u1 - u0) * S::kGroups;
+            const uint32_t gr = p.a.x_col == 1 ? rest % groups : rest / n_tok, tok = p.a.x_col == 1 ? rest / groups : rest % n_tok;
             float v[8], sum_hi = 0.0f, sum_lo = 0.0f;
             uint32_t hi[4], lo[4];
             if (e < items) {
                 const float up = power_of_two(14 - exponent(tok));
                 const uint32_t col = (u0 * S::kGroups + gr) * 32u + piece * 8u;
+                load8<T>(p, tok0 + tok, col, v);
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) v[i] = col + i < p.w.cols ? load_x(p.a, tok0 + tok, col + i) * up : 0.0f;
+                for (uint32_t i = 0; i < 8u; ++i) v[i] *= up;
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i) {
                     if constexpr (SPLIT) {
@@ -343,17 +376,9 @@ q4_matmul_kernel(Q4Params p) {
         }
         if (ranks > 1u) cluster.sync();
         else __syncthreads();
-        // a rank adds up its share of the rows
-        const uint32_t rows = kRowsBlock / ranks;
-        for (uint32_t e = tid; e < rows * n_tok; e += kThreads) {
-            uint32_t r, tok;
-            if (p.a.y_row == 1) {
-                tok = e / rows;
-                r = rank * rows + e % rows;
-            } else {
-                tok = e % n_tok;
-                r = rank * rows + e / n_tok;
-            }
+        // a rank adds up its share
+        for (uint32_t e = rank * kThreads + tid; e < kRowsBlock * n_tok; e += ranks * kThreads) {
+            const uint32_t r = p.a.y_row == 1 ? e % kRowsBlock : e / n_tok, tok = p.a.y_row == 1 ? e / kRowsBlock : e % n_tok;
             const size_t row = static_cast<size_t>(block) * kRowsBlock + r;
             if (row >= p.w.rows) continue;
             float sum = p.a.bias ? p.a.bias[row] : 0.0f;
@@ -365,40 +390,41 @@ q4_matmul_kernel(Q4Params p) {
     if (ranks > 1u) cluster.sync();      // others may still read this CTA's shared memory
 }
 
-template <int FMT, int NT, bool SPLIT>
+template <typename T, int FMT, int NT>
 void launch(csdr_context* ctx, Q4Params p) {
-    using S = Q4Shape<FMT, NT, SPLIT>;
-    const uint32_t tiles = (p.w.rows + 15u) / 16u;
+    using S = Q4Shape<FMT, NT, std::is_same<T, float>::value>;
     p.n_blocks = (p.w.rows + kRowsBlock - 1u) / kRowsBlock;
-    // Columns are cut until there are sixteen warps for every SM, or a unit a warp, and further while the activations of
-    // a cut do not fit beside another CTA's. 4096 rows of 4096: 8 cuts 5.3 us.
     constexpr uint32_t kMostStaged = (96u * 1024u - S::kSumBytes) / S::kStageBytes;
-    uint32_t ranks = 1;
-    while (ranks < 8u && ranks < p.w.n_units &&
-           (tiles * ranks < static_cast<uint32_t>(ctx->sm_count) * 16u || (p.w.n_units + ranks - 1u) / ranks > kMostStaged))
-        ranks *= 2u;
+    // Two CTAs an SM. Cut the columns so that the CTA with most to do has least: blocks in turn, each its units and about
+    // two more for the join. A cut whose activations do not fit at a time stages them anew for every block.
+    const uint32_t slots = static_cast<uint32_t>(ctx->sm_count) * 2u;
+    uint32_t ranks = 1, least = UINT32_MAX;
+    for (uint32_t r = 1; r <= 8u && r <= p.w.n_units; ++r) {
+        const uint32_t units = (p.w.n_units + r - 1u) / r, clusters = slots / r;
+        const uint32_t turns = (p.n_blocks + clusters - 1u) / clusters;
+        const uint32_t cost = turns * (units * (units > kMostStaged ? 3u : 1u) + 2u);
+        if (cost < least) {
+            least = cost;
+            ranks = r;
+        }
+    }
     p.units_rank = (p.w.n_units + ranks - 1u) / ranks;
     p.units_staged = std::min(p.units_rank, kMostStaged);
     const size_t smem = S::kSumBytes + static_cast<size_t>(p.units_staged) * S::kStageBytes;
-    auto kern = q4_matmul_kernel<FMT, NT, SPLIT>;
+    p.x_vec = p.a.x_col == 1 && (reinterpret_cast<uintptr_t>(p.a.x) | p.a.x_token * sizeof(T)) % 16u == 0;
+    auto kern = q4_matmul_kernel<T, FMT, NT>;
     ctx->opt_in_smem(reinterpret_cast<const void*>(kern), smem);
-    const uint32_t clusters = std::max(1u, std::min(p.n_blocks, static_cast<uint32_t>(ctx->sm_count) * 2u / ranks));
+    const uint32_t clusters = std::min(p.n_blocks, slots / ranks);
     const dim3 grid(clusters * ranks, static_cast<unsigned>((p.a.batch + S::kTokens - 1u) / S::kTokens));
     launch_op(ctx, kern, grid, kThreads, smem, ranks, p);
 }
 
-template <int FMT>
-void launch_format(csdr_context* ctx, const Q4Params& p) {
-    const size_t m = p.a.batch;
-    if (p.a.x_dtype == CSDR_DTYPE_F32) {
-        if (m <= 4) launch<FMT, 1, true>(ctx, p);
-        else if (m <= 8) launch<FMT, 2, true>(ctx, p);
-        else launch<FMT, 4, true>(ctx, p);
-    } else {
-        if (m <= 8) launch<FMT, 1, false>(ctx, p);
-        else if (m <= 16) launch<FMT, 2, false>(ctx, p);
-        else launch<FMT, 4, false>(ctx, p);
-    }
+template <typename T, int FMT>
+void launch_tokens(csdr_context* ctx, const Q4Params& p) {
+    const size_t m = p.a.batch * (std::is_same<T, float>::value ? 2u : 1u);
+    if (m <= 8) launch<T, FMT, 1>(ctx, p);
+    else if (m <= 16) launch<T, FMT, 2>(ctx, p);
+    else launch<T, FMT, 4>(ctx, p);
 }
 
 }  // namespace
@@ -423,8 +449,11 @@ void launch_q4_matmul(csdr_context* ctx, const Q4View& w, const Q4Args& a) {
         p.a.x = static_cast<const uint8_t*>(a.x) + t0 * a.x_token * (a.x_dtype == CSDR_DTYPE_F32 ? 4u : 2u);
         p.a.y = a.y + t0 * a.y_token;
         LaunchScope ls(ctx, KC_Q4);
-        if (w.format == 0) launch_format<0>(ctx, p);
-        else launch_format<1>(ctx, p);
+        with_dtype(a.x_dtype, [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            if (w.format == 0) launch_tokens<T, 0>(ctx, p);
+            else launch_tokens<T, 1>(ctx, p);
+        });
         ls.done("q4_matmul_kernel");
     }
 }
