@@ -9,13 +9,14 @@
 // W warps, of the warps' ceil(k / W)-th best so far (in the first round: of the lanes' maxima, before any is in a
 // list). Some hundred logits of a row reach it; a row in rising order, where all do, is slow and right.
 // Keys are (logit, index), so neither lists nor results depend on who comes first. Few rows are cut over the CTAs of a
-// cluster, whose leader joins them. What bounds it: the logits' bytes; exponentials and comparisons come to eight
-// operations a 16-bit logit, some 0.8 of the issue slots at the memory's rate.
+// cluster, whose leader joins them. What bounds it: the logits' bytes, and behind them the exponentials (one a logit,
+// sixteen a clock and SM: 0.7 of the memory's time for 16-bit logits); the rest is packed by twos.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 #include <cfloat>
 
+#include "codes4.cuh"
 #include "logprobs.hpp"
 #include "op_common.cuh"
 
@@ -25,7 +26,7 @@ namespace csdr {
 
 namespace {
 
-constexpr uint32_t kThreads = 512, kWarps = kThreads / 32, kRound = 4;     // 128-bit loads a thread has under way
+constexpr uint32_t kRound = 4;     // 128-bit loads a thread has under way
 typedef unsigned long long u64;
 
 // Orders as the logits do; above zero for every logit.
@@ -46,11 +47,11 @@ __device__ __forceinline__ float ex2(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Maximum, sum of exp(x - maximum), sum of exp(x - maximum) (x - maximum).
+// Maximum, sum of p = exp(x - maximum), sum of p log2 p.
 struct Sums {
     float m = -FLT_MAX, s = 0.0f, e = 0.0f;
     __device__ __forceinline__ void raise(float top) {
-        const float d = fmaxf(m - top, -1000.0f), f = ex2(d * kLog2e);      // an empty sum has no distance
+        const float d = fmaxf((m - top) * kLog2e, -1000.0f), f = ex2(d);      // an empty sum has no distance
         e = f * fmaf(d, s, e);
         s *= f;
         m = top;
@@ -63,28 +64,57 @@ struct Sums {
         s += b.s;
         e += b.e;
     }
+    // One logit, not above the maximum. (x - m is exact near the maximum; products with log2 e are not)
+    __device__ __forceinline__ void one(float x) {
+        const float d = (x - m) * kLog2e, p = ex2(d);
+        s += p;
+        e = fmaf(p, fmaxf(d, -1000.0f), e);
+    }
 };
 
+// A 128-bit piece: pairs of logits, and the greatest.
 template <typename T>
-struct Vec {
-    static constexpr uint32_t N = 16u / sizeof(T);
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr uint32_t N = 4;
     uint4 w;
-    __device__ __forceinline__ float operator[](uint32_t i) const;
+    __device__ __forceinline__ float2 pair(uint32_t i) const {
+        return i ? make_float2(__uint_as_float(w.z), __uint_as_float(w.w)) : make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+    }
+    __device__ __forceinline__ float top() const {
+        return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    }
+};
+__device__ __forceinline__ uint32_t word_of(const uint4& w, uint32_t i) { return i == 0u ? w.x : i == 1u ? w.y : i == 2u ? w.z : w.w; }
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr uint32_t N = 8;
+    uint4 w;
+    __device__ __forceinline__ float2 pair(uint32_t i) const {
+        const uint32_t p = word_of(w, i);
+        return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xFFFF0000u));
+    }
+    __device__ __forceinline__ float top() const {
+        auto h = [&](uint32_t i) { const uint32_t p = word_of(w, i); return *reinterpret_cast<const __nv_bfloat162*>(&p); };
+        const __nv_bfloat162 m = __hmax2(__hmax2(h(0), h(1)), __hmax2(h(2), h(3)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
 };
 template <>
-__device__ __forceinline__ float Vec<float>::operator[](uint32_t i) const {
-    return __uint_as_float(i == 0u ? w.x : i == 1u ? w.y : i == 2u ? w.z : w.w);
-}
-template <>
-__device__ __forceinline__ float Vec<__nv_bfloat16>::operator[](uint32_t i) const {
-    const uint32_t p = i / 2u == 0u ? w.x : i / 2u == 1u ? w.y : i / 2u == 2u ? w.z : w.w;
-    return __uint_as_float(i & 1u ? p & 0xFFFF0000u : p << 16);
-}
-template <>
-__device__ __forceinline__ float Vec<__half>::operator[](uint32_t i) const {
-    const uint32_t p = i / 2u == 0u ? w.x : i / 2u == 1u ? w.y : i / 2u == 2u ? w.z : w.w;
-    return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1u ? p >> 16 : p)));
-}
+struct Vec<__half> {
+    static constexpr uint32_t N = 8;
+    uint4 w;
+    __device__ __forceinline__ float2 pair(uint32_t i) const {
+        const uint32_t p = word_of(w, i);
+        return __half22float2(*reinterpret_cast<const __half2*>(&p));
+    }
+    __device__ __forceinline__ float top() const {
+        auto h = [&](uint32_t i) { const uint32_t p = word_of(w, i); return *reinterpret_cast<const __half2*>(&p); };
+        const __half2 m = __hmax2(__hmax2(h(0), h(1)), __hmax2(h(2), h(3)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+};
 
 // The warp's list: lane i has the i-th greatest key, zero where there is none.
 __device__ __forceinline__ void insert(u64& list, u64 key, uint32_t lane) {
@@ -104,6 +134,7 @@ __device__ __forceinline__ uint32_t nth_greatest(uint32_t v, uint32_t j) {
     return top;
 }
 
+template <uint32_t kWarps>
 struct Shared {
     Sums sums[kWarps];
     Sums joined;                 // of this CTA
@@ -113,10 +144,11 @@ struct Shared {
     uint32_t count;
 };
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 2)
+template <typename T, bool TOP, uint32_t kThreads>
+__global__ void __launch_bounds__(kThreads, 768 / kThreads)
 logprob_kernel(LogprobArgs a) {
-    __shared__ Shared sh;
+    constexpr uint32_t kWarps = kThreads / 32;
+    __shared__ Shared<kWarps> sh;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
@@ -149,24 +181,26 @@ logprob_kernel(LogprobArgs a) {
         bound = max(bound, __reduce_min_sync(0xFFFFFFFFu, b));
         reach = bound ? logit_of(bound) : -INFINITY;
     };
-    bool first = true;
-    for (uint32_t base = v0; base < v1 || first; base += kThreads * kRound) {
-        Vec<T> w[kRound];
-        float top[kRound], most = -FLT_MAX;
+    Vec<T> w[kRound], ahead[kRound];
+    auto fetch = [&](uint32_t base) {
 #pragma unroll
         for (uint32_t j = 0; j < kRound; ++j) {
             const uint32_t i = base + j * kThreads + tid;
-            if (i < v1) w[j].w = __ldcs(vec + i);
+            ahead[j].w = make_uint4(0u, 0u, 0u, 0u);
+            if (i < v1) ahead[j].w = __ldcs(vec + i);
         }
+    };
+    fetch(v0);
+    bool first = true;
+    for (uint32_t base = v0; base < v1 || first; base += kThreads * kRound) {
+        float top[kRound], most = -FLT_MAX;
 #pragma unroll
         for (uint32_t j = 0; j < kRound; ++j) {
-            top[j] = -INFINITY;
-            if (base + j * kThreads + tid < v1) {
-#pragma unroll
-                for (uint32_t e = 0; e < N; ++e) top[j] = fmaxf(top[j], w[j][e]);
-            }
+            w[j] = ahead[j];
+            top[j] = base + j * kThreads + tid < v1 ? w[j].top() : -INFINITY;
             most = fmaxf(most, top[j]);
         }
+        if (base + kThreads * kRound < v1) fetch(base + kThreads * kRound);
         if (TOP) {
             if (first) {
                 // so many lanes have a logit of at least this
@@ -177,27 +211,55 @@ logprob_kernel(LogprobArgs a) {
             new_bound();
         }
         if (most > mine.m) mine.raise(most);
-        const float m = mine.m;
+        const f32x2 less = pack2(-mine.m, -mine.m), log2e = pack2(kLog2e, kLog2e);
+        f32x2 s2 = pack2(0.0f, 0.0f), e2 = s2;
 #pragma unroll
         for (uint32_t j = 0; j < kRound; ++j) {
-            const uint32_t i = base + j * kThreads + tid;
-            const bool there = i < v1;
-            if (there) {
+            if (base + j * kThreads + tid >= v1) break;
 #pragma unroll
-                for (uint32_t e = 0; e < N; ++e) {
-                    const float d = w[j][e] - m, p = ex2(d * kLog2e);
-                    mine.s += p;
-                    mine.e = fmaf(p, fmaxf(d, -1000.0f), mine.e);     // exp(-infinity) counts as nothing
-                }
-            }
-            if (TOP && __any_sync(0xFFFFFFFFu, there && !(top[j] < reach))) {
-#pragma unroll
-                for (uint32_t e = 0; e < N; ++e) consider(w[j][e], head + i * N + e, there);
+            for (uint32_t i = 0; i < Vec<T>::N / 2u; ++i) {
+                const float2 v = w[j].pair(i);
+                const f32x2 d = mul2(add2(pack2(v.x, v.y), less), log2e);
+                const float2 y = unpack2(d);
+                const f32x2 q = pack2(ex2(y.x), ex2(y.y));
+                s2 = add2(s2, q);
+                e2 = fma2(q, d, e2);
             }
         }
+        {
+            const float2 sv = unpack2(s2), ev = unpack2(e2);
+            float e = ev.x + ev.y;
+            if (e != e) {        // a -infinity, which counts as nothing (or a NaN, which the sum has too)
+                e = 0.0f;
+#pragma unroll
+                for (uint32_t j = 0; j < kRound; ++j) {
+                    if (base + j * kThreads + tid >= v1) break;
+#pragma unroll
+                    for (uint32_t i = 0; i < Vec<T>::N / 2u; ++i) {
+                        const float2 v = w[j].pair(i);
+                        const float dx = fmaxf((v.x - mine.m) * kLog2e, -1000.0f), dy = fmaxf((v.y - mine.m) * kLog2e, -1000.0f);
+                        e = fmaf(ex2(dx), dx, fmaf(ex2(dy), dy, e));
+                    }
+                }
+            }
+            mine.s += sv.x + sv.y;
+            mine.e += e;
+        }
         if (TOP) {
+#pragma unroll
+            for (uint32_t j = 0; j < kRound; ++j) {
+                const uint32_t i = base + j * kThreads + tid;
+                const bool there = i < v1;
+                if (!__any_sync(0xFFFFFFFFu, there && !(top[j] < reach))) continue;
+#pragma unroll
+                for (uint32_t e = 0; e < Vec<T>::N / 2u; ++e) {
+                    const float2 v = w[j].pair(e);
+                    consider(v.x, head + i * N + 2u * e, there);
+                    consider(v.y, head + i * N + 2u * e + 1u, there);
+                }
+            }
             const uint32_t b = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, list, share - 1u) >> 32);
-            if (lane == 0 && b > sh.bound[warp]) sh.bound[warp] = b;
+            if (lane == 0 && b > sh.bound[warp]) *reinterpret_cast<volatile uint32_t*>(&sh.bound[warp]) = b;
         }
         first = false;
     }
@@ -209,9 +271,7 @@ logprob_kernel(LogprobArgs a) {
         const float v = there ? op_widen(x[i]) : 0.0f;
         if (there) {
             if (v > mine.m) mine.raise(v);
-            const float d = v - mine.m, p = ex2(d * kLog2e);
-            mine.s += p;
-            mine.e = fmaf(p, fmaxf(d, -1000.0f), mine.e);
+            mine.one(v);
         }
         if (TOP) consider(v, i, there);
     }
@@ -227,18 +287,27 @@ logprob_kernel(LogprobArgs a) {
     if (lane == 0) sh.sums[warp] = mine;
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    if (tid == 0) {
-        Sums all = sh.sums[0];
-        for (uint32_t i = 1; i < kWarps; ++i) all.add(sh.sums[i]);
-        sh.joined = all;
+    if (warp == 0) {
+        Sums all = sh.sums[lane % kWarps];
+#pragma unroll
+        for (uint32_t o = kWarps / 2u; o; o >>= 1) {
+            Sums b;
+            b.m = __shfl_xor_sync(0xFFFFFFFFu, all.m, o);
+            b.s = __shfl_xor_sync(0xFFFFFFFFu, all.s, o);
+            b.e = __shfl_xor_sync(0xFFFFFFFFu, all.e, o);
+            all.add(b);
+        }
+        if (lane == 0) sh.joined = all;
     }
-    // The best of n keys in `from`, in order: a key's place is the number of greater ones (keys differ).
+    // The best of n keys in `from`, in order: a key's place is the number of greater ones (keys differ, but for zeros,
+    // which stand for none).
     auto rank_keys = [&](const u64* from, uint32_t n, u64* to) {
         for (uint32_t i = tid; i < n; i += kThreads) {
             const u64 key = from[i];
             uint32_t at = 0;
-            for (uint32_t j = 0; j < n && at < k; ++j) at += from[j] > key;
-            if (at < k) to[at] = key;
+#pragma unroll 8
+            for (uint32_t j = 0; j < n; ++j) at += from[j] > key;
+            if (at < k && key) to[at] = key;
         }
     };
     if (TOP) {
@@ -262,7 +331,6 @@ logprob_kernel(LogprobArgs a) {
             if (TOP) {
                 for (uint32_t i = tid; i < ranks * k; i += kThreads) sh.keys[i] = cluster.map_shared_rank(sh.best, i / k)[i % k];
                 __syncthreads();
-                // a CTA with fewer than k logits leaves zeros, which rank behind every key
                 rank_keys(sh.keys, ranks * k, sh.best);
                 __syncthreads();
             }
@@ -274,7 +342,7 @@ logprob_kernel(LogprobArgs a) {
                 const int32_t t = a.targets[row];
                 a.logprob[row] = fine && t >= 0 && static_cast<uint32_t>(t) < a.vocab ? op_widen(x[t]) - all.m - ls : NAN;
             }
-            if (a.entropy) a.entropy[row] = fine ? ls - all.e / all.s : NAN;
+            if (a.entropy) a.entropy[row] = fine ? ls - all.e / all.s * 0.6931471805599453f : NAN;
         }
         if (TOP && tid < k) {
             const u64 key = sh.best[tid];
@@ -292,14 +360,19 @@ void launch_logprobs(csdr_context* ctx, int dtype, const LogprobArgs& a) {
     LaunchScope ls(ctx, KC_LOGPROB);
     with_dtype(dtype, [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        // two CTAs an SM; a row is cut while that leaves some idle and its parts are longer than a round
+        // three CTAs of 256 threads an SM; where a row is cut because there are few, one of 512
         uint32_t ranks = 1;
-        while (ranks < 8u && static_cast<uint64_t>(a.rows) * ranks * 2u <= static_cast<uint64_t>(ctx->sm_count) * 2u &&
-               a.vocab / (ranks * 2u) >= kThreads * Vec<T>::N)
+        while (ranks < 8u && static_cast<uint64_t>(a.rows) * ranks * 2u <= static_cast<uint64_t>(ctx->sm_count) &&
+               a.vocab / (ranks * 2u) >= 512u * Vec<T>::N)
             ranks *= 2u;
         const dim3 grid(a.rows * ranks);
-        if (a.top) launch_op(ctx, logprob_kernel<T, true>, grid, kThreads, 0, ranks, a);
-        else launch_op(ctx, logprob_kernel<T, false>, grid, kThreads, 0, ranks, a);
+        if (ranks == 1u) {
+            if (a.top) launch_op(ctx, logprob_kernel<T, true, 256>, grid, 256, 0, 1, a);
+            else launch_op(ctx, logprob_kernel<T, false, 256>, grid, 256, 0, 1, a);
+        } else {
+            if (a.top) launch_op(ctx, logprob_kernel<T, true, 512>, grid, 512, 0, ranks, a);
+            else launch_op(ctx, logprob_kernel<T, false, 512>, grid, 512, 0, ranks, a);
+        }
     });
     ls.done("logprob_kernel");
 }
