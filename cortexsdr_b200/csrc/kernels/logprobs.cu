@@ -140,7 +140,9 @@ struct Shared {
     Sums joined;                 // of this CTA
     uint32_t bound[kWarps];      // each warp's: an order that so many of its logits reach
     u64 keys[kWarps * kMaxTop];
-    u64 best[kMaxTop];           // of this CTA
+    u64 best[kMaxTop];           // of this CTA; the leader's: of the row
+    Sums parts[8];               // the leader's: of every CTA of the cluster
+    u64 offered[8 * kMaxTop];
     uint32_t count;
 };
 
@@ -152,6 +154,8 @@ logprob_kernel(LogprobArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    // what the others write into the leader's shared memory needs it to be there
+    if (ranks > 1u) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     op_enter();
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
     constexpr uint32_t N = Vec<T>::N;
@@ -182,11 +186,26 @@ logprob_kernel(LogprobArgs a) {
         reach = bound ? logit_of(bound) : -INFINITY;
     };
     Vec<T> w[kRound], ahead[kRound];
+    // The pieces of the lanes in `who`, one lane's after the other: its logits spread over the lanes.
+    auto consider_pieces = [&](uint32_t who, const Vec<T>& v, uint32_t i) {
+        while (who) {
+            const uint32_t from = __ffs(who) - 1u;
+            who &= who - 1u;
+            Vec<T> one;
+            one.w.x = __shfl_sync(0xFFFFFFFFu, v.w.x, from);
+            one.w.y = __shfl_sync(0xFFFFFFFFu, v.w.y, from);
+            one.w.z = __shfl_sync(0xFFFFFFFFu, v.w.z, from);
+            one.w.w = __shfl_sync(0xFFFFFFFFu, v.w.w, from);
+            const uint32_t at = head + __shfl_sync(0xFFFFFFFFu, i, from) * N + lane;
+            const uint32_t pr = lane / 2u % (N / 2u);
+            const float2 f = pr < 2u ? (pr & 1u ? one.pair(1) : one.pair(0)) : (pr & 1u ? one.pair(N / 2u - 1u) : one.pair(N / 2u - 2u));
+            consider(lane & 1u ? f.y : f.x, at, lane < N);
+        }
+    };
     auto fetch = [&](uint32_t base) {
 #pragma unroll
         for (uint32_t j = 0; j < kRound; ++j) {
             const uint32_t i = base + j * kThreads + tid;
-            ahead[j].w = make_uint4(0u, 0u, 0u, 0u);
             if (i < v1) ahead[j].w = __ldcs(vec + i);
         }
     };
@@ -249,14 +268,8 @@ logprob_kernel(LogprobArgs a) {
 #pragma unroll
             for (uint32_t j = 0; j < kRound; ++j) {
                 const uint32_t i = base + j * kThreads + tid;
-                const bool there = i < v1;
-                if (!__any_sync(0xFFFFFFFFu, there && !(top[j] < reach))) continue;
-#pragma unroll
-                for (uint32_t e = 0; e < Vec<T>::N / 2u; ++e) {
-                    const float2 v = w[j].pair(e);
-                    consider(v.x, head + i * N + 2u * e, there);
-                    consider(v.y, head + i * N + 2u * e + 1u, there);
-                }
+                const uint32_t who = __ballot_sync(0xFFFFFFFFu, i < v1 && !(top[j] < reach));
+                if (who) consider_pieces(who, w[j], i);
             }
             const uint32_t b = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, list, share - 1u) >> 32);
             if (lane == 0 && b > sh.bound[warp]) *reinterpret_cast<volatile uint32_t*>(&sh.bound[warp]) = b;
@@ -322,16 +335,28 @@ logprob_kernel(LogprobArgs a) {
         __syncthreads();
         rank_keys(sh.keys, sh.count, sh.best);
     }
-    if (ranks > 1u) cluster.sync();
-    else __syncthreads();
+    if (ranks > 1u) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        __syncthreads();
+        if (tid == 0) *cluster.map_shared_rank(&sh.parts[rank], 0) = sh.joined;
+        if (TOP && tid < k) cluster.map_shared_rank(sh.offered, 0)[rank * k + tid] = sh.best[tid];
+        cluster.sync();
+    } else {
+        __syncthreads();
+    }
     if (rank == 0) {
         Sums all = sh.joined;
         if (ranks > 1u) {
-            for (uint32_t r = 1; r < ranks; ++r) all.add(*cluster.map_shared_rank(&sh.joined, r));
+            all = sh.parts[lane % ranks];
+            for (uint32_t o = ranks / 2u; o; o >>= 1) {
+                Sums b;
+                b.m = __shfl_xor_sync(0xFFFFFFFFu, all.m, o);
+                b.s = __shfl_xor_sync(0xFFFFFFFFu, all.s, o);
+                b.e = __shfl_xor_sync(0xFFFFFFFFu, all.e, o);
+                all.add(b);
+            }
             if (TOP) {
-                for (uint32_t i = tid; i < ranks * k; i += kThreads) sh.keys[i] = cluster.map_shared_rank(sh.best, i / k)[i % k];
-                __syncthreads();
-                rank_keys(sh.keys, ranks * k, sh.best);
+                rank_keys(sh.offered, ranks * k, sh.best);
                 __syncthreads();
             }
         }
@@ -351,7 +376,6 @@ logprob_kernel(LogprobArgs a) {
             a.top_logprobs[at] = fine ? logit_of(static_cast<uint32_t>(key >> 32)) - all.m - ls : NAN;
         }
     }
-    if (ranks > 1u) cluster.sync();      // the leader may still read this CTA's shared memory
 }
 
 }  // namespace
