@@ -4,13 +4,14 @@
 // +infinity among the logits, or nothing above -infinity) answers NaN, and -1 for the ids.
 //
 // One pass over the logits. A thread keeps the maximum, the sum and the weighted sum of what it has seen, scaled anew
-// when the maximum grows. For the alternatives a warp keeps a sorted list of the best it has met, a key a lane; a logit
-// is looked at only if it reaches a bound that the k-th best of the row cannot be below: the least, over the CTA's
-// W warps, of the warps' ceil(k / W)-th best so far (in the first round: of the lanes' maxima, before any is in a
-// list). Some hundred logits of a row reach it; a row in rising order, where all do, is slow and right.
-// Keys are (logit, index), so neither lists nor results depend on who comes first. Few rows are cut over the CTAs of a
-// cluster, whose leader joins them. What bounds it: the logits' bytes, and behind them the exponentials (one a logit,
-// sixteen a clock and SM: 0.7 of the memory's time for 16-bit logits); the rest is packed by twos.
+// when the maximum grows. A logit may be among the alternatives only if it reaches a bound that the k-th best cannot be below:
+// the least, over the CTA's W warps, of the ceil(k / W)-th greatest of the lanes' maxima so far, taken after the first
+// round and whenever the logits seen have doubled. What reaches it is put aside, some hundred pieces of a row,
+// and ranked at the end (2048 rows of 151936 with 20 alternatives: 108 us without, 156 with lists kept in order on the
+// way). A row where more do than there is room for (rising order) is read again with the
+// bound it ended with, into sorted lists. Keys are (logit, index), so results do not depend on who comes first. Few rows
+// are cut over the CTAs of a cluster, whose leader joins them. What bounds it: the logits' bytes, and behind them the
+// exponentials (one a logit, sixteen a clock and SM: 0.7 of the memory's time for 16-bit logits).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -56,13 +57,14 @@ struct Sums {
         s *= f;
         m = top;
     }
-    __device__ __forceinline__ void add(const Sums& o) {
-        Sums b = o;
-        const float top = fmaxf(m, b.m);
-        raise(top);
-        b.raise(top);
-        s += b.s;
-        e += b.e;
+    // Of the warp's lanes together, in every lane.
+    __device__ __forceinline__ void over_lanes() {
+        raise(logit_of(__reduce_max_sync(0xFFFFFFFFu, order_of(m))));
+#pragma unroll
+        for (uint32_t o = 16; o; o >>= 1) {
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            e += __shfl_xor_sync(0xFFFFFFFFu, e, o);
+        }
     }
     // One logit, not above the maximum. (x - m is exact near the maximum; products with log2 e are not)
     __device__ __forceinline__ void one(float x) {
@@ -126,6 +128,7 @@ __device__ __forceinline__ void insert(u64& list, u64 key, uint32_t lane) {
 // The j-th greatest (from 0) of the lanes' values.
 __device__ __forceinline__ uint32_t nth_greatest(uint32_t v, uint32_t j) {
     uint32_t top = 0;
+#pragma unroll 1
     for (uint32_t i = 0; i <= j; ++i) {
         top = __reduce_max_sync(0xFFFFFFFFu, v);
         const uint32_t who = __ffs(__ballot_sync(0xFFFFFFFFu, v == top)) - 1u;      // one of equal ones
@@ -134,17 +137,37 @@ __device__ __forceinline__ uint32_t nth_greatest(uint32_t v, uint32_t j) {
     return top;
 }
 
+constexpr uint32_t kAside = 640, kMostKeys = 16 * kMaxTop;
 template <uint32_t kWarps>
 struct Shared {
     Sums sums[kWarps];
     Sums joined;                 // of this CTA
     uint32_t bound[kWarps];      // each warp's: an order that so many of its logits reach
-    u64 keys[kWarps * kMaxTop];
+    uint4 piece[kAside];         // pieces with a logit that reached the bound, and which ones
+    uint32_t aside[kAside];
+    u64 keys[kMostKeys];         // logits that reach the last bound; in a second reading, the warps' lists
     u64 best[kMaxTop];           // of this CTA; the leader's: of the row
     Sums parts[8];               // the leader's: of every CTA of the cluster
     u64 offered[8 * kMaxTop];
-    uint32_t count;
+    uint32_t n_aside, n_keys;
 };
+
+// The best k of n keys in `from`, in order: a key's place is the number of greater ones (keys differ, but for zeros, which
+// stand for none). Not inlined: what runs once a row is mostly waiting for its own instructions.
+template <uint32_t kThreads>
+__device__ __noinline__ void best_of(const u64* from, uint32_t n, u64* to, uint32_t k) {
+    // four lanes a key; a warp's lanes stay together
+    for (uint32_t i0 = 0; i0 < n; i0 += kThreads / 4u) {
+        const uint32_t i = i0 + threadIdx.x / 4u;
+        const u64 key = i < n ? from[i] : 0u;
+        uint32_t at = 0;
+#pragma unroll 8
+        for (uint32_t j = threadIdx.x & 3u; j < n; j += 4u) at += from[j] > key;
+        at += __shfl_xor_sync(0xFFFFFFFFu, at, 1);
+        at += __shfl_xor_sync(0xFFFFFFFFu, at, 2);
+        if (!(threadIdx.x & 3u) && at < k && key) to[at] = key;
+    }
+}
 
 template <typename T, bool TOP, uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads, 768 / kThreads)
@@ -154,6 +177,8 @@ logprob_kernel(LogprobArgs a) {
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    if (threadIdx.x == 0) sh.n_aside = sh.n_keys = 0;
+    if (TOP && threadIdx.x < kMaxTop) sh.best[threadIdx.x] = 0;
     // what the others write into the leader's shared memory needs it to be there
     if (ranks > 1u) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     op_enter();
@@ -210,24 +235,44 @@ logprob_kernel(LogprobArgs a) {
         }
     };
     fetch(v0);
-    bool first = true;
+    bool first = true, fresh = true;
+    uint32_t round = 1;
+    float lane_top = -INFINITY;
+    // so many lanes of the warp have a logit of at least its bound
+    auto publish = [&]() {
+        const uint32_t b = nth_greatest(order_of(lane_top), share - 1u);
+        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(&sh.bound[warp]) = b;
+    };
+    auto put_aside = [&](const Vec<T>& v, uint32_t piece) {
+        const uint32_t at = atomicAdd(&sh.n_aside, 1u);
+        if (at < kAside) {
+            sh.aside[at] = piece;
+            sh.piece[at] = v.w;
+        }
+    };
     for (uint32_t base = v0; base < v1 || first; base += kThreads * kRound) {
-        float top[kRound], most = -FLT_MAX;
+        float top[kRound], most_there = -INFINITY;
 #pragma unroll
         for (uint32_t j = 0; j < kRound; ++j) {
             w[j] = ahead[j];
             top[j] = base + j * kThreads + tid < v1 ? w[j].top() : -INFINITY;
-            most = fmaxf(most, top[j]);
+            most_there = fmaxf(most_there, top[j]);
         }
+        const float most = fmaxf(most_there, -FLT_MAX);
         if (base + kThreads * kRound < v1) fetch(base + kThreads * kRound);
         if (TOP) {
+            lane_top = fmaxf(lane_top, most_there);
             if (first) {
-                // so many lanes have a logit of at least this
-                const uint32_t b = nth_greatest(order_of(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), share - 1u);
-                if (lane == 0) sh.bound[warp] = b;
+                publish();
                 __syncthreads();
             }
-            new_bound();
+            if (fresh) new_bound();
+            fresh = first;
+            if ((round & (round - 1u)) == 0u) {
+                if (!first) publish();
+                fresh = true;
+            }
+            ++round;
         }
         if (most > mine.m) mine.raise(most);
         const f32x2 less = pack2(-mine.m, -mine.m), log2e = pack2(kLog2e, kLog2e);
@@ -268,11 +313,8 @@ logprob_kernel(LogprobArgs a) {
 #pragma unroll
             for (uint32_t j = 0; j < kRound; ++j) {
                 const uint32_t i = base + j * kThreads + tid;
-                const uint32_t who = __ballot_sync(0xFFFFFFFFu, i < v1 && !(top[j] < reach));
-                if (who) consider_pieces(who, w[j], i);
+                if (i < v1 && !(top[j] < reach)) put_aside(w[j], i);
             }
-            const uint32_t b = static_cast<uint32_t>(__shfl_sync(0xFFFFFFFFu, list, share - 1u) >> 32);
-            if (lane == 0 && b > sh.bound[warp]) *reinterpret_cast<volatile uint32_t*>(&sh.bound[warp]) = b;
         }
         first = false;
     }
@@ -286,54 +328,63 @@ logprob_kernel(LogprobArgs a) {
             if (v > mine.m) mine.raise(v);
             mine.one(v);
         }
-        if (TOP) consider(v, i, there);
     }
+    if (TOP) publish();
     // ---- the CTA's sums and best ----
-#pragma unroll
-    for (uint32_t o = 16; o; o >>= 1) {
-        Sums b;
-        b.m = __shfl_xor_sync(0xFFFFFFFFu, mine.m, o);
-        b.s = __shfl_xor_sync(0xFFFFFFFFu, mine.s, o);
-        b.e = __shfl_xor_sync(0xFFFFFFFFu, mine.e, o);
-        mine.add(b);
-    }
+    mine.over_lanes();
     if (lane == 0) sh.sums[warp] = mine;
-    if (tid == 0) sh.count = 0;
     __syncthreads();
     if (warp == 0) {
-        Sums all = sh.sums[lane % kWarps];
-#pragma unroll
-        for (uint32_t o = kWarps / 2u; o; o >>= 1) {
-            Sums b;
-            b.m = __shfl_xor_sync(0xFFFFFFFFu, all.m, o);
-            b.s = __shfl_xor_sync(0xFFFFFFFFu, all.s, o);
-            b.e = __shfl_xor_sync(0xFFFFFFFFu, all.e, o);
-            all.add(b);
-        }
+        Sums all;
+        if (lane < kWarps) all = sh.sums[lane];
+        all.over_lanes();
         if (lane == 0) sh.joined = all;
     }
-    // The best of n keys in `from`, in order: a key's place is the number of greater ones (keys differ, but for zeros,
-    // which stand for none).
-    auto rank_keys = [&](const u64* from, uint32_t n, u64* to) {
-        for (uint32_t i = tid; i < n; i += kThreads) {
-            const u64 key = from[i];
-            uint32_t at = 0;
-#pragma unroll 8
-            for (uint32_t j = 0; j < n; ++j) at += from[j] > key;
-            if (at < k && key) to[at] = key;
-        }
-    };
+    auto rank_keys = [&](const u64* from, uint32_t n, u64* to) { best_of<kThreads>(from, n, to, k); };
     if (TOP) {
         new_bound();
-        const bool keep = lane < k && list != 0u && static_cast<uint32_t>(list >> 32) >= bound;
-        const uint32_t who = __ballot_sync(0xFFFFFFFFu, keep);
-        uint32_t at = 0;
-        if (lane == 0 && who) at = atomicAdd(&sh.count, __popc(who));
-        at = __shfl_sync(0xFFFFFFFFu, at, 0);
-        if (keep) sh.keys[at + __popc(who & ((1u << lane) - 1u))] = list;
-        if (tid < kMaxTop) sh.best[tid] = 0;
+        const uint32_t n = sh.n_aside;
+        auto offer = [&](float v, uint32_t i) {
+            if (v < reach) return;
+            const uint32_t at = atomicAdd(&sh.n_keys, 1u);
+            if (at < kMostKeys) sh.keys[at] = key_of(v, i);
+        };
+        const uint32_t loose = rank == ranks - 1u ? head + (a.vocab - tail) : 0u;
+        if (n <= kAside) {
+#pragma unroll 1
+            for (uint32_t e = tid; e < n * N; e += kThreads) {
+                offer(op_widen(reinterpret_cast<const T*>(sh.piece)[e]), head + sh.aside[e / N] * N + e % N);
+            }
+            if (tid < loose) {
+                const uint32_t i = tid < head ? tid : tail + tid - head;
+                offer(op_widen(x[i]), i);
+            }
+            __syncthreads();
+        }
+        if (n > kAside || sh.n_keys > kMostKeys) {      // again, each warp into a list
+            __syncthreads();
+            if (tid == 0) sh.n_keys = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (uint32_t base = v0; base < v1; base += kThreads) {
+                const uint32_t i = base + tid;
+                Vec<T> v;
+                v.w = make_uint4(0u, 0u, 0u, 0u);
+                if (i < v1) v.w = vec[i];
+                // a full list takes what is greater: an equal logit has the higher index
+                const u64 least = __shfl_sync(0xFFFFFFFFu, list, k - 1u);
+                const bool enters = least ? v.top() > logit_of(static_cast<uint32_t>(least >> 32)) : !(v.top() < reach);
+                const uint32_t who = __ballot_sync(0xFFFFFFFFu, i < v1 && enters);
+                if (who) consider_pieces(who, v, i);
+            }
+            if (warp == 0 && loose) {
+                const uint32_t i = lane < head ? lane : tail + lane - head;
+                consider(lane < loose ? op_widen(x[i]) : 0.0f, i, lane < loose);
+            }
+            if (lane < k && list != 0u) sh.keys[atomicAdd(&sh.n_keys, 1u)] = list;
+        }
         __syncthreads();
-        rank_keys(sh.keys, sh.count, sh.best);
+        rank_keys(sh.keys, sh.n_keys, sh.best);
     }
     if (ranks > 1u) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
@@ -347,14 +398,9 @@ logprob_kernel(LogprobArgs a) {
     if (rank == 0) {
         Sums all = sh.joined;
         if (ranks > 1u) {
-            all = sh.parts[lane % ranks];
-            for (uint32_t o = ranks / 2u; o; o >>= 1) {
-                Sums b;
-                b.m = __shfl_xor_sync(0xFFFFFFFFu, all.m, o);
-                b.s = __shfl_xor_sync(0xFFFFFFFFu, all.s, o);
-                b.e = __shfl_xor_sync(0xFFFFFFFFu, all.e, o);
-                all.add(b);
-            }
+            all = Sums{};
+            if (lane < ranks) all = sh.parts[lane];
+            all.over_lanes();
             if (TOP) {
                 rank_keys(sh.offered, ranks * k, sh.best);
                 __syncthreads();
