@@ -1,11 +1,17 @@
 // Paged key/value cache held in 4 bits: appending (with the rotary embedding on the way) and reading back.
 //
 // A key row is rotated as the decoder rotates it (adjacent pairs, angle = position * theta^(-i / head_dim);
-// apply_rope_inplace, api/cortex_sdk.cpp:1363-1423), angles and products in 64 bits: at position 10^5 an
-// fp32 angle is off by 4e-3. Then each group of 64 values x of a row becomes
+// apply_rope_inplace, api/cortex_sdk.cpp:1363-1423), angles in 64 bits: at position 10^5 an fp32 angle is off by
+// 4e-3. Then each group of 64 values x of a row becomes
 //   minimum = fp16(min x),  step = fp16((max x - min x) / 15),  code = clamp(rint((x - minimum) / step), 0, 15)
 // against the rounded minimum and step, so that their rounding does not add to the codes' error (half a
 // step). A group that holds a value that is not finite reads back as NaN; |x| past 65504 saturates.
+//
+// What is held is that of 64-bit arithmetic, value for value: a code that falls the other way is a whole step off. The
+// arithmetic is fp32 with a bound on its error; a group with a number that the bound leaves open - next to a border between
+// two codes, or where minimum or step round - is done again in 64 bits (one in fifty for keys, fewer for values).
+// Eight lanes have a group, eight neighbouring values each, so a warp moves 256 values at a time in 128-bit pieces. The bound
+// is the bytes of q, k and v.
 #include <algorithm>
 
 #include "codes4.cuh"
@@ -59,130 +65,240 @@ __device__ __forceinline__ uint32_t meta_offset(uint32_t tok, uint32_t d, uint32
     return 16u * HD + of_values * HD + ((d >> 6) * 16u + tok) * 4u;
 }
 
-template <int HD>
-__device__ __forceinline__ void quantise_row(const double (&x)[HD / 32], uint8_t* block, uint32_t tok, uint32_t of_values, uint32_t lane) {
-    constexpr uint32_t E = HD / 32, kLanes = 64 / E;
-    double lo = x[0], hi = x[0];
+// cos and sin of position * freq, to fp32's precision: the angle is reduced by multiples of pi / 2 in 64 bits (Cody
+// and Waite: pi / 2 as a 33-bit head, whose multiples are exact, and the rest), then Taylor series, 1e-9 at pi / 4.
+__device__ __forceinline__ float2 turn(int32_t pos, double freq) {
+    const double a = static_cast<double>(pos) * freq, k = rint(a * 0.63661977236758134);
+    const double x = fma(k, -6.077100506506192e-11, fma(k, -1.5707963267341256, a)), z = x * x;
+    const double s = x * fma(z, fma(z, fma(z, fma(z, 1.0 / 362880, -1.0 / 5040), 1.0 / 120), -1.0 / 6), 1.0);
+    const double c = fma(z, fma(z, fma(z, fma(z, fma(z, -1.0 / 3628800, 1.0 / 40320), -1.0 / 720), 1.0 / 24), -0.5), 1.0);
+    const int q = static_cast<int>(static_cast<long long>(k) & 3);
+    const double cc = q & 1 ? s : c, ss = q & 1 ? c : s;
+    return make_float2(static_cast<float>(q == 1 || q == 2 ? -cc : cc), static_cast<float>(q >= 2 ? -ss : ss));
+}
+
+// Eight neighbouring elements.
+template <typename T>
+__device__ __forceinline__ void load8(const T* from, bool vec, float (&x)[8]) {
+    if (vec) {
+        constexpr uint32_t N = 16u / sizeof(T);
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i += N) {
+            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from + i));
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) x[i + j] = op_widen(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) x[i] = op_widen(from[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* to, bool vec, const float (&x)[8]) {
+    T r[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) r[i] = op_narrow<T>(x[i]);
+    if (vec) {
+        const uint4* from = reinterpret_cast<const uint4*>(r);
+        reinterpret_cast<uint4*>(to)[0] = from[0];
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(to)[1] = from[1];
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) to[i] = r[i];
+    }
+}
+
+template <typename F>
+__device__ __forceinline__ F over_group(F v, F (*op)(F, F)) {
+#pragma unroll
+    for (uint32_t o = 4; o; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+__device__ __forceinline__ float least(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double least(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
+
+// A group in 64 bits. All lanes of the warp come along.
+__device__ __noinline__ void quantise_slowly(const float (&v)[8], bool rotate, int32_t pos, const double* freq, uint32_t (&c)[8], __half& mn, __half& st) {
+    double x[8], lo, hi;
     bool fine = true;
 #pragma unroll
-    for (uint32_t i = 0; i < E; ++i) {
+    for (uint32_t i = 0; i < 8u; i += 2u) {
+        double co = 1.0, si = 0.0;
+        if (rotate) sincos(static_cast<double>(pos) * freq[i / 2u], &si, &co);
+        x[i] = v[i] * co - v[i + 1] * si;
+        x[i + 1] = v[i] * si + v[i + 1] * co;
+    }
+    lo = hi = x[0];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) {
         lo = fmin(lo, x[i]);
         hi = fmax(hi, x[i]);
         fine = fine && isfinite(x[i]);
     }
-#pragma unroll
-    for (uint32_t o = kLanes / 2; o; o >>= 1) {
-        lo = fmin(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
-        hi = fmax(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
-        fine = __shfl_xor_sync(0xFFFFFFFFu, static_cast<int>(fine), o) && fine;
-    }
+    lo = over_group<double>(lo, least);
+    hi = over_group<double>(hi, most);
+    fine = (__ballot_sync(0xFFFFFFFFu, fine) >> (threadIdx.x & 24u) & 0xFFu) == 0xFFu;
     lo = fmin(fmax(lo, -65504.0), 65504.0);
     hi = fmin(fmax(hi, -65504.0), 65504.0);
-    const __half mn = fine ? __float2half_rn(static_cast<float>(lo)) : __ushort_as_half(0x7FFF);
-    const __half st = fine ? __float2half_rn(static_cast<float>((hi - lo) / 15.0)) : __ushort_as_half(0);
+    mn = fine ? __float2half_rn(static_cast<float>(lo)) : __ushort_as_half(0x7FFF);
+    st = fine ? __float2half_rn(static_cast<float>((hi - lo) / 15.0)) : __ushort_as_half(0);
     const double m = __half2float(mn), s = __half2float(st);
-    uint32_t c[E];
 #pragma unroll
-    for (uint32_t i = 0; i < E; ++i) c[i] = s > 0.0 ? static_cast<uint32_t>(fmin(fmax(rint((x[i] - m) / s), 0.0), 15.0)) : 0u;
-    const uint32_t d = E * lane;
-    uint8_t* to = block + (of_values ? value_offset<HD>(tok, d) : key_offset<HD>(tok, d));
-    if constexpr (E == 2) {       // two lanes share a half word
-        const uint32_t c2 = __shfl_down_sync(0xFFFFFFFFu, c[0], 1), c3 = __shfl_down_sync(0xFFFFFFFFu, c[1], 1);
-        if (!(lane & 1u)) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(pack_codes(c[0], c[1], c2, c3));
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < E; i += 4u)
-            *reinterpret_cast<uint16_t*>(to + (of_values ? i : i / 2u)) = static_cast<uint16_t>(pack_codes(c[i], c[i + 1], c[i + 2], c[i + 3]));
-    }
-    if (lane % kLanes == 0) {
-        const __half2 both = __halves2half2(mn, st);
-        *reinterpret_cast<__half2*>(block + meta_offset<HD>(tok, d, of_values)) = both;
-    }
+    for (uint32_t i = 0; i < 8u; ++i) c[i] = s > 0.0 ? static_cast<uint32_t>(fmin(fmax(rint((x[i] - m) / s), 0.0), 15.0)) : 0u;
 }
 
-// grid (token, slice of the heads); a warp takes a head at a time, a lane HD / 32 neighbouring values.
+// fp16 of every number between a and b is one and the same.
+__device__ __forceinline__ bool settled(float a, float b, __half& h) {
+    h = __float2half_rn(a);
+    return __half_as_ushort(h) == __half_as_ushort(__float2half_rn(b));
+}
+
+// grid (token, slice of the heads). A warp takes four groups at a time: of q (rotated only), then k, then v.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWarps * 32)
 kv_append_kernel(KvView kv, KvBatchView b, KvAppend a) {
     op_enter();
-    constexpr uint32_t E = HD / 32;
-    const uint32_t t = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    constexpr uint32_t G = HD / 64;
+    __shared__ float2 turns[HD / 2];
+    const uint32_t t = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, l = lane & 7u;
     int32_t pos, page;
     if (!locate(kv, b, t, pos, page)) return;
-    double c[E / 2], s[E / 2];
-#pragma unroll
-    for (uint32_t i = 0; i < E / 2; ++i) {
-        c[i] = 1.0;
-        s[i] = 0.0;
-        if (a.freq) sincos(static_cast<double>(pos) * a.freq[E / 2 * lane + i], &s[i], &c[i]);
+    if (a.freq) {
+        for (uint32_t i = threadIdx.x; i < HD / 2; i += kWarps * 32) turns[i] = turn(pos, a.freq[i]);
+        __syncthreads();
     }
-    const uint32_t qh = a.q ? a.q_heads : 0u, units = qh + 2u * kv.kv_heads;
-    for (uint32_t u = blockIdx.y * kWarps + warp; u < units; u += gridDim.y * kWarps) {
-        const bool is_q = u < qh, is_v = u >= qh + kv.kv_heads;
-        const uint32_t head = is_q ? u : is_v ? u - qh - kv.kv_heads : u - qh;
-        const T* src = static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + t * (is_q ? a.q_stride : a.kv_stride) + head * HD + E * lane;
-        if (!is_q && page < 0) continue;
-        double x[E];
+    const uint32_t nq = (a.q ? a.q_heads : 0u) * G, nk = kv.kv_heads * G, units = nq + 2u * nk;
+    const uint32_t at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
+    for (uint32_t u0 = (blockIdx.y * kWarps + warp) * 4u; u0 < units; u0 += gridDim.y * kWarps * 4u) {
+        const uint32_t u = u0 + (lane >> 3);
+        const bool there = u < units, is_q = u < nq, is_v = there && u >= nq + nk;
+        const uint32_t gr = is_q ? u : is_v ? u - nq - nk : u - nq, d = gr % G * 64u + 8u * l;
+        float x[8], raw[8];
 #pragma unroll
-        for (uint32_t i = 0; i < E; ++i) x[i] = op_widen(src[i]);
-        if (!is_v) {
+        for (uint32_t i = 0; i < 8u; ++i) x[i] = 0.0f;
+        if (there) {
+            const T* src = static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + t * (is_q ? a.q_stride : a.kv_stride) + gr * 64u + 8u * l;
+            load8(src, is_q ? a.q_vec : a.kv_vec, x);
+        }
+        const bool rotate = a.freq && !is_v;
+        float wide = 0.0f;      // of the sums that a rotated value is at most
 #pragma unroll
-            for (uint32_t i = 0; i < E / 2; ++i) {
-                const double y0 = x[2 * i] * c[i] - x[2 * i + 1] * s[i], y1 = x[2 * i] * s[i] + x[2 * i + 1] * c[i];
-                x[2 * i] = y0;
-                x[2 * i + 1] = y1;
+        for (uint32_t i = 0; i < 8u; i += 2u) {
+            raw[i] = x[i];
+            raw[i + 1] = x[i + 1];
+            if (rotate) {
+                const float2 r = turns[d / 2u + i / 2u];
+                const float y0 = fmaf(x[i], r.x, -x[i + 1] * r.y), y1 = fmaf(x[i], r.y, x[i + 1] * r.x);
+                wide = fmaxf(wide, fabsf(x[i]) + fabsf(x[i + 1]));
+                x[i] = y0;
+                x[i + 1] = y1;
             }
         }
-        if (is_q) {
-            T* dst = static_cast<T*>(a.q_out) + t * a.q_out_stride + head * HD + E * lane;
+        if (there && is_q) store8(static_cast<T*>(a.q_out) + t * a.q_out_stride + gr * 64u + 8u * l, a.q_out_vec, x);
+        if (u0 + 4u <= nq || page < 0) continue;       // for the whole warp
+        // ---- the group: fp32, and what its error leaves open ----
+        float lo = x[0], hi = x[0];
+        bool fine = true;
 #pragma unroll
-            for (uint32_t i = 0; i < E; ++i) dst[i] = op_narrow<T>(static_cast<float>(x[i]));
+        for (uint32_t i = 0; i < 8u; ++i) {
+            lo = fminf(lo, x[i]);
+            hi = fmaxf(hi, x[i]);
+            fine = fine && fabsf(x[i]) <= 65504.0f;      // what saturates or is not finite: slowly
+        }
+        lo = over_group<float>(lo, least);
+        hi = over_group<float>(hi, most);
+        wide = over_group<float>(wide, most);
+        // rotation: cos and sin 2^-24, three roundings of 2^-24; 2^-21 of |x0| + |x1| has room
+        const float err = wide * 0x1p-21f;
+        const float width = hi - lo, step = width * (1.0f / 15.0f), step_err = fmaf(step, 0x1p-21f, err * 0.2f);
+        __half mn, st;
+        fine = fine && settled(lo - err, lo + err, mn);
+        fine = fine && settled(step - step_err, step + step_err, st);
+        const float m = __half2float(mn), s = __half2float(st);
+        uint32_t c[8];
+        if (s > 0.0f) {
+            // (x - m) / s: two roundings, 1 / s another; at most 17 where it matters
+            const float by = 1.0f / s, open = 0.5f - fmaf(err, by, 17.0f * 0x1p-21f);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) {
+                const float q = (x[i] - m) * by, r = rintf(q);
+                fine = fine && fabsf(q - r) < open;
+                c[i] = static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f));
+            }
         } else {
-            const uint32_t at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u);
-            quantise_row<HD>(x, kv.base + kv.block_at(page, head, at), at & 15u, is_v, lane);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) c[i] = 0u;
+        }
+        if (!__all_sync(0xFFFFFFFFu, fine)) quantise_slowly(raw, rotate, pos, a.freq ? a.freq + d / 2u : nullptr, c, mn, st);
+        if (there && !is_q) {
+            uint8_t* block = kv.base + kv.block_at(page, gr / G, at);
+            const uint32_t h0 = pack_codes(c[0], c[1], c[2], c[3]), h1 = pack_codes(c[4], c[5], c[6], c[7]);
+            if (is_v) {
+                uint16_t* to = reinterpret_cast<uint16_t*>(block + value_offset<HD>(tok, d));
+                to[0] = static_cast<uint16_t>(h0);
+                to[2] = static_cast<uint16_t>(h1);
+            } else {
+                *reinterpret_cast<uint32_t*>(block + key_offset<HD>(tok, d)) = h0 | h1 << 16;
+            }
+            if (l == 0u) *reinterpret_cast<__half2*>(block + meta_offset<HD>(tok, d, is_v)) = __halves2half2(mn, st);
         }
     }
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kWarps * 32)
-kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restrict__ v) {
+kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restrict__ v, bool vec) {
     op_enter();
-    constexpr uint32_t E = HD / 32;
-    const uint32_t t = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, d = E * lane;
+    constexpr uint32_t G = HD / 64;
+    const uint32_t t = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, l = lane & 7u;
     int32_t pos, page;
     if (!locate(kv, b, t, pos, page)) return;
-    for (uint32_t u = blockIdx.y * kWarps + warp; u < 2u * kv.kv_heads; u += gridDim.y * kWarps) {
-        const uint32_t is_v = u >= kv.kv_heads, head = is_v ? u - kv.kv_heads : u;
-        float* dst = (is_v ? v : k) + (static_cast<size_t>(t) * kv.kv_heads + head) * HD + d;
-        uint32_t codes[E] = {};
-        float st = 0.0f, mn = 0.0f;
+    const uint32_t nk = kv.kv_heads * G, at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
+    for (uint32_t u = (blockIdx.y * kWarps + warp) * 4u + (lane >> 3); u < 2u * nk; u += gridDim.y * kWarps * 4u) {
+        const bool is_v = u >= nk;
+        const uint32_t gr = is_v ? u - nk : u, d = gr % G * 64u + 8u * l;
+        float x[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) x[i] = 0.0f;
         if (page >= 0) {
-            const uint32_t at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
-            const uint8_t* block = kv.base + kv.block_at(page, head, at);
-            const uint8_t* from = block + (is_v ? value_offset<HD>(tok, d) : key_offset<HD>(tok, d));
+            const uint8_t* block = kv.base + kv.block_at(page, gr / G, at);
+            uint32_t h[2];
+            if (is_v) {
+                const uint16_t* from = reinterpret_cast<const uint16_t*>(block + value_offset<HD>(tok, d));
+                h[0] = from[0];
+                h[1] = from[2];
+            } else {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(block + key_offset<HD>(tok, d));
+                h[0] = w & 0xFFFFu;
+                h[1] = w >> 16;
+            }
+            const float2 both = __half22float2(*reinterpret_cast<const __half2*>(block + meta_offset<HD>(tok, d, is_v)));
 #pragma unroll
-            for (uint32_t i = 0; i < E; ++i)
-                codes[i] = unpack_code(*reinterpret_cast<const uint16_t*>(from + (is_v ? i / 4u * 4u : i / 4u * 2u)), (d + i) & 3u);
-            const __half2 both = *reinterpret_cast<const __half2*>(block + meta_offset<HD>(tok, d, is_v));
-            mn = __low2float(both);
-            st = __high2float(both);
+            for (uint32_t i = 0; i < 8u; ++i) x[i] = fmaf(static_cast<float>(unpack_code(h[i / 4u], i & 3u)), both.y, both.x);
         }
-#pragma unroll
-        for (uint32_t i = 0; i < E; ++i) dst[i] = fmaf(static_cast<float>(codes[i]), st, mn);
+        store8((is_v ? v : k) + (static_cast<size_t>(t) * nk + gr) * 64u + 8u * l, vec, x);
     }
 }
 
-// Slices of a token's heads: few tokens still fill the GPU, many take whole tokens.
+// Slices of a token's groups: few tokens still fill the GPU, many take whole tokens.
 uint32_t slices(const csdr_context* ctx, uint32_t tokens, uint32_t units) {
-    const uint32_t most = (units + kWarps - 1) / kWarps;
+    const uint32_t most = (units + kWarps * 4u - 1u) / (kWarps * 4u);
     return std::max(1u, std::min(most, static_cast<uint32_t>(ctx->sm_count) * 8u / std::max(1u, tokens)));
 }
 
 }  // namespace
 
-void launch_kv_append(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAppend& a) {
-    const uint32_t units = (a.q ? a.q_heads : 0u) + 2u * kv.kv_heads;
+void launch_kv_append(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAppend& given) {
+    const uint32_t units = ((given.q ? given.q_heads : 0u) + 2u * kv.kv_heads) * (head_dim / kKvGroup);
+    const size_t es = dtype == CSDR_DTYPE_F32 ? 4u : 2u;
+    auto vec = [&](const void* p, size_t stride) { return (reinterpret_cast<uintptr_t>(p) | stride * es) % 16u == 0; };
+    KvAppend a = given;
+    a.q_vec = vec(a.q, a.q_stride);
+    a.q_out_vec = vec(a.q_out, a.q_out_stride);
+    a.kv_vec = vec(a.k, a.kv_stride) && vec(a.v, 0);
     const dim3 grid(b.n_tokens, slices(ctx, b.n_tokens, units));
     LaunchScope ls(ctx, KC_KV_CACHE);
     with_dtype(dtype, [&](auto* t) {
@@ -195,11 +311,12 @@ void launch_kv_append(csdr_context* ctx, const KvView& kv, uint32_t head_dim, co
 }
 
 void launch_kv_read(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, float* k, float* v) {
-    const dim3 grid(b.n_tokens, slices(ctx, b.n_tokens, 2u * kv.kv_heads));
+    const dim3 grid(b.n_tokens, slices(ctx, b.n_tokens, 2u * kv.kv_heads * (head_dim / kKvGroup)));
+    const bool vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16u == 0;
     LaunchScope ls(ctx, KC_KV_CACHE);
-    if (head_dim == 64) launch_op(ctx, kv_read_kernel<64>, grid, kWarps * 32, 0, 1, kv, b, k, v);
-    else if (head_dim == 128) launch_op(ctx, kv_read_kernel<128>, grid, kWarps * 32, 0, 1, kv, b, k, v);
-    else launch_op(ctx, kv_read_kernel<256>, grid, kWarps * 32, 0, 1, kv, b, k, v);
+    if (head_dim == 64) launch_op(ctx, kv_read_kernel<64>, grid, kWarps * 32, 0, 1, kv, b, k, v, vec);
+    else if (head_dim == 128) launch_op(ctx, kv_read_kernel<128>, grid, kWarps * 32, 0, 1, kv, b, k, v, vec);
+    else launch_op(ctx, kv_read_kernel<256>, grid, kWarps * 32, 0, 1, kv, b, k, v, vec);
     ls.done("kv_read_kernel");
 }
 

@@ -45,6 +45,7 @@ struct KvAppend {
     size_t kv_stride, q_stride, q_out_stride;   // elements between tokens
     uint32_t q_heads;
     const double* freq;      // rotation per position of each pair; null: stored as they come
+    bool q_vec, q_out_vec, kv_vec;      // rows start on 16 bytes (set by the launcher)
 };
 void launch_kv_append(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAppend& a);
 // The values the batch's new tokens are held as, fp32 (token, kv head, head_dim); zeros where a token has no place.
