@@ -22,31 +22,40 @@ namespace csdr {
 
 namespace {
 
-constexpr uint32_t kWarps = 8;
+constexpr uint32_t kWarps = 8, kTokens = 4;      // of a CTA, the most
 
-// The sequence that row t belongs to: how many of first[1 ..] are at most t. All threads of the CTA.
-__device__ __forceinline__ uint32_t sequence_of(const KvBatchView& b, int32_t t) {
-    uint32_t below = 0;
+// Where a CTA's rows' tokens lie: rows t0 to t0 + n - 1 (n at most kTokens), by all threads. own: the row belongs to a sequence.
+struct Places {
+    int32_t pos[kTokens], page[kTokens];      // page: -1 for a token that has no place
+    uint32_t own[kTokens];
+};
+__device__ __forceinline__ void locate(const KvView& kv, const KvBatchView& b, uint32_t t0, uint32_t n, Places& at) {
+    // the first row's sequence: how many of first[1 ..] are at most that row
+    uint32_t s = 0;
     for (uint32_t i = 0; i < b.n_seqs; i += blockDim.x) {
-        const uint32_t s = i + threadIdx.x;
-        below += __syncthreads_count(s < b.n_seqs && b.first[s + 1] <= t);
+        const uint32_t q = i + threadIdx.x;
+        s += __syncthreads_count(q < b.n_seqs && b.first[q + 1] <= static_cast<int32_t>(t0));
     }
-    return below;
-}
-
-// Where row t's token lies: its position, and its page or -1 where it has no place.
-__device__ __forceinline__ bool locate(const KvView& kv, const KvBatchView& b, uint32_t t, int32_t& pos, int32_t& page) {
-    const uint32_t s = sequence_of(b, static_cast<int32_t>(t));
-    pos = page = -1;
-    if (s >= b.n_seqs) return false;
-    const int32_t first = b.first[s];
-    if (static_cast<int32_t>(t) < first) return false;
-    const int64_t p = static_cast<int64_t>(b.length[s]) - b.first[s + 1] + static_cast<int32_t>(t);
-    if (p < 0 || (p >> kv.page_shift) >= b.pages_per_seq) return true;
-    pos = static_cast<int32_t>(p);
-    page = b.pages[static_cast<size_t>(s) * b.pages_per_seq + (p >> kv.page_shift)];
-    if (page < 0 || static_cast<uint32_t>(page) >= kv.n_pages) page = -1;
-    return true;
+    if (threadIdx.x < n) {
+        const int32_t t = static_cast<int32_t>(t0 + threadIdx.x);
+        while (s < b.n_seqs && b.first[s + 1] <= t) ++s;
+        int32_t pos = -1, page = -1;
+        const bool own = s < b.n_seqs && t >= b.first[s];
+        if (own) {
+            const int64_t p = static_cast<int64_t>(b.length[s]) - b.first[s + 1] + t;
+            if (p >= 0 && (p >> kv.page_shift) < b.pages_per_seq) {
+                pos = static_cast<int32_t>(p);
+                page = b.pages[static_cast<size_t>(s) * b.pages_per_seq + (p >> kv.page_shift)];
+                if (page < 0 || static_cast<uint32_t>(page) >= kv.n_pages) page = -1;
+            } else if (p >= 0) {
+                pos = static_cast<int32_t>(min(p, static_cast<int64_t>(0x7FFFFFFF)));
+            }
+        }
+        at.pos[threadIdx.x] = pos;
+        at.page[threadIdx.x] = page;
+        at.own[threadIdx.x] = own;
+    }
+    __syncthreads();
 }
 
 // Where the half word with values d & ~3 .. + 3 of a token lies.
@@ -77,23 +86,22 @@ __device__ __forceinline__ float2 turn(int32_t pos, double freq) {
     return make_float2(static_cast<float>(q == 1 || q == 2 ? -cc : cc), static_cast<float>(q >= 2 ? -ss : ss));
 }
 
-// Eight neighbouring elements.
+// Eight neighbouring elements, as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* from, bool vec, float (&x)[8]) {
-    if (vec) {
-        constexpr uint32_t N = 16u / sizeof(T);
+struct Eight {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* from, bool vec) {
+        if (vec) {
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i += N) {
-            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from + i));
-            const T* e = reinterpret_cast<const T*>(&v);
+            for (uint32_t i = 0; i < sizeof(T) / 2; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(from) + i);
+        } else {
+            T* e = reinterpret_cast<T*>(w);
 #pragma unroll
-            for (uint32_t j = 0; j < N; ++j) x[i + j] = op_widen(e[j]);
+            for (uint32_t i = 0; i < 8u; ++i) e[i] = from[i];
         }
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) x[i] = op_widen(from[i]);
     }
-}
+    __device__ __forceinline__ float operator[](uint32_t i) const { return op_widen(reinterpret_cast<const T*>(w)[i]); }
+};
 template <typename T>
 __device__ __forceinline__ void store8(T* to, bool vec, const float (&x)[8]) {
     T r[8];
@@ -156,45 +164,57 @@ __device__ __forceinline__ bool settled(float a, float b, __half& h) {
     return __half_as_ushort(h) == __half_as_ushort(__float2half_rn(b));
 }
 
-// grid (token, slice of the heads). A warp takes four groups at a time: of q (rotated only), then k, then v.
+// grid (tokens, slice of their groups). A warp takes four groups of a token at a time: of q (rotated only), then k, then v; the
+// next four are on their way meanwhile.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWarps * 32)
-kv_append_kernel(KvView kv, KvBatchView b, KvAppend a) {
+kv_append_kernel(KvView kv, KvBatchView b, KvAppend a, uint32_t tokens) {
     op_enter();
     constexpr uint32_t G = HD / 64;
-    __shared__ float2 turns[HD / 2];
-    const uint32_t t = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, l = lane & 7u;
-    int32_t pos, page;
-    if (!locate(kv, b, t, pos, page)) return;
+    __shared__ float2 turns[kTokens][HD / 2];
+    __shared__ Places places;
+    const uint32_t t0 = blockIdx.x * tokens, n_tok = min(tokens, b.n_tokens - t0);
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, l = lane & 7u;
+    locate(kv, b, t0, n_tok, places);
     if (a.freq) {
-        for (uint32_t i = threadIdx.x; i < HD / 2; i += kWarps * 32) turns[i] = turn(pos, a.freq[i]);
+        for (uint32_t i = threadIdx.x; i < n_tok * (HD / 2); i += kWarps * 32) turns[i / (HD / 2)][i % (HD / 2)] = turn(places.pos[i / (HD / 2)], a.freq[i % (HD / 2)]);
         __syncthreads();
     }
-    const uint32_t nq = (a.q ? a.q_heads : 0u) * G, nk = kv.kv_heads * G, units = nq + 2u * nk;
-    const uint32_t at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
-    for (uint32_t u0 = (blockIdx.y * kWarps + warp) * 4u; u0 < units; u0 += gridDim.y * kWarps * 4u) {
-        const uint32_t u = u0 + (lane >> 3);
-        const bool there = u < units, is_q = u < nq, is_v = there && u >= nq + nk;
+    const uint32_t nq = (a.q ? a.q_heads : 0u) * G, nk = kv.kv_heads * G, units = nq + 2u * nk, fours = (units + 3u) / 4u;
+    Eight<T> ahead;
+    // a warp's i-th four: token and group of this lane
+    auto fetch = [&](uint32_t i) {
+        const uint32_t j = i / fours, u = i % fours * 4u + (lane >> 3), t = t0 + j;
+        if (u >= units || !places.own[j]) return;
+        if (u < nq) ahead.load(static_cast<const T*>(a.q) + t * a.q_stride + u * 64u + 8u * l, a.q_vec);
+        else if (places.page[j] < 0) return;
+        else if (u < nq + nk) ahead.load(static_cast<const T*>(a.k) + t * a.kv_stride + (u - nq) * 64u + 8u * l, a.kv_vec);
+        else ahead.load(static_cast<const T*>(a.v) + t * a.kv_stride + (u - nq - nk) * 64u + 8u * l, a.kv_vec);
+    };
+    const uint32_t step = gridDim.y * kWarps, n_fours = n_tok * fours;
+    uint32_t i = blockIdx.y * kWarps + warp;
+    if (i < n_fours) fetch(i);
+    for (; i < n_fours; i += step) {
+        const uint32_t j = i / fours, u0 = i % fours * 4u, u = u0 + (lane >> 3), t = t0 + j;
+        const int32_t pos = places.pos[j], page = places.page[j];
+        const uint32_t at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
+        const Eight<T> raw = ahead;
+        if (i + step < n_fours) fetch(i + step);
+        if (!places.own[j]) continue;
+        const bool is_q = u < nq, is_v = u >= nq + nk, there = u < units && (is_q || page >= 0);
         const uint32_t gr = is_q ? u : is_v ? u - nq - nk : u - nq, d = gr % G * 64u + 8u * l;
-        float x[8], raw[8];
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) x[i] = 0.0f;
-        if (there) {
-            const T* src = static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) + t * (is_q ? a.q_stride : a.kv_stride) + gr * 64u + 8u * l;
-            load8(src, is_q ? a.q_vec : a.kv_vec, x);
-        }
         const bool rotate = a.freq && !is_v;
-        float wide = 0.0f;      // of the sums that a rotated value is at most
+        float x[8], wide = 0.0f;      // wide: the most that a rotated value can be
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i += 2u) {
-            raw[i] = x[i];
-            raw[i + 1] = x[i + 1];
-            if (rotate) {
-                const float2 r = turns[d / 2u + i / 2u];
-                const float y0 = fmaf(x[i], r.x, -x[i + 1] * r.y), y1 = fmaf(x[i], r.y, x[i + 1] * r.x);
-                wide = fmaxf(wide, fabsf(x[i]) + fabsf(x[i + 1]));
-                x[i] = y0;
-                x[i + 1] = y1;
+        for (uint32_t e = 0; e < 8u; ++e) x[e] = there ? raw[e] : 0.0f;
+        if (rotate) {
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; e += 2u) {
+                const float2 r = turns[j][d / 2u + e / 2u];
+                const float y0 = fmaf(x[e], r.x, -x[e + 1] * r.y), y1 = fmaf(x[e], r.y, x[e + 1] * r.x);
+                wide = fmaxf(wide, fabsf(x[e]) + fabsf(x[e + 1]));
+                x[e] = y0;
+                x[e + 1] = y1;
             }
         }
         if (there && is_q) store8(static_cast<T*>(a.q_out) + t * a.q_out_stride + gr * 64u + 8u * l, a.q_out_vec, x);
@@ -211,28 +231,32 @@ kv_append_kernel(KvView kv, KvBatchView b, KvAppend a) {
         lo = over_group<float>(lo, least);
         hi = over_group<float>(hi, most);
         wide = over_group<float>(wide, most);
-        // rotation: cos and sin 2^-24, three roundings of 2^-24; 2^-21 of |x0| + |x1| has room
-        const float err = wide * 0x1p-21f;
-        const float width = hi - lo, step = width * (1.0f / 15.0f), step_err = fmaf(step, 0x1p-21f, err * 0.2f);
+        // rotation: cos and sin are 2^-24.9 off, a product and the sum round: 2.6 2^-24 (|x0| + |x1|)
+        const float err = wide * 0x1p-22f;
+        const float width = hi - lo, step15 = width * (1.0f / 15.0f), step_err = fmaf(step15, 0x1p-22f, err * 0.134f);
         __half mn, st;
         fine = fine && settled(lo - err, lo + err, mn);
-        fine = fine && settled(step - step_err, step + step_err, st);
+        fine = fine && settled(step15 - step_err, step15 + step_err, st);
         const float m = __half2float(mn), s = __half2float(st);
         uint32_t c[8];
-        if (s > 0.0f) {
-            // (x - m) / s: two roundings, 1 / s another; at most 17 where it matters
-            const float by = 1.0f / s, open = 0.5f - fmaf(err, by, 17.0f * 0x1p-21f);
+        {
+            // (x - m) / s: three roundings of 2^-24 on at most 16. What lies outside 0 .. 15 by less than half a code falls to
+            // the same side whatever its error
+            const float by = s > 0.0f ? 1.0f / s : 0.0f, open = 0.5f - fmaf(err, by, 17.0f * 0x1p-22f);
+            constexpr float kWhole = 12582912.0f;      // 1.5 2^23: adding it rounds to a whole number, which its low bits are
 #pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) {
-                const float q = (x[i] - m) * by, r = rintf(q);
-                fine = fine && fabsf(q - r) < open;
-                c[i] = static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f));
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const float q = fminf(fmaxf((x[e] - m) * by, 0.0f), 15.0f), r = q + kWhole;
+                fine = fine && fabsf(q - (r - kWhole)) < open;
+                c[e] = __float_as_uint(r) & 15u;
             }
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) c[i] = 0u;
         }
-        if (!__all_sync(0xFFFFFFFFu, fine)) quantise_slowly(raw, rotate, pos, a.freq ? a.freq + d / 2u : nullptr, c, mn, st);
+        if (!__all_sync(0xFFFFFFFFu, fine)) {
+            float v[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e) v[e] = there ? raw[e] : 0.0f;
+            quantise_slowly(v, rotate, pos, a.freq ? a.freq + d / 2u : nullptr, c, mn, st);
+        }
         if (there && !is_q) {
             uint8_t* block = kv.base + kv.block_at(page, gr / G, at);
             const uint32_t h0 = pack_codes(c[0], c[1], c[2], c[3]), h1 = pack_codes(c[4], c[5], c[6], c[7]);
@@ -250,14 +274,20 @@ kv_append_kernel(KvView kv, KvBatchView b, KvAppend a) {
 
 template <int HD>
 __global__ void __launch_bounds__(kWarps * 32)
-kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restrict__ v, bool vec) {
+kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restrict__ v, bool vec, uint32_t tokens) {
     op_enter();
     constexpr uint32_t G = HD / 64;
-    const uint32_t t = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, l = lane & 7u;
-    int32_t pos, page;
-    if (!locate(kv, b, t, pos, page)) return;
-    const uint32_t nk = kv.kv_heads * G, at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
-    for (uint32_t u = (blockIdx.y * kWarps + warp) * 4u + (lane >> 3); u < 2u * nk; u += gridDim.y * kWarps * 4u) {
+    __shared__ Places places;
+    const uint32_t t0 = blockIdx.x * tokens, n_tok = min(tokens, b.n_tokens - t0);
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, l = lane & 7u;
+    locate(kv, b, t0, n_tok, places);
+    const uint32_t nk = kv.kv_heads * G, units = 2u * nk, fours = (units + 3u) / 4u;
+#pragma unroll 2
+    for (uint32_t f = blockIdx.y * kWarps + warp; f < n_tok * fours; f += gridDim.y * kWarps) {
+        const uint32_t j = f / fours, u = f % fours * 4u + (lane >> 3), t = t0 + j;
+        if (u >= units || !places.own[j]) continue;
+        const int32_t page = places.page[j];
+        const uint32_t at = static_cast<uint32_t>(places.pos[j]) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
         const bool is_v = u >= nk;
         const uint32_t gr = is_v ? u - nk : u, d = gr % G * 64u + 8u * l;
         float x[8];
@@ -283,40 +313,42 @@ kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restric
     }
 }
 
-// Slices of a token's groups: few tokens still fill the GPU, many take whole tokens.
-uint32_t slices(const csdr_context* ctx, uint32_t tokens, uint32_t units) {
-    const uint32_t most = (units + kWarps * 4u - 1u) / (kWarps * 4u);
-    return std::max(1u, std::min(most, static_cast<uint32_t>(ctx->sm_count) * 8u / std::max(1u, tokens)));
+// Few tokens: a CTA has one, or a slice of its groups, so that they fill the GPU. Many: four a CTA, whose prologue is shared.
+struct Shape {
+    dim3 grid;
+    uint32_t tokens;
+};
+Shape shape_of(const csdr_context* ctx, uint32_t n_tokens, uint32_t groups) {
+    const uint32_t room = static_cast<uint32_t>(ctx->sm_count) * 4u, tokens = n_tokens >= room * kTokens ? kTokens : 1u;
+    const uint32_t most = (groups + kWarps * 4u - 1u) / (kWarps * 4u);
+    return {dim3((n_tokens + tokens - 1u) / tokens, std::max(1u, std::min(most, room * 2u / std::max(1u, n_tokens)))), tokens};
 }
 
 }  // namespace
 
 void launch_kv_append(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAppend& given) {
-    const uint32_t units = ((given.q ? given.q_heads : 0u) + 2u * kv.kv_heads) * (head_dim / kKvGroup);
     const size_t es = dtype == CSDR_DTYPE_F32 ? 4u : 2u;
     auto vec = [&](const void* p, size_t stride) { return (reinterpret_cast<uintptr_t>(p) | stride * es) % 16u == 0; };
     KvAppend a = given;
     a.q_vec = vec(a.q, a.q_stride);
     a.q_out_vec = vec(a.q_out, a.q_out_stride);
     a.kv_vec = vec(a.k, a.kv_stride) && vec(a.v, 0);
-    const dim3 grid(b.n_tokens, slices(ctx, b.n_tokens, units));
+    const Shape s = shape_of(ctx, b.n_tokens, ((a.q ? a.q_heads : 0u) + 2u * kv.kv_heads) * (head_dim / kKvGroup));
     LaunchScope ls(ctx, KC_KV_CACHE);
     with_dtype(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (head_dim == 64) launch_op(ctx, kv_append_kernel<T, 64>, grid, kWarps * 32, 0, 1, kv, b, a);
-        else if (head_dim == 128) launch_op(ctx, kv_append_kernel<T, 128>, grid, kWarps * 32, 0, 1, kv, b, a);
-        else launch_op(ctx, kv_append_kernel<T, 256>, grid, kWarps * 32, 0, 1, kv, b, a);
+        auto kern = head_dim == 64 ? kv_append_kernel<T, 64> : head_dim == 128 ? kv_append_kernel<T, 128> : kv_append_kernel<T, 256>;
+        launch_op(ctx, kern, s.grid, kWarps * 32, 0, 1, kv, b, a, s.tokens);
     });
     ls.done("kv_append_kernel");
 }
 
 void launch_kv_read(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, float* k, float* v) {
-    const dim3 grid(b.n_tokens, slices(ctx, b.n_tokens, 2u * kv.kv_heads * (head_dim / kKvGroup)));
+    const Shape s = shape_of(ctx, b.n_tokens, 2u * kv.kv_heads * (head_dim / kKvGroup));
     const bool vec = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16u == 0;
     LaunchScope ls(ctx, KC_KV_CACHE);
-    if (head_dim == 64) launch_op(ctx, kv_read_kernel<64>, grid, kWarps * 32, 0, 1, kv, b, k, v, vec);
-    else if (head_dim == 128) launch_op(ctx, kv_read_kernel<128>, grid, kWarps * 32, 0, 1, kv, b, k, v, vec);
-    else launch_op(ctx, kv_read_kernel<256>, grid, kWarps * 32, 0, 1, kv, b, k, v, vec);
+    auto kern = head_dim == 64 ? kv_read_kernel<64> : head_dim == 128 ? kv_read_kernel<128> : kv_read_kernel<256>;
+    launch_op(ctx, kern, s.grid, kWarps * 32, 0, 1, kv, b, k, v, vec, s.tokens);
     ls.done("kv_read_kernel");
 }
 
