@@ -33,7 +33,6 @@ constexpr uint32_t kWarps = 4, kThreads = kWarps * 32, kPiece = 32, kBlockKeys =
 constexpr float kSlack = 6.0f;
 template <int HD>
 constexpr uint32_t kPitch = HD + 4;      // of a row of outputs with its maximum and sum
-constexpr uint32_t kMostPerSm = 5;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -121,108 +120,132 @@ struct Seq {
     __device__ __forceinline__ uint64_t head_weight() const { return static_cast<uint64_t>(tiles / 2u) * pair_weight + mid_weight; }
 };
 
-// One warp's eight query rows: fragments, running maxima and sums, outputs. Lane (g, t) = (lane / 4, lane % 4) has the
-// scores of row g for keys 2t, 2t + 1 of every eight, and the outputs of rows 2t, 2t + 1 for values 64 u + 8 g .. + 7.
-template <typename T, int HD>
+// A warp's query rows, 8 H of them: fragments, running maxima and sums, outputs. Lane (g, t) = (lane / 4, lane % 4) has the
+// scores of rows g + 8 h for keys 2t, 2t + 1 of every eight, and the outputs of rows 8 h + 2t, + 2t + 1 for values
+// 64 u + 8 g .. + 7.
+// H = 1: eight rows, q and p step each as a rounding and what it left. H = 2: sixteen rows, roundings alone (16-bit q are
+// exact in fp16; p step rounds to 2^-12 of itself, next to what rounding the output costs).
+template <typename T, int HD, int H>
 struct Rows {
     static constexpr uint32_t W = HD / 32, G = HD / 64;
-    static constexpr bool kOnce = std::is_same<T, __nv_bfloat16>::value, kFine = std::is_same<T, float>::value;
+    static constexpr bool kFine = std::is_same<T, float>::value;
+    static constexpr bool kOnce = H == 2 || std::is_same<T, __nv_bfloat16>::value;      // bf16 rounds eight times as coarsely as p step
     static constexpr float kOdd = kFine ? 1.0f : 16.0f;      // odd pairs of codes count one in kOdd
     static constexpr bool kShared = HD >= 128;     // q fragments in shared memory: the registers go to the outputs
     static constexpr uint32_t kMetaBytes = 2u * G * 16u * 16u;      // of a piece, widened
     uint32_t q[kShared ? 1 : W * 2][4];
-    float o[G][4][4];    // tile n of a group: values 8 g + n (rows 2t, 2t + 1), 8 g + 4 + n (rows 2t, 2t + 1)
-    f32x2 om[G], l;      // over even and odd keys
-    float sum_q[G];
-    float factor, m, escale;
-    uint32_t vmax;      // the largest step of the values so far, as bits
-    int32_t limit;      // keys that this lane's row sees
-    int32_t least;      // the fewest that one of the warp's rows sees, the most
+    float o[H][G][4][4];     // tile n of a group: values 8 g + n (rows 2t, 2t + 1), 8 g + 4 + n (rows 2t, 2t + 1)
+    f32x2 om[H][G], l[H];    // over even and odd keys
+    float sum_q[H][G];
+    float factor[H], m[H], escale;
+    uint32_t vmax;           // the largest step of the values so far, as bits
+    int32_t limit[H];        // keys that this lane's rows see
+    int32_t least;           // the fewest that one of the warp's rows sees, the most
     int32_t most;
 
-    // Lane (g, t): row g of the tile, values 64 (w / 2) + 16 t + 8 (w % 2) + n of words w.
-    // Of `parts` warps with the same rows, number `part` writes its part of shared fragments.
+    // Lane (g, t): rows g + 8 h of the tile, values 64 (w / 2) + 16 t + 8 (w % 2) + n of words w. Of `parts` warps with the
+    // same rows, number `part` writes its part of shared fragments.
     __device__ __forceinline__ void load(const AttnParams& p, const Seq& s, uint32_t kvh, uint32_t row, uint32_t lane, uint4* shared, uint32_t part,
                                          uint32_t parts) {
-        const uint32_t t = lane & 3u, rr = row + (lane >> 2);
-        const uint32_t tok = rr / p.group, head = kvh * p.group + rr % p.group;
-        const bool there = tok < s.n_new;
-        limit = there ? static_cast<int32_t>(min(max(s.base + tok + 1, static_cast<int64_t>(0)), s.cap)) : 0;
-        least = __reduce_min_sync(0xFFFFFFFFu, there ? limit : 0x7FFFFFFF);
-        most = __reduce_max_sync(0xFFFFFFFFu, limit);
-        const T* src = static_cast<const T*>(p.a.q) + static_cast<size_t>(s.row0 + (there ? tok : 0u)) * p.a.q_stride + static_cast<size_t>(head) * HD;
-        if (!there) src = static_cast<const T*>(p.a.q);
-        float x[W][8], big = 0.0f;
+        const uint32_t t = lane & 3u;
+        least = 0x7FFFFFFF;
+        most = 0;
+        uint32_t kept[H][H == 2 ? W * 4 : 1];      // a row's roundings, for H = 2 to be paired with the other row's
 #pragma unroll
-        for (uint32_t w = 0; w < W; ++w) {
-            const T* from = src + 64u * (w / 2u) + 16u * t + 8u * (w % 2u);
-            if (p.vec) {
-                constexpr uint32_t N = 16u / sizeof(T);
+        for (uint32_t h = 0; h < H; ++h) {
+            const uint32_t rr = row + 8u * h + (lane >> 2), tok = rr / p.group, head = kvh * p.group + rr % p.group;
+            const bool there = tok < s.n_new;
+            limit[h] = there ? static_cast<int32_t>(min(max(s.base + tok + 1, static_cast<int64_t>(0)), s.cap)) : 0;
+            least = min(least, there ? limit[h] : 0x7FFFFFFF);
+            most = max(most, limit[h]);
+            const T* src = static_cast<const T*>(p.a.q) + static_cast<size_t>(s.row0 + (there ? tok : 0u)) * p.a.q_stride + static_cast<size_t>(head) * HD;
+            if (!there) src = static_cast<const T*>(p.a.q);
+            float x[W][8], big = 0.0f;
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; i += N) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(from + i);
-                    const T* e = reinterpret_cast<const T*>(&v);
+            for (uint32_t w = 0; w < W; ++w) {
+                const T* from = src + 64u * (w / 2u) + 16u * t + 8u * (w % 2u);
+                if (p.vec) {
+                    constexpr uint32_t N = 16u / sizeof(T);
 #pragma unroll
-                    for (uint32_t j = 0; j < N; ++j) x[w][i + j] = op_widen(e[j]);
-                }
-            } else {
+                    for (uint32_t i = 0; i < 8u; i += N) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(from + i);
+                        const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) x[w][i] = op_widen(from[i]);
-            }
-        }
-#pragma unroll
-        for (uint32_t w = 0; w < W; ++w)
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) {
-                if (!there) x[w][i] = 0.0f;
-                big = fmaxf(big, fabsf(x[w][i]));
-            }
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-        // 2^e above the largest |q|: q 2^(top - e) < 2^15 (and sixteen times that), exact but for the last bits of what is
-        // 2^-20 of the largest
-        constexpr int kTop = kFine ? 15 : 11;
-        const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : kTop;
-        // the scale's sign goes with q: the largest score / factor is the largest score
-        const float up = copysignf(power_of_two(kTop - e), p.a.scale);
-        factor = fabsf(p.a.scale) * 1.4426950408889634f * power_of_two(min(e - kTop + kCodeShift, 127));
-#pragma unroll
-        for (uint32_t g = 0; g < G; ++g) sum_q[g] = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < W; ++w) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) {
-                x[w][i] *= up;
-                sum_q[w / 2u] += x[w][i];
-            }
-#pragma unroll
-            for (uint32_t h = 0; h < 2u; ++h) {
-                if (kShared && w % parts != part) continue;
-                // values 2h, 2h + 4 meet even pairs of codes, 2h + 1, 2h + 5 odd ones
-                uint32_t f[4];
-                split(pack2(x[w][2 * h], x[w][2 * h + 4]), f[0], f[1]);
-                split(pack2(x[w][2 * h + 1] * kOdd, x[w][2 * h + 5] * kOdd), f[2], f[3]);
-                if constexpr (kShared) {
-                    shared[(w * 2u + h) * 32u + lane] = make_uint4(f[0], f[1], f[2], f[3]);
+                        for (uint32_t j = 0; j < N; ++j) x[w][i + j] = op_widen(e[j]);
+                    }
                 } else {
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; ++i) q[w * 2u + h][i] = f[i];
+                    for (uint32_t i = 0; i < 8u; ++i) x[w][i] = op_widen(from[i]);
                 }
             }
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w)
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    if (!there) x[w][i] = 0.0f;
+                    big = fmaxf(big, fabsf(x[w][i]));
+                }
+            big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+            // 2^e above the largest |q|: q 2^(top - e) < 2^15 (and sixteen times that), exact but for the last bits of what is
+            // 2^-20 of the largest
+            constexpr int kTop = kFine ? 15 : 11;
+            const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : kTop;
+            // the scale's sign goes with q: the largest score / factor is the largest score
+            const float up = copysignf(power_of_two(kTop - e), p.a.scale);
+            factor[h] = fabsf(p.a.scale) * 1.4426950408889634f * power_of_two(min(e - kTop + kCodeShift, 127));
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g) sum_q[h][g] = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    x[w][i] *= up;
+                    sum_q[h][w / 2u] += x[w][i];
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 2u; ++i) {
+                    if (kShared && w % parts != part) continue;
+                    // values 2i, 2i + 4 meet even pairs of codes, 2i + 1, 2i + 5 odd ones
+                    const f32x2 even = pack2(x[w][2 * i], x[w][2 * i + 4]), odd = pack2(x[w][2 * i + 1] * kOdd, x[w][2 * i + 5] * kOdd);
+                    uint32_t f[4];
+                    if constexpr (H == 1) {
+                        split(even, f[0], f[1]);
+                        split(odd, f[2], f[3]);
+                    } else {
+                        const float2 ev = unpack2(even), od = unpack2(odd);
+                        kept[h][(w * 2u + i) * 2u] = bits_of(__floats2half2_rn(ev.x, ev.y));
+                        kept[h][(w * 2u + i) * 2u + 1u] = bits_of(__floats2half2_rn(od.x, od.y));
+                        if (h == 0u) continue;
+                        f[0] = kept[0][(w * 2u + i) * 2u];
+                        f[1] = kept[H - 1][(w * 2u + i) * 2u];
+                        f[2] = kept[0][(w * 2u + i) * 2u + 1u];
+                        f[3] = kept[H - 1][(w * 2u + i) * 2u + 1u];
+                    }
+                    if constexpr (kShared) {
+                        shared[(w * 2u + i) * 32u + lane] = make_uint4(f[0], f[1], f[2], f[3]);
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; ++j) q[w * 2u + i][j] = f[j];
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g) {
+                sum_q[h][g] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[h][g], 1);
+                sum_q[h][g] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[h][g], 2);
+                sum_q[h][g] *= power_of_two(-kCodeShift);
+                om[h][g] = pack2(0.0f, 0.0f);
+#pragma unroll
+                for (uint32_t n = 0; n < 4u; ++n)
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j) o[h][g][n][j] = 0.0f;
+            }
+            m[h] = -FLT_MAX;
+            l[h] = pack2(0.0f, 0.0f);
         }
-#pragma unroll
-        for (uint32_t g = 0; g < G; ++g) {
-            sum_q[g] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[g], 1);
-            sum_q[g] += __shfl_xor_sync(0xFFFFFFFFu, sum_q[g], 2);
-            sum_q[g] *= power_of_two(-kCodeShift);
-            om[g] = pack2(0.0f, 0.0f);
-#pragma unroll
-            for (uint32_t n = 0; n < 4u; ++n)
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) o[g][n][j] = 0.0f;
-        }
-        m = -FLT_MAX;
-        l = pack2(0.0f, 0.0f);
+        least = __reduce_min_sync(0xFFFFFFFFu, least);
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
         escale = 1.0f;
         vmax = 0;
     }
@@ -262,7 +285,7 @@ struct Rows {
         }
         __syncwarp();
         // ---- scores ----
-        f32x2 sc[4];             // scores / factor
+        f32x2 sc[H][4];             // scores / factor
 #pragma unroll
         for (uint32_t gq = 0; gq < G; ++gq) {
             float acc[4][4];
@@ -295,41 +318,47 @@ struct Rows {
                     mma16816(acc[nt], f[1][0], f[1][1], f[1][2], f[1][3], r[2], r[3]);
                 }
             }
-            const f32x2 sq = pack2(sum_q[gq], sum_q[gq]);
 #pragma unroll
             for (uint32_t nt = 0; nt < 4u; ++nt) {
                 const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(meta + (gq * 16u + 4u * nt + t) * 16u);     // steps, minima
-                const f32x2 low = gq ? fma2(v.y, sq, sc[nt]) : mul2(v.y, sq);
-                sc[nt] = fma2(v.x, add2(pack2(acc[nt][0], acc[nt][1]), pack2(acc[nt][2], acc[nt][3])), low);
+#pragma unroll
+                for (uint32_t h = 0; h < H; ++h) {
+                    const f32x2 sq = pack2(sum_q[h][gq], sum_q[h][gq]);
+                    const f32x2 low = gq ? fma2(v.y, sq, sc[h][nt]) : mul2(v.y, sq);
+                    const f32x2 dot = H == 1 ? add2(pack2(acc[nt][0], acc[nt][1]), pack2(acc[nt][2], acc[nt][3]))
+                                             : pack2(acc[nt][2 * h], acc[nt][2 * h + 1]);
+                    sc[h][nt] = fma2(v.x, dot, low);
+                }
             }
         }
-        if (edge) {
-            // keys that a row does not see weigh nothing, whatever lies there
+        float top[H];
+        bool grows = big > vmax;
+#pragma unroll
+        for (uint32_t h = 0; h < H; ++h) {
+            if (edge) {
+                // keys that a row does not see weigh nothing, whatever lies there
+#pragma unroll
+                for (uint32_t nt = 0; nt < 4u; ++nt) {
+                    float2 v = unpack2(sc[h][nt]);
+                    const int32_t tok = tok0 + static_cast<int32_t>(8u * nt + 2u * t);
+                    const bool gone = !(there >> (nt >> 1) & 1u);
+                    if (gone || tok >= limit[h]) v.x = -INFINITY;
+                    if (gone || tok + 1 >= limit[h]) v.y = -INFINITY;
+                    sc[h][nt] = pack2(v.x, v.y);
+                }
+            }
+            top[h] = -INFINITY;
 #pragma unroll
             for (uint32_t nt = 0; nt < 4u; ++nt) {
-                float2 v = unpack2(sc[nt]);
-                const int32_t tok = tok0 + static_cast<int32_t>(8u * nt + 2u * t);
-                const bool gone = !(there >> (nt >> 1) & 1u);
-                if (gone || tok >= limit) v.x = -INFINITY;
-                if (gone || tok + 1 >= limit) v.y = -INFINITY;
-                sc[nt] = pack2(v.x, v.y);
+                const float2 v = unpack2(sc[h][nt]);
+                top[h] = fmaxf(top[h], fmaxf(v.x, v.y));
             }
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 2)) * factor[h];
+            grows = grows || top[h] > m[h] + kSlack;
         }
-        float top = -INFINITY;
-#pragma unroll
-        for (uint32_t nt = 0; nt < 4u; ++nt) {
-            const float2 v = unpack2(sc[nt]);
-            top = fmaxf(top, fmaxf(v.x, v.y));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2)) * factor;
         // The maximum follows in steps: weights may reach 2^kSlack before outputs are scaled anew
-        if (__any_sync(0xFFFFFFFFu, top > m + kSlack || big > vmax)) {
-            const float next = fmaxf(m, top), f = ex2(m - next);
-            m = next;
-            l = mul2(l, pack2(f, f));
-#pragma unroll
-            for (uint32_t u = 0; u < G; ++u) om[u] = mul2(om[u], pack2(f, f));
+        if (__any_sync(0xFFFFFFFFu, grows)) {
             float down = 1.0f;
             big = __reduce_max_sync(0xFFFFFFFFu, big);
             if (big > vmax) {
@@ -339,52 +368,71 @@ struct Rows {
                 down = next_scale / escale;
                 escale = next_scale;
             }
-            const float2 fc = of_columns(f, lane);
-            const f32x2 both = pack2(fc.x * down, fc.y * down);
 #pragma unroll
-            for (uint32_t u = 0; u < G; ++u)
+            for (uint32_t h = 0; h < H; ++h) {
+                const float next = fmaxf(m[h], top[h]), f = ex2(m[h] - next);
+                m[h] = next;
+                l[h] = mul2(l[h], pack2(f, f));
+                const float2 fc = of_columns(f, lane);
+                const f32x2 both = pack2(fc.x * down, fc.y * down);
 #pragma unroll
-                for (uint32_t n = 0; n < 4u; ++n) scale_tile(o[u][n], both);
+                for (uint32_t u = 0; u < G; ++u) {
+                    om[h][u] = mul2(om[h][u], pack2(f, f));
+#pragma unroll
+                    for (uint32_t n = 0; n < 4u; ++n) scale_tile(o[h][u][n], both);
+                }
+            }
         }
-        f32x2 p[4], pe[4];
-        const f32x2 fac = pack2(factor, factor), less = pack2(-m, -m), es = pack2(escale, escale);
+        f32x2 p[H][4];
+        const f32x2 es = pack2(escale, escale);
 #pragma unroll
-        for (uint32_t nt = 0; nt < 4u; ++nt) {
-            const float2 v = unpack2(fma2(sc[nt], fac, less));
-            p[nt] = pack2(ex2(v.x), ex2(v.y));
-            pe[nt] = mul2(p[nt], es);
-            l = add2(l, p[nt]);
+        for (uint32_t h = 0; h < H; ++h) {
+            const f32x2 fac = pack2(factor[h], factor[h]), less = pack2(-m[h], -m[h]);
+#pragma unroll
+            for (uint32_t nt = 0; nt < 4u; ++nt) {
+                const float2 v = unpack2(fma2(sc[h][nt], fac, less));
+                p[h][nt] = pack2(ex2(v.x), ex2(v.y));
+                l[h] = add2(l[h], p[h][nt]);
+            }
         }
         // ---- outputs ----
 #pragma unroll
         for (uint32_t u = 0; u < G; ++u) {
-            uint32_t hi[4], lo[4];
-            float eight[4];
+            uint32_t hi[H][4], lo[4];
+            float eight[H][4];
 #pragma unroll
             for (uint32_t nt = 0; nt < 4u; ++nt) {
-                ulonglong2 v = *reinterpret_cast<const ulonglong2*>(meta + ((G + u) * 16u + 4u * nt + t) * 16u);     // steps, minima + 8 steps
-                if (edge) {
-                    const int32_t tok = tok0 + static_cast<int32_t>(8u * nt + 2u * t);
-                    float2 st = unpack2(v.x), mn = unpack2(v.y);
-                    if (tok >= limit) st.x = mn.x = 0.0f;
-                    if (tok + 1 >= limit) st.y = mn.y = 0.0f;
-                    v.x = pack2(st.x, st.y);
-                    v.y = pack2(mn.x, mn.y);
-                }
-                om[u] = fma2(p[nt], v.y, om[u]);
-                const f32x2 w = mul2(pe[nt], v.x);
-                if constexpr (kOnce) {       // bf16 outputs round eight times as coarsely as fp16 weights
-                    const float2 x = unpack2(w);
-                    hi[nt] = bits_of(__floats2half2_rn(x.x, x.y));
-                } else {
-                    split(w, hi[nt], lo[nt]);
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(meta + ((G + u) * 16u + 4u * nt + t) * 16u);     // steps, minima + 8 steps
+                const f32x2 steps = mul2(v.x, es);
+#pragma unroll
+                for (uint32_t h = 0; h < H; ++h) {
+                    f32x2 st = steps, mn = v.y;
+                    if (edge) {
+                        const int32_t tok = tok0 + static_cast<int32_t>(8u * nt + 2u * t);
+                        float2 a = unpack2(st), b = unpack2(mn);
+                        if (tok >= limit[h]) a.x = b.x = 0.0f;
+                        if (tok + 1 >= limit[h]) a.y = b.y = 0.0f;
+                        st = pack2(a.x, a.y);
+                        mn = pack2(b.x, b.y);
+                    }
+                    om[h][u] = fma2(p[h][nt], mn, om[h][u]);
+                    const f32x2 w = mul2(p[h][nt], st);
+                    if constexpr (kOnce) {
+                        const float2 x = unpack2(w);
+                        hi[h][nt] = bits_of(__floats2half2_rn(x.x, x.y));
+                    } else {
+                        split(w, hi[h][nt], lo[nt]);
+                    }
                 }
             }
-            mma16816_first(eight, kEights, kEights, kEights, kEights, hi[0], hi[1]);
-            mma16816(eight, kEights, kEights, kEights, kEights, hi[2], hi[3]);
-            if constexpr (!kOnce) {
-                mma16816(eight, kEights, kEights, kEights, kEights, lo[0], lo[1]);
-                mma16816(eight, kEights, kEights, kEights, kEights, lo[2], lo[3]);
+#pragma unroll
+            for (uint32_t h = 0; h < H; ++h) {
+                mma16816_first(eight[h], kEights, kEights, kEights, kEights, hi[h][0], hi[h][1]);
+                mma16816(eight[h], kEights, kEights, kEights, kEights, hi[h][2], hi[h][3]);
+                if constexpr (!kOnce) {
+                    mma16816(eight[h], kEights, kEights, kEights, kEights, lo[0], lo[1]);
+                    mma16816(eight[h], kEights, kEights, kEights, kEights, lo[2], lo[3]);
+                }
             }
 #pragma unroll
             for (uint32_t b = 0; b < 2u; ++b) {
@@ -397,15 +445,16 @@ struct Rows {
                 widen_codes<kFine>(w1.y, r3);
 #pragma unroll
                 for (uint32_t n = 0; n < 4u; ++n) {
-                    mma16816(o[u][n], r0[n], r1[n], r2[n], r3[n], hi[2u * b], hi[2u * b + 1u]);
-                    if constexpr (!kOnce) mma16816(o[u][n], r0[n], r1[n], r2[n], r3[n], lo[2u * b], lo[2u * b + 1u]);
+#pragma unroll
+                    for (uint32_t h = 0; h < H; ++h) mma16816(o[h][u][n], r0[n], r1[n], r2[n], r3[n], hi[h][2u * b], hi[h][2u * b + 1u]);
+                    if constexpr (!kOnce) mma16816(o[0][u][n], r0[n], r1[n], r2[n], r3[n], lo[2u * b], lo[2u * b + 1u]);
                 }
             }
 #pragma unroll
             for (uint32_t n = 0; n < 4u; ++n) {
                 const float times = n & 1u ? -1.0f / kOdd : -1.0f;
-                const f32x2 e = pack2(eight[0], eight[1]), k = pack2(times, times);
-                add_tile(o[u][n], e, k);
+#pragma unroll
+                for (uint32_t h = 0; h < H; ++h) add_tile(o[h][u][n], pack2(eight[h][0], eight[h][1]), pack2(times, times));
             }
         }
     }
@@ -428,8 +477,8 @@ struct Rows {
         c[3] = b.y;
     }
 
-    // Calls out(row, value of the head, eight values) with the outputs before the division, for rows 2t and 2t + 1, and
-    // row(row, maximum, sum) once for each row.
+    // Calls out(row, value of the head, eight values, sum) with the outputs before the division, for rows 8 h + 2t and + 2t + 1,
+    // and row(row, maximum, sum) once for each row.
     template <typename Out, typename Row>
     __device__ __forceinline__ void finish(uint32_t lane, Out&& out, Row&& row) {
         const uint32_t g = lane >> 2, t = lane & 3u;
@@ -439,23 +488,27 @@ struct Rows {
             x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
             return x + __shfl_xor_sync(0xFFFFFFFFu, x, 2);
         };
-        const float sum = all(l), down = power_of_two(kCodeShift) / escale;
-        const float2 sums = of_columns(sum, lane);
-        if (t == 0) row(g, m, sum);
+        const float down = power_of_two(kCodeShift) / escale;
 #pragma unroll
-        for (uint32_t u = 0; u < G; ++u) {
-            const float2 mins = of_columns(all(om[u]), lane);
-            float v[2][8];
+        for (uint32_t h = 0; h < H; ++h) {
+            const float sum = all(l[h]);
+            const float2 sums = of_columns(sum, lane);
+            if (t == 0) row(8u * h + g, m[h], sum);
 #pragma unroll
-            for (uint32_t n = 0; n < 4u; ++n) {
-                const float d = n & 1u ? down * kOdd : down;
-                v[0][n] = fmaf(o[u][n][0], d, mins.x);
-                v[1][n] = fmaf(o[u][n][1], d, mins.y);
-                v[0][4 + n] = fmaf(o[u][n][2], d, mins.x);
-                v[1][4 + n] = fmaf(o[u][n][3], d, mins.y);
+            for (uint32_t u = 0; u < G; ++u) {
+                const float2 mins = of_columns(all(om[h][u]), lane);
+                float v[2][8];
+#pragma unroll
+                for (uint32_t n = 0; n < 4u; ++n) {
+                    const float d = n & 1u ? down * kOdd : down;
+                    v[0][n] = fmaf(o[h][u][n][0], d, mins.x);
+                    v[1][n] = fmaf(o[h][u][n][1], d, mins.y);
+                    v[0][4 + n] = fmaf(o[h][u][n][2], d, mins.x);
+                    v[1][4 + n] = fmaf(o[h][u][n][3], d, mins.y);
+                }
+                out(8u * h + 2u * t, 64u * u + 8u * g, v[0], sums.x);
+                out(8u * h + 2u * t + 1u, 64u * u + 8u * g, v[1], sums.y);
             }
-            out(2u * t, 64u * u + 8u * g, v[0], sums.x);
-            out(2u * t + 1u, 64u * u + 8u * g, v[1], sums.y);
         }
     }
     // Row r's output before the division, maximum and sum, to `to`: [row][HD + 4].
@@ -515,6 +568,9 @@ __device__ __forceinline__ void store_row(T* to, const float (&v)[8], float by, 
     }
 }
 
+// CTAs an SM: what the registers of the outputs leave room for.
+template <int HD, int H>
+__host__ __device__ constexpr int ctas() { return HD > 128 ? 2 : HD * H > 128 ? 3 : 4; }
 // Stages of 32 keys that a warp (KEYS) or the CTA keeps on their way.
 template <int HD, bool KEYS>
 __host__ __device__ constexpr uint32_t stages() { return !KEYS || HD == 64 ? 4u : 2u; }
@@ -524,13 +580,13 @@ constexpr size_t smem_bytes() {
            (HD >= 128 ? (KEYS ? 1u : kWarps) * (HD / 16u) * 512u : 0u);
 }
 
-// KEYS: the four warps share a tile of eight rows and take sixteen keys of a block each (a decode step);
-// else each has eight rows of a tile of 32 of its own and all see the same keys (prompts).
-template <typename T, int HD, bool KEYS>
-__global__ void __launch_bounds__(kThreads, HD > 128 ? 2 : 5)
+// KEYS: the four warps share a tile of eight rows and take 32 keys of a block each (a decode step); else each has 8 H
+// rows of its own and all see the same keys (prompts).
+template <typename T, int HD, bool KEYS, int H>
+__global__ void __launch_bounds__(kThreads, ctas<HD, H>())
 kv_attention_kernel(AttnParams p) {
-    constexpr uint32_t TILE = KEYS ? 8u : 32u, SB = 18u * HD;      // SB: a block of sixteen tokens
-    using Warp = Rows<T, HD>;
+    constexpr uint32_t TILE = KEYS ? 8u : 32u * H, SB = 18u * HD;      // SB: a block of sixteen tokens
+    using Warp = Rows<T, HD, H>;
     constexpr uint32_t kStages = stages<HD, KEYS>(), kStageBytes = 2u * SB;
     extern __shared__ __align__(128) uint8_t smem[];
     // stages (of each warp, or of all); for each warp, widened steps and minima; q fragments (head_dim 128 and 256). Rows to be
@@ -720,7 +776,7 @@ kv_attention_kernel(AttnParams p) {
             };
             if (tid == 0)
                 for (uint32_t i = 0; i < min(n, kStages); ++i) issue(i);
-            rows.load(p, sq, kvh, tile * TILE + warp * 8u, lane, my_q, 0u, 1u);
+            rows.load(p, sq, kvh, tile * TILE + warp * 8u * H, lane, my_q, 0u, 1u);
             __syncwarp();
             for (uint32_t i = 0; i < n; ++i) {
                 const uint32_t k = turn + i, st = k % kStages, sub = 2u * (first + i);
@@ -765,10 +821,10 @@ kv_attention_kernel(AttnParams p) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the stages are copied into again
             __syncthreads();
         } else if (!whole) {
-            rows.store(slot + warp * 8u * kPitch<HD>, lane);
+            rows.store(slot + warp * 8u * H * kPitch<HD>, lane);
         } else {
             rows.finish(
-                lane, [&](uint32_t r, uint32_t d, const float(&v)[8], float sum) { write(warp * 8u + r, d, v, sum); }, [](uint32_t, float, float) {});
+                lane, [&](uint32_t r, uint32_t d, const float(&v)[8], float sum) { write(warp * 8u * H + r, d, v, sum); }, [](uint32_t, float, float) {});
         }
         if (!whole) {
             // CTA c has place v if floor(c total / ctas) <= v < floor((c + 1) total / ctas)
@@ -804,33 +860,39 @@ kv_attention_kernel(AttnParams p) {
     }
 }
 
-template <typename T, int HD, bool KEYS>
+template <typename T, int HD, bool KEYS, int H>
 void launch(csdr_context* ctx, AttnParams& p) {
     constexpr size_t smem = smem_bytes<HD, KEYS>();
-    auto kern = kv_attention_kernel<T, HD, KEYS>;
+    auto kern = kv_attention_kernel<T, HD, KEYS, H>;
     const void* key = reinterpret_cast<const void*>(kern);
     ctx->opt_in_smem(key, smem);
     auto& fit = ctx->occupancy[key];
     if (!fit.second) {
         int n = 0;
         CSDR_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kThreads, smem));
-        fit = {smem, std::max(1, std::min(n, static_cast<int>(kMostPerSm)))};
+        fit = {smem, std::max(1, std::min(n, ctas<HD, H>()))};
     }
     launch_op(ctx, kern, dim3(static_cast<unsigned>(ctx->sm_count * fit.second)), kThreads, smem, 1, p);
 }
 
-template <typename T>
-void launch_typed(csdr_context* ctx, uint32_t head_dim, bool keys, AttnParams& p) {
-    if (head_dim == 64) keys ? launch<T, 64, true>(ctx, p) : launch<T, 64, false>(ctx, p);
-    else if (head_dim == 128) keys ? launch<T, 128, true>(ctx, p) : launch<T, 128, false>(ctx, p);
-    else keys ? launch<T, 256, true>(ctx, p) : launch<T, 256, false>(ctx, p);
+template <typename T, int HD>
+void launch_rows(csdr_context* ctx, uint64_t rows, AttnParams& p) {
+    // query rows of a sequence and kv head, on average. Less than two tiles of eight: the warps share the rows; more: the keys
+    if (rows < 16u) {
+        launch<T, HD, true, 1>(ctx, p);
+    } else if constexpr (std::is_same<T, float>::value || HD > 128) {
+        launch<T, HD, false, 1>(ctx, p);
+    } else {
+        launch<T, HD, false, 2>(ctx, p);
+    }
 }
 
 }  // namespace
 
-size_t kv_attention_counters(const csdr_context* ctx) { return static_cast<size_t>(ctx->sm_count) * kMostPerSm; }
+size_t kv_attention_counters(const csdr_context* ctx) { return static_cast<size_t>(ctx->sm_count) * 4u; }
 size_t kv_attention_workspace(const csdr_context* ctx, uint32_t head_dim) {
-    return kv_attention_counters(ctx) * (4u + 2u * 32u * (head_dim + 4u) * 4u);
+    // two pieces of a tile of at most 64 rows (32 for the widest heads) a CTA, at most four CTAs an SM
+    return kv_attention_counters(ctx) * (4u + 2u * (head_dim > 128u ? 32u : 64u) * (head_dim + 4u) * 4u);
 }
 
 void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim, const KvBatchView& b, int dtype, const KvAttend& a, void* workspace) {
@@ -846,10 +908,14 @@ void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim,
     const size_t es = dtype == CSDR_DTYPE_F32 ? 4 : 2;
     p.vec = (reinterpret_cast<uintptr_t>(a.q) | a.q_stride * es) % 16u == 0;
     p.vec_out = (reinterpret_cast<uintptr_t>(a.out) | a.out_stride * es) % 16u == 0;
-    // rows of a sequence that share keys: from two tiles of eight on, warps with rows of their own
-    const bool keys = static_cast<uint64_t>(b.n_tokens) * p.group < 16u * static_cast<uint64_t>(b.n_seqs);
+    const uint64_t rows = static_cast<uint64_t>(b.n_tokens) * p.group / b.n_seqs;
     LaunchScope ls(ctx, KC_KV_ATTENTION);
-    with_dtype(dtype, [&](auto* t) { launch_typed<std::remove_pointer_t<decltype(t)>>(ctx, head_dim, keys, p); });
+    with_dtype(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (head_dim == 64) launch_rows<T, 64>(ctx, rows, p);
+        else if (head_dim == 128) launch_rows<T, 128>(ctx, rows, p);
+        else launch_rows<T, 256>(ctx, rows, p);
+    });
     ls.done("kv_attention_kernel");
 }
 
