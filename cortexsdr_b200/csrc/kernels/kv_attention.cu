@@ -594,6 +594,8 @@ kv_attention_kernel(AttnParams p) {
     uint8_t* ring = smem;
     uint8_t* meta_s = smem + (KEYS ? kWarps : 1u) * kStages * kStageBytes;
     __shared__ uint64_t bars[kWarps * kStages];
+    __shared__ uint64_t empty[kStages];      // where the warps share stages: all are through with one
+    __shared__ uint32_t there_s[kStages];
     __shared__ uint64_t scan[kWarps];
     __shared__ uint64_t found_at;
     __shared__ uint32_t found, flag, longest;
@@ -606,6 +608,7 @@ kv_attention_kernel(AttnParams p) {
     const uint32_t my_bar = smem_u32(&bars[KEYS ? warp * kStages : 0u]);
     if (tid == 0) {
         for (uint32_t i = 0; i < kWarps * kStages; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&bars[i])));
+        for (uint32_t i = 0; i < kStages; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&empty[i])), "r"(kWarps));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         longest = 0;
     }
@@ -764,33 +767,40 @@ kv_attention_kernel(AttnParams p) {
             __syncwarp();
             rows.store(rows_of(warp), lane);
         } else {
-            // all warps see every piece; thread 0 copies, everyone asks for the pages
-            const uint32_t first = 4u * b0, n = min(4u * (b1 - b0), (max(subs, 2u * first) - 2u * first + 1u) / 2u);
-            auto page_at = [&](uint32_t sub) -> int32_t {
-                const int32_t page = sub < subs ? __ldg(table + (sub >> (p.kv.page_shift - 4u))) : -1;
-                return static_cast<uint32_t>(page) < p.kv.n_pages ? page : -1;
-            };
+            // All warps see every piece. Warp 0 copies: a stage when all are through with it, one piece behind their work
+            const uint32_t first = 4u * b0, n = min(4u * (b1 - b0), (max(subs, 2u * first) - 2u * first + 1u) / 2u), turn0 = turn;
+            int32_t page_of = -1;
             auto issue = [&](uint32_t i) {
-                const uint32_t st = (turn + i) % kStages, sub = 2u * (first + i);
-                fetch(my_ring + st * kStageBytes, my_bar + 8u * st, sub, page_at(sub), page_at(sub + 1u));
+                if ((i & 15u) == 0u) {
+                    const uint32_t sub = 2u * (first + i) + lane;
+                    page_of = sub < subs ? __ldg(table + (sub >> (p.kv.page_shift - 4u))) : -1;
+                    if (static_cast<uint32_t>(page_of) >= p.kv.n_pages) page_of = -1;
+                }
+                const int32_t pg0 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u)), pg1 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u) + 1u);
+                const uint32_t k = turn0 + i, st = k % kStages;
+                if (k >= kStages) live = live && mbar_wait(smem_u32(&empty[st]), (k / kStages - 1u) & 1u, p.spin);
+                if (live && lane == 0) {
+                    there_s[st] = (pg0 >= 0 ? 1u : 0u) | (pg1 >= 0 ? 2u : 0u);
+                    fetch(my_ring + st * kStageBytes, my_bar + 8u * st, 2u * (first + i), pg0, pg1);
+                }
             };
-            if (tid == 0)
+            if (warp == 0)
                 for (uint32_t i = 0; i < min(n, kStages); ++i) issue(i);
             rows.load(p, sq, kvh, tile * TILE + warp * 8u * H, lane, my_q, 0u, 1u);
             __syncwarp();
-            for (uint32_t i = 0; i < n; ++i) {
-                const uint32_t k = turn + i, st = k % kStages, sub = 2u * (first + i);
-                live = live && mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
-                const int32_t tok = static_cast<int32_t>(16u * sub);
-                if (live && tok < rows.most)
-                    rows.piece(my_ring + st * kStageBytes, tok, (page_at(sub) >= 0 ? 1u : 0u) | (page_at(sub + 1u) >= 0 ? 2u : 0u), lane, my_q, my_meta);
-                live = __syncthreads_and(live);
+            for (uint32_t i = 0; i < n && live; ++i) {
+                const uint32_t k = turn0 + i, st = k % kStages;
+                live = mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
                 if (!live) break;
-                if (tid == 0 && i + kStages < n) issue(i + kStages);
+                const int32_t tok = static_cast<int32_t>(kPiece * (first + i));
+                if (tok < rows.most) rows.piece(my_ring + st * kStageBytes, tok, there_s[st], lane, my_q, my_meta);
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[st])) : "memory");
+                if (warp == 0 && i >= 1u && i - 1u + kStages < n) issue(i - 1u + kStages);
             }
             turn += n;
         }
-        if constexpr (KEYS) live = __syncthreads_and(live);
+        live = __syncthreads_and(live);
         if (!live) {
             if (tid == 0) atomicExch(p.status, 1);
         }
