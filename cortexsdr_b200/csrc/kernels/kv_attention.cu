@@ -34,30 +34,6 @@ constexpr float kSlack = 6.0f;
 template <int HD>
 constexpr uint32_t kPitch = HD + 4;      // of a row of outputs with its maximum and sum
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"      // callers stop at p.spin, the wait limit
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return done != 0u;
-}
-// The whole warp waits, and gives up as one.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
-    if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
-    for (uint32_t spin = 0; spin < limit; ++spin)
-        if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
-    return false;
-}
-
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

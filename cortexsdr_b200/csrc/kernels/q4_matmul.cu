@@ -84,6 +84,9 @@ struct Q4Params {
     uint32_t n_blocks;          // of 128 rows
     uint32_t units_rank;        // units of a row tile that a CTA of a cluster takes
     uint32_t units_staged;      // of those, units whose activations fit into shared memory at a time
+    uint8_t* planes;            // activations as fragments, [token tile][unit]; null: the CTAs make them
+    int* status;
+    uint32_t spin;              // wait limit
     uint32_t x_vec;             // a token's columns lie one behind the other and start on 16 bytes
 };
 
@@ -91,33 +94,127 @@ template <int FMT, int NT, bool SPLIT>
 struct Q4Shape {
     static constexpr uint32_t kTokens = NT * (SPLIT ? 4u : 8u), kColumns = NT * 8u;
     static constexpr uint32_t kUnitCols = FMT ? 256u : 128u, kGroups = kUnitCols / 32u;
-    // activations of a unit as fragments, then the group sums that its columns need
-    static constexpr uint32_t kStageBytes = kGroups * kColumns * (64u + 4u);
-    static constexpr uint32_t kSumBytes = 2u * kRowsBlock * kTokens * 4u;      // partial results, twice
+    // of a unit: activations as fragments [group][column][t], the group sums that its columns need [group][column], and the powers
+    // of two that products are times as large [column]
+    static constexpr uint32_t kSumsAt = kGroups * kColumns * 64u, kBacksAt = kSumsAt + kGroups * kColumns * 4u;
+    static constexpr uint32_t kStageBytes = kBacksAt + kColumns * 4u;
+    // partial results of all ranks (runs of 32, so up to a run a rank more than there are), twice
+    static constexpr uint32_t kSums = kRowsBlock * kTokens + 8u * 32u, kSumBytes = 2u * kSums * 4u;
+    // units whose activations fit beside the partial results, with n CTAs an SM
+    static constexpr uint32_t staged(uint32_t n) { return ((n == 2u ? 104u : 208u) * 1024u - kSumBytes) / kStageBytes; }
 };
 
-// Eight neighbouring columns of a token; what lies behind the matrix is zero.
+// Eight neighbouring columns of a token as they lie in memory; what lies behind the matrix is zero.
 template <typename T>
-__device__ __forceinline__ void load8(const Q4Params& p, size_t tok, uint32_t col, float (&v)[8]) {
-    const T* x = static_cast<const T*>(p.a.x) + tok * p.a.x_token + static_cast<size_t>(col) * p.a.x_col;
-    if (p.x_vec) {       // columns come in multiples of 32
-        if (col >= p.w.cols) {
+struct Eight {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const Q4Params& p, size_t tok, uint32_t col) {
+        const T* x = static_cast<const T*>(p.a.x) + tok * p.a.x_token + static_cast<size_t>(col) * p.a.x_col;
+        if (col >= p.w.cols) {       // columns come in multiples of 32
 #pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) v[i] = 0.0f;
-            return;
+            for (uint32_t i = 0; i < sizeof(T) / 2; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
+        } else if (p.x_vec) {
+#pragma unroll
+            for (uint32_t i = 0; i < sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(x)[i];
+        } else {
+            T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) e[i] = x[i * p.a.x_col];
         }
-        constexpr uint32_t N = 16u / sizeof(T);
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; i += N) {
-            const uint4 q = *reinterpret_cast<const uint4*>(x + i);
-            const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-            for (uint32_t j = 0; j < N; ++j) v[i + j] = op_widen(e[j]);
-        }
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) v[i] = col + i < p.w.cols ? op_widen(x[i * p.a.x_col]) : 0.0f;
     }
+    __device__ __forceinline__ float operator[](uint32_t i) const { return op_widen(reinterpret_cast<const T*>(w)[i]); }
+};
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, uint32_t i) { return i == 0u ? v.x : i == 1u ? v.y : i == 2u ? v.z : v.w; }
+__device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// Activations as fragments: units u0 to u1, of the n_tok tokens from tok0, one unit behind the other from `to`. A power of two
+// for each token and unit brings the largest below 2^15. Sixteen lanes (32 for q4_k) have a token's columns of a unit, eight
+// each: pieces t of the unit's groups. Items `first`, `first + step`, ... of whole warps.
+template <typename T, int FMT, int NT>
+__device__ __forceinline__ void stage(const Q4Params& p, uint32_t u0, uint32_t u1, size_t tok0, uint32_t n_tok, uint8_t* to, uint32_t first, uint32_t step) {
+    constexpr bool SPLIT = std::is_same<T, float>::value, kScaled = !std::is_same<T, __half>::value;      // fp16 are operands as they come
+    using S = Q4Shape<FMT, NT, SPLIT>;
+    constexpr uint32_t kLanes = S::kGroups * 4u;
+    const uint32_t units = u1 - u0, n = units * n_tok * kLanes;
+    for (uint32_t e0 = first & ~31u; e0 < n; e0 += step) {
+        const uint32_t e = e0 + (first & 31u), q = e / kLanes, piece = e & 3u;
+        // neighbours: units or tokens, whichever lie closer in memory
+        const uint32_t unit = p.a.x_col == 1 ? q % units : q / n_tok, tok = p.a.x_col == 1 ? q / units : q % n_tok;
+        const uint32_t gr = e % kLanes / 4u;
+        const bool there = e < n;
+        float v[8];
+        uint32_t big = 0;
+        if (there) {
+            Eight<T> raw;
+            raw.load(p, tok0 + tok, ((u0 + unit) * S::kGroups + gr) * 32u + piece * 8u);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) {
+                v[i] = raw[i];
+                if (kScaled) big = max(big, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+            }
+        }
+        int ex = 14;
+        if (kScaled) {
+#pragma unroll
+            for (uint32_t o = kLanes / 2u; o; o >>= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+            // what is not finite stays as it is; 2^-100 counts as the smallest
+            if (big != 0u && big < 0x7F800000u) ex = max(static_cast<int>(big >> 23) - 127, -100);
+        }
+        const float up = power_of_two(14 - ex);
+        float sum_hi = 0.0f, sum_lo = 0.0f;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const float x = there ? v[i] * up : 0.0f, z = there ? v[i + 4] * up : 0.0f;
+            if constexpr (SPLIT) {
+                split(pack2(x, z), hi[i], lo[i]);
+                const float2 r = halves(lo[i]), h = halves(hi[i]);
+                sum_lo += r.x + r.y;
+                sum_hi += h.x + h.y;
+            } else {
+                hi[i] = bits_of(__floats2half2_rn(x, z));
+                sum_hi += x + z;      // fp16 holds them as they are
+            }
+        }
+        sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 1);
+        sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 2);
+        if constexpr (SPLIT) {
+            sum_lo += __shfl_xor_sync(0xFFFFFFFFu, sum_lo, 1);
+            sum_lo += __shfl_xor_sync(0xFFFFFFFFu, sum_lo, 2);
+        }
+        if (there) {
+            // q4_0: what the 8 of every code adds to the product; q4_k: the sum that the minimum meets
+            constexpr float kTake = FMT ? 1.0f : -8.0f / (1u << kCodeShift);
+            const uint32_t column = SPLIT ? tok / 4u * 8u + tok % 4u : tok, at = gr * S::kColumns + column;
+            uint8_t* mine = to + static_cast<size_t>(unit) * S::kStageBytes;
+            uint4* frags = reinterpret_cast<uint4*>(mine);
+            float* sums = reinterpret_cast<float*>(mine + S::kSumsAt);
+            frags[at * 4u + piece] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (SPLIT) frags[(at + 4u) * 4u + piece] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if (piece == 0u) {
+                sums[at] = sum_hi * kTake;
+                if constexpr (SPLIT) sums[at + 4u] = sum_lo * kTake;
+            }
+            if (e % kLanes == 0u) {
+                float* backs = reinterpret_cast<float*>(mine + S::kBacksAt);
+                backs[column] = power_of_two(ex - 14);
+                if constexpr (SPLIT) backs[column + 4u] = power_of_two(ex - 14);
+            }
+        }
+    }
+}
+
+// The fragments of all units and of a launch's token tiles in global memory, for products whose CTAs would otherwise all do it.
+template <typename T, int FMT, int NT>
+__global__ void __launch_bounds__(kThreads)
+q4_stage_kernel(Q4Params p, uint32_t units_cta) {
+    op_enter();
+    using S = Q4Shape<FMT, NT, std::is_same<T, float>::value>;
+    const size_t tok0 = static_cast<size_t>(blockIdx.y) * S::kTokens;
+    const uint32_t n_tok = static_cast<uint32_t>(min(static_cast<size_t>(S::kTokens), p.a.batch - tok0));
+    const uint32_t u0 = blockIdx.x * units_cta, u1 = min(u0 + units_cta, p.w.n_units);
+    stage<T, FMT, NT>(p, u0, u1, tok0, n_tok, p.planes + (static_cast<size_t>(blockIdx.y) * p.w.n_units + u0) * S::kStageBytes, threadIdx.x, kThreads);
 }
 
 // A lane's pieces of a unit: codes (pairs of groups), steps of rows g and g + 8.
@@ -140,21 +237,16 @@ struct Q4Unit {
     }
 };
 
-__device__ __forceinline__ uint32_t word_of(const uint4& v, uint32_t i) { return i == 0u ? v.x : i == 1u ? v.y : i == 2u ? v.z : v.w; }
-__device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-
-template <typename T, int FMT, int NT>
+template <typename T, int FMT, int NT, bool ONE>
 __global__ void __launch_bounds__(kThreads, 2)
 q4_matmul_kernel(Q4Params p) {
     constexpr bool SPLIT = std::is_same<T, float>::value;
     using S = Q4Shape<FMT, NT, SPLIT>;
     constexpr uint32_t kBytes = q4_unit_bytes(FMT), kAhead = FMT ? 2u : 4u;
-    constexpr bool kScaled = !std::is_same<T, __half>::value;       // fp16 activations are operands as they come
     extern __shared__ __align__(16) uint8_t smem[];
-    float* part = reinterpret_cast<float*>(smem);                             // [2][tokens][128 rows]
-    uint8_t* xs = smem + S::kSumBytes;                                        // [unit][group][column][t] 16 bytes
-    float* sums = reinterpret_cast<float*>(xs + p.units_staged * S::kGroups * S::kColumns * 64u);   // [unit][group][column]
-    __shared__ uint32_t largest[S::kTokens];
+    float* part = reinterpret_cast<float*>(smem);                             // twice
+    uint8_t* xs = smem + S::kSumBytes;                                        // units
+    __shared__ uint64_t bar;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
@@ -177,98 +269,41 @@ q4_matmul_kernel(Q4Params p) {
     // weights do not depend on what runs before
     uint32_t block = blockIdx.x / ranks;
     if (block < p.n_blocks) fetch_first(block, u_begin, min(u_end, u_begin + p.units_staged));
+    // what the others write into this CTA's shared memory needs it to be there
+    if (ranks > 1u) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     op_enter();
 
-    // ---- activations: a power of two for each token brings its largest below 2^15 ----
-    for (uint32_t i = tid; i < S::kTokens; i += kThreads) largest[i] = 0u;
-    __syncthreads();
-    if constexpr (kScaled) {
-        const uint32_t c0 = u_begin * S::kUnitCols, c1 = min(u_end * S::kUnitCols, p.w.cols);
-        if (p.a.x_col == 1) {       // a warp a token
-            for (uint32_t tok = warp; tok < n_tok; tok += kThreads / 32u) {
-                uint32_t big = 0;
-#pragma unroll 4
-                for (uint32_t c = c0 + lane * 8u; c < c1; c += 256u) {
-                    float v[8];
-                    load8<T>(p, tok0 + tok, c, v);
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) big = max(big, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-                }
-                big = __reduce_max_sync(0xFFFFFFFFu, big);
-                if (lane == 0) largest[tok] = big;
-            }
-        } else {                    // neighbouring threads have neighbouring tokens
-            const uint32_t each = kThreads / n_tok, tok = tid % n_tok;
-            const T* x = static_cast<const T*>(p.a.x) + (tok0 + tok) * p.a.x_token;
-            uint32_t big = 0;
-            if (tid / n_tok < each) {
-#pragma unroll 4
-                for (uint32_t c = c0 + tid / n_tok; c < c1; c += each) big = max(big, __float_as_uint(op_widen(x[static_cast<size_t>(c) * p.a.x_col])) & 0x7FFFFFFFu);
-                atomicMax(&largest[tok], big);
-            }
+    if (p.planes) {
+        if (tid == 0) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&bar)));
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            asm volatile("fence.proxy.async;" ::: "memory");
         }
+        __syncthreads();
     }
-    __syncthreads();
-    // what is not finite stays as it is; 2^-100 counts as the smallest
-    auto exponent = [&](uint32_t tok) {
-        if constexpr (!kScaled) return 14;
-        const uint32_t b = largest[tok];
-        return b == 0u || b >= 0x7F800000u ? 14 : max(static_cast<int>(b >> 23) - 127, -100);
-    };
-    // Columns 8 t .. 8 t + 7 of a group for one token, as one lane's operands of two products.
-    auto stage = [&](uint32_t u0, uint32_t u1) {
-        const uint32_t items = (u1 - u0) * S::kGroups * 4u * n_tok;
-        for (uint32_t e0 = 0; e0 < items; e0 += kThreads) {
-            const uint32_t e = e0 + tid;
-            // neighbouring threads: the four pieces of a group, then tokens or groups, whichever lie closer
-            const uint32_t piece = e & 3u, rest = e >> 2, groups = (u1 - u0) * S::kGroups;
-            const uint32_t gr = p.a.x_col == 1 ? rest % groups : rest / n_tok, tok = p.a.x_col == 1 ? rest / groups : rest % n_tok;
-            float v[8], sum_hi = 0.0f, sum_lo = 0.0f;
-            uint32_t hi[4], lo[4];
-            if (e < items) {
-                const float up = power_of_two(14 - exponent(tok));
-                const uint32_t col = (u0 * S::kGroups + gr) * 32u + piece * 8u;
-                load8<T>(p, tok0 + tok, col, v);
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) v[i] *= up;
-#pragma unroll
-                for (uint32_t i = 0; i < 4u; ++i) {
-                    if constexpr (SPLIT) {
-                        split(pack2(v[i], v[i + 4]), hi[i], lo[i]);
-                        const float2 r = halves(lo[i]);
-                        sum_lo += r.x + r.y;
-                    } else {
-                        hi[i] = bits_of(__floats2half2_rn(v[i], v[i + 4]));
-                    }
-                    const float2 r = halves(hi[i]);
-                    sum_hi += r.x + r.y;
-                }
-            }
-            sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 1);
-            sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 2);
-            if constexpr (SPLIT) {
-                sum_lo += __shfl_xor_sync(0xFFFFFFFFu, sum_lo, 1);
-                sum_lo += __shfl_xor_sync(0xFFFFFFFFu, sum_lo, 2);
-            }
-            if (e < items) {
-                // q4_0: what the 8 of every code adds to the product; q4_k: the sum that the minimum meets
-                constexpr float kTake = FMT ? 1.0f : -8.0f / (1u << kCodeShift);
-                const uint32_t column = SPLIT ? tok / 4u * 8u + tok % 4u : tok;
-                const uint32_t at = gr * S::kColumns + column;
-                reinterpret_cast<uint4*>(xs)[at * 4u + piece] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if constexpr (SPLIT) reinterpret_cast<uint4*>(xs)[(at + 4u) * 4u + piece] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                if (piece == 0u) {
-                    sums[at] = sum_hi * kTake;
-                    if constexpr (SPLIT) sums[at + 4u] = sum_lo * kTake;
-                }
-            }
+    uint32_t copies = 0;
+    bool live = true;
+    auto bring = [&](uint32_t u0, uint32_t u1) {
+        if (!p.planes) {
+            stage<T, FMT, NT>(p, u0, u1, tok0, n_tok, xs, tid, kThreads);
+            return;
         }
+        if (tid == 0) {
+            const uint32_t bytes = (u1 - u0) * S::kStageBytes;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&bar)), "r"(bytes) : "memory");
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(xs)),
+                         "l"(p.planes + (static_cast<size_t>(blockIdx.y) * p.w.n_units + u0) * S::kStageBytes), "r"(bytes), "r"(smem_u32(&bar))
+                         : "memory");
+        }
+        live = live && mbar_wait(smem_u32(&bar), copies & 1u, p.spin);
+        ++copies;
     };
-    if (staged_once) {
-        stage(u_begin, u_end);
+    if (staged_once && u_end > u_begin) {
+        bring(u_begin, u_end);
         __syncthreads();
     }
 
+    if (ranks > 1u) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     uint32_t turn = 0;
     bool fetched = true;
     for (; block < p.n_blocks; block += gridDim.x / ranks, turn ^= 1u) {
@@ -280,7 +315,7 @@ q4_matmul_kernel(Q4Params p) {
             const uint32_t s1 = min(s0 + p.units_staged, u_end);
             if (!staged_once) {
                 __syncthreads();
-                stage(s0, s1);
+                bring(s0, s1);
                 __syncthreads();
                 if (!fetched) fetch_first(block, s0, s1);
                 fetched = false;
@@ -291,7 +326,10 @@ q4_matmul_kernel(Q4Params p) {
                     for (uint32_t i = 0; i < kAhead; ++i) {
                         if (u + i >= s1) break;
                         Q4Unit<FMT>& w = ahead[i];
-                        const uint32_t at = (u + i - s0) * S::kGroups;
+                        const uint8_t* staged = xs + (u + i - s0) * S::kStageBytes;
+                        float z[NT][4];      // of this unit
+#pragma unroll
+                        for (uint32_t n = 0; n < NT; ++n) z[n][0] = z[n][1] = z[n][2] = z[n][3] = 0.0f;
                         float2 dA{}, dB{};
                         if constexpr (FMT) {
                             // 6-bit integers as subnormals come back times 2^-24
@@ -324,8 +362,8 @@ q4_matmul_kernel(Q4Params p) {
                             }
 #pragma unroll
                             for (uint32_t n = 0; n < NT; ++n) {
-                                const uint4 f = *(reinterpret_cast<const uint4*>(xs) + ((at + gr) * S::kColumns + n * 8u + g) * 4u + t);
-                                const float2 s = *reinterpret_cast<const float2*>(sums + (at + gr) * S::kColumns + n * 8u + 2u * t);
+                                const uint4 f = *(reinterpret_cast<const uint4*>(staged) + (gr * S::kColumns + n * 8u + g) * 4u + t);
+                                const float2 s = *reinterpret_cast<const float2*>(staged + S::kSumsAt + (gr * S::kColumns + n * 8u + 2u * t) * 4u);
                                 float c[4];
                                 if constexpr (FMT == 0) {
                                     c[0] = c[2] = s.x;
@@ -336,15 +374,29 @@ q4_matmul_kernel(Q4Params p) {
                                 }
                                 mma16816(c, a[2], b[2], a[3], b[3], f.z, f.w);
                                 if constexpr (FMT) {
-                                    y[n][0] = fmaf(mA, s.x, y[n][0]);
-                                    y[n][1] = fmaf(mA, s.y, y[n][1]);
-                                    y[n][2] = fmaf(mB, s.x, y[n][2]);
-                                    y[n][3] = fmaf(mB, s.y, y[n][3]);
+                                    z[n][0] = fmaf(mA, s.x, z[n][0]);
+                                    z[n][2] = fmaf(mB, s.x, z[n][2]);
+                                    if constexpr (!ONE) {
+                                        z[n][1] = fmaf(mA, s.y, z[n][1]);
+                                        z[n][3] = fmaf(mB, s.y, z[n][3]);
+                                    }
                                 }
-                                y[n][0] = fmaf(sA, c[0], y[n][0]);
-                                y[n][1] = fmaf(sA, c[1], y[n][1]);
-                                y[n][2] = fmaf(sB, c[2], y[n][2]);
-                                y[n][3] = fmaf(sB, c[3], y[n][3]);
+                                z[n][0] = fmaf(sA, c[0], z[n][0]);
+                                z[n][2] = fmaf(sB, c[2], z[n][2]);
+                                if constexpr (!ONE) {      // odd columns: a single token has none
+                                    z[n][1] = fmaf(sA, c[1], z[n][1]);
+                                    z[n][3] = fmaf(sB, c[3], z[n][3]);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t n = 0; n < NT; ++n) {
+                            const float2 f = *reinterpret_cast<const float2*>(staged + S::kBacksAt + (n * 8u + 2u * t) * 4u);
+                            y[n][0] = fmaf(z[n][0], f.x, y[n][0]);
+                            y[n][2] = fmaf(z[n][2], f.x, y[n][2]);
+                            if constexpr (!ONE) {
+                                y[n][1] = fmaf(z[n][1], f.y, y[n][1]);
+                                y[n][3] = fmaf(z[n][3], f.y, y[n][3]);
                             }
                         }
                         if (u + i + kAhead < s1) w.load(unit_at(block, u + i + kAhead), lane);
@@ -355,7 +407,9 @@ q4_matmul_kernel(Q4Params p) {
         // the next block's weights are on their way while this one's results are added up
         const uint32_t next = block + gridDim.x / ranks;
         if (staged_once && next < p.n_blocks) fetch_first(next, u_begin, u_end);
-        float* mine_part = part + turn * S::kTokens * kRowsBlock;
+        // A rank adds up every ranks-th run of 32 rows times tokens; all write into its shared memory. [turn][rank][result]
+        const uint32_t n_out = kRowsBlock * n_tok, share = (n_out / 32u + ranks - 1u) / ranks * 32u;
+        float* into = part + turn * S::kSums;
         if (mine) {
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) {
@@ -368,61 +422,96 @@ q4_matmul_kernel(Q4Params p) {
 #pragma unroll
                 for (uint32_t i = 0; i < 2u; ++i) {
                     if (tok + i >= n_tok) continue;
-                    const float down = power_of_two(exponent(tok + i) - 14), codes = power_of_two(FMT ? 0 : kCodeShift);
-                    mine_part[(tok + i) * kRowsBlock + row] = y[n][i] * codes * down;
-                    mine_part[(tok + i) * kRowsBlock + row + 8u] = y[n][2u + i] * codes * down;
+                    constexpr float kCodes = FMT ? 1.0f : 1u << kCodeShift;
+#pragma unroll
+                    for (uint32_t h = 0; h < 2u; ++h) {
+                        const uint32_t e = (tok + i) * kRowsBlock + row + 8u * h, run = e / 32u, owner = run % ranks;
+                        float* to = into + rank * share + run / ranks * 32u + e % 32u;
+                        *cluster.map_shared_rank(to, owner) = y[n][2u * h + i] * kCodes;
+                    }
                 }
             }
         }
         if (ranks > 1u) cluster.sync();
         else __syncthreads();
-        // a rank adds up its share
-        for (uint32_t e = rank * kThreads + tid; e < kRowsBlock * n_tok; e += ranks * kThreads) {
-            const uint32_t r = p.a.y_row == 1 ? e % kRowsBlock : e / n_tok, tok = p.a.y_row == 1 ? e / kRowsBlock : e % n_tok;
-            const size_t row = static_cast<size_t>(block) * kRowsBlock + r;
+        for (uint32_t i = tid; i < share; i += kThreads) {
+            const uint32_t e = (i / 32u * ranks + rank) * 32u + i % 32u;
+            if (e >= n_out) continue;
+            const uint32_t tok = e / kRowsBlock;
+            const size_t row = static_cast<size_t>(block) * kRowsBlock + e % kRowsBlock;
             if (row >= p.w.rows) continue;
             float sum = p.a.bias ? p.a.bias[row] : 0.0f;
-            float* at = mine_part + tok * kRowsBlock + r;
-            for (uint32_t i = 0; i < ranks; ++i) sum += *cluster.map_shared_rank(at, i);
+            for (uint32_t r = 0; r < ranks; ++r) sum += into[r * share + i];
             p.a.y[(tok0 + tok) * p.a.y_token + row * p.a.y_row] = sum;
         }
     }
-    if (ranks > 1u) cluster.sync();      // others may still read this CTA's shared memory
+    if (!live && lane == 0) atomicExch(p.status, 1);      // results are wrong, and said to be
 }
 
-template <typename T, int FMT, int NT>
+template <typename T, int FMT, int NT, bool ONE = false>
 void launch(csdr_context* ctx, Q4Params p) {
     using S = Q4Shape<FMT, NT, std::is_same<T, float>::value>;
     p.n_blocks = (p.w.rows + kRowsBlock - 1u) / kRowsBlock;
-    constexpr uint32_t kMostStaged = (96u * 1024u - S::kSumBytes) / S::kStageBytes;
-    // Two CTAs an SM. Cut the columns so that the CTA with most to do has least: blocks in turn, each its units and about
-    // two more for the join. A cut whose activations do not fit at a time stages them anew for every block.
-    const uint32_t slots = static_cast<uint32_t>(ctx->sm_count) * 2u;
-    uint32_t ranks = 1, least = UINT32_MAX;
-    for (uint32_t r = 1; r <= 8u && r <= p.w.n_units; ++r) {
-        const uint32_t units = (p.w.n_units + r - 1u) / r, clusters = slots / r;
-        const uint32_t turns = (p.n_blocks + clusters - 1u) / clusters;
-        const uint32_t cost = turns * (units * (units > kMostStaged ? 3u : 1u) + 2u);
-        if (cost < least) {
-            least = cost;
-            ranks = r;
+    // Cut the columns so that the CTA with most to do has least: blocks in turn, each its units and about two more for the
+    // join. Two CTAs an SM, or one with all of the shared memory (half the warps: a CTA alone is little faster); activations that
+    // do not fit at a time are staged anew for every block.
+    uint32_t ranks = 1, per_sm = 2;
+    float least = 1e30f;
+    for (uint32_t n = 2; n >= 1; --n) {
+        const uint32_t slots = static_cast<uint32_t>(ctx->sm_count) * n, fits = S::staged(n);
+        for (uint32_t r = 1; r <= 8u && r <= p.w.n_units; ++r) {
+            const uint32_t units = (p.w.n_units + r - 1u) / r, clusters = slots / r, turns = (p.n_blocks + clusters - 1u) / clusters;
+            const float cost = static_cast<float>(turns * (units * (units > fits ? 4u : 1u) + 2u)) * (n == 2u ? 1.0f : 0.9f);
+            if (cost < least) {
+                least = cost;
+                ranks = r;
+                per_sm = n;
+            }
         }
     }
     p.units_rank = (p.w.n_units + ranks - 1u) / ranks;
-    p.units_staged = std::min(p.units_rank, kMostStaged);
+    p.units_staged = std::min(p.units_rank, S::staged(per_sm));
     const size_t smem = S::kSumBytes + static_cast<size_t>(p.units_staged) * S::kStageBytes;
     p.x_vec = p.a.x_col == 1 && (reinterpret_cast<uintptr_t>(p.a.x) | p.a.x_token * sizeof(T)) % 16u == 0;
-    auto kern = q4_matmul_kernel<T, FMT, NT>;
+    const uint32_t clusters = std::min(p.n_blocks, static_cast<uint32_t>(ctx->sm_count) * per_sm / ranks);
+    auto kern = q4_matmul_kernel<T, FMT, NT, ONE>;
     ctx->opt_in_smem(reinterpret_cast<const void*>(kern), smem);
-    const uint32_t clusters = std::min(p.n_blocks, slots / ranks);
-    const dim3 grid(clusters * ranks, static_cast<unsigned>((p.a.batch + S::kTokens - 1u) / S::kTokens));
-    launch_op(ctx, kern, grid, kThreads, smem, ranks, p);
+    p.status = ctx->status_word;
+    p.spin = ctx->spin_limit_barrier;
+    // A CTA makes its activations' fragments itself while that is a turn or two of its threads (11008 x 4096 q4_0, one token: 9 us,
+    // with a launch before it 10.4); else a launch makes them once for all (11008 x 4096 q4_k, 8 fp16 tokens: 16 us without,
+    // 12.9 with; 32 tokens: 47 and 34). Token tiles a launch: what 16 MB of fragments hold. Where nothing may be allocated, the
+    // CTAs do it.
+    const size_t tiles = (p.a.batch + S::kTokens - 1u) / S::kTokens, tile_bytes = static_cast<size_t>(p.w.n_units) * S::kStageBytes;
+    const size_t items = static_cast<size_t>(p.units_rank) * std::min<size_t>(p.a.batch, S::kTokens) * S::kGroups * 4u;
+    size_t each = std::max<size_t>(1, std::min<size_t>(tiles, (16u << 20) / tile_bytes));
+    bool ahead = items > 2u * kThreads;
+    if (ahead && (!ctx->scratch[5] || ctx->scratch[5]->bytes < each * tile_bytes) && ctx->capturing()) ahead = false;
+    if (!ahead) each = tiles;
+    const Q4Args all = p.a;
+    for (size_t t0 = 0; t0 < tiles; t0 += each) {
+        const size_t n = std::min(each, tiles - t0), tok = t0 * S::kTokens;
+        p.a.x = static_cast<const T*>(all.x) + tok * all.x_token;
+        p.a.y = all.y + tok * all.y_token;
+        p.a.batch = std::min(all.batch - tok, n * S::kTokens);
+        if (ahead) {
+            p.planes = static_cast<uint8_t*>(ctx->scratch_get(5, each * tile_bytes));
+            constexpr uint32_t kUnits = 2;
+            LaunchScope ls(ctx, KC_Q4);
+            launch_op(ctx, q4_stage_kernel<T, FMT, NT>, dim3((p.w.n_units + kUnits - 1u) / kUnits, static_cast<unsigned>(n)), kThreads, 0, 1, p, kUnits);
+            ls.done("q4_stage_kernel");
+        }
+        LaunchScope ls(ctx, KC_Q4);
+        launch_op(ctx, kern, dim3(clusters * ranks, static_cast<unsigned>(n)), kThreads, smem, ranks, p);
+        ls.done("q4_matmul_kernel");
+    }
 }
 
 template <typename T, int FMT>
 void launch_tokens(csdr_context* ctx, const Q4Params& p) {
     const size_t m = p.a.batch * (std::is_same<T, float>::value ? 2u : 1u);
-    if (m <= 8) launch<T, FMT, 1>(ctx, p);
+    if (p.a.batch == 1) launch<T, FMT, 1, true>(ctx, p);
+    else if (m <= 8) launch<T, FMT, 1>(ctx, p);
     else if (m <= 16) launch<T, FMT, 2>(ctx, p);
     else launch<T, FMT, 4>(ctx, p);
 }
@@ -448,13 +537,11 @@ void launch_q4_matmul(csdr_context* ctx, const Q4View& w, const Q4Args& a) {
         p.a.batch = std::min(kMost, a.batch - t0);
         p.a.x = static_cast<const uint8_t*>(a.x) + t0 * a.x_token * (a.x_dtype == CSDR_DTYPE_F32 ? 4u : 2u);
         p.a.y = a.y + t0 * a.y_token;
-        LaunchScope ls(ctx, KC_Q4);
         with_dtype(a.x_dtype, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
             if (w.format == 0) launch_tokens<T, 0>(ctx, p);
             else launch_tokens<T, 1>(ctx, p);
         });
-        ls.done("q4_matmul_kernel");
     }
 }
 
