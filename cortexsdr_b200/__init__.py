@@ -851,7 +851,8 @@ class Decoder:
     def __init__(self, loader: SDRModelLoader, *, n_layers, hidden, q_heads, kv_heads, head_dim,
                  inter, vocab, max_seq, max_batch=1, rms_eps=1e-5, rope_theta=1e6, comm: "NcclComm | None" = None,
                  all_gather=None, kv_dtype="f32"):
-        """kv_dtype: "f32" (the reference's arithmetic), "f16" or "bf16" (cache rows rounded to 16 bits, sums fp32).
+        """kv_dtype: "f32" (the reference's arithmetic), "f16" or "bf16" (cache rows rounded to 16 bits, sums fp32), "q4"
+        (cache rows in 4 bits, KVCache; head_dim 64, 128 or 256).
         all_gather: a callable bytes -> list[bytes] (one entry per rank, rank order) supplied by
         the host program, e.g. built on torch.distributed.all_gather_object. When given with a
         communicator of 2 to 8 ranks, the ranks exchange CUDA IPC handles through it and sum their
@@ -860,7 +861,7 @@ class Decoder:
         self.cfg = DecoderConfig(n_layers, hidden, q_heads, kv_heads, head_dim, inter, vocab,
                                  max_seq, max_batch, rms_eps, rope_theta, comm.rank if comm else 0,
                                  comm.world if comm else 1, comm._h if comm else None,
-                                 {"f32": 0, "bf16": 1, "f16": 2}[kv_dtype])
+                                 {"f32": 0, "bf16": 1, "f16": 2, "q4": _lib.KV_Q4}[kv_dtype])
         h = C.c_void_p()
         _check(self.ctx._lib.csdr_decoder_create(loader._h, C.byref(self.cfg), C.byref(h)))
         self._h = h
@@ -897,6 +898,20 @@ class Decoder:
             self._h, seq, t.ctypes.data_as(C.POINTER(C.c_int32)), t.size,
             _fp(logits) if want_logits else None, _fp(hidden) if want_hidden else None))
         return logits, hidden
+
+    def score(self, tokens, seq: int = 0, targets=None, top: int = 0):
+        """Run the tokens as forward() does and score each position: (log probabilities of `targets`, or of the next tokens (the
+        last: NaN), entropies, ids and log probabilities of the `top` alternatives)."""
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        want = None if targets is None else np.ascontiguousarray(targets, dtype=np.int32)
+        if want is not None and want.size != t.size:
+            raise ValueError("one target per token")
+        lp, ent = np.empty(t.size, np.float32), np.empty(t.size, np.float32)
+        ids, alt = np.empty((t.size, top), np.int32), np.empty((t.size, top), np.float32)
+        _check(self.ctx._lib.csdr_decoder_score(
+            self._h, seq, t.ctypes.data_as(C.POINTER(C.c_int32)), t.size, want.ctypes.data if want is not None else None,
+            _fp(lp), _fp(ent), top, ids.ctypes.data if top else None, alt.ctypes.data if top else None))
+        return lp, ent, ids, alt
 
     def step(self, tokens, want_logits=False):
         t = np.ascontiguousarray(tokens, dtype=np.int32)

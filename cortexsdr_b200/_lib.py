@@ -26,6 +26,7 @@ ERR_CODE_RANGE = -11
 ERR_LIMIT = -12
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+KV_Q4 = 16
 FEATURE_MAJOR, TOKEN_MAJOR = 0, 1
 
 
@@ -151,6 +152,7 @@ SIGNATURES = {
     "csdr_decoder_exchange_import": (C.c_int, [_P, _P, _SZ]),
     "csdr_decoder_seek": (C.c_int, [_P, C.c_uint32, C.c_uint32]),
     "csdr_decoder_forward": (C.c_int, [_P, C.c_uint32, C.POINTER(C.c_int32), _SZ, _F, _F]),
+    "csdr_decoder_score": (C.c_int, [_P, C.c_uint32, C.POINTER(C.c_int32), _SZ, _P, _F, _F, C.c_uint32, _P, _P]),
     "csdr_decoder_step": (C.c_int, [_P, C.POINTER(C.c_int32), _SZ, C.POINTER(C.c_int32), _F]),
     "csdr_decoder_step_device_async": (C.c_int, [_P, _P, _SZ, _P]),
     "csdr_kv_cache_create": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float,

@@ -20,6 +20,9 @@
 #include "kernels/gemm_tcgen05.hpp"
 #include "kernels/gemv_fused.hpp"
 #include "kernels/gemv_queue.hpp"
+#include "kernels/kv_cache.hpp"
+#include "kernels/logprobs.hpp"
+#include "kernels/q4_matmul.hpp"
 
 using namespace csdr;
 
@@ -67,13 +70,22 @@ void rethrow_last(int rc) {
     if (rc != CSDR_OK) throw Error(rc, csdr_last_error());
 }
 
-// One linear layer of the model: an HSDR image (whole or this rank's row shard) or a
-// stored-raw fp32 matrix.
+struct Q4Free {
+    void operator()(csdr_q4_weight* w) const { csdr_q4_destroy(w); }
+};
+struct KvFree {
+    void operator()(csdr_kv_cache* c) const { csdr_kv_cache_destroy(c); }
+};
+
+// One linear layer of the model: an HSDR image (whole or this rank's row shard), a stored-raw matrix
+// widened to fp32, or one in 4-bit blocks that stays packed.
 struct Linear {
     const csdr_segment* seg = nullptr;  // owned by the archive
     csdr_segment* shard = nullptr;      // owned here
     DevPtr raw;                         // fp32 (rows_local x cols), rows already sliced
+    std::shared_ptr<csdr_q4_weight> q4; // 4-bit blocks
     uint32_t rows = 0, cols = 0, rows_local = 0, cols_local = 0;
+    bool stored_raw() const { return raw || q4; }
     const csdr_segment* use() const { return shard ? shard : seg; }
 };
 
@@ -99,6 +111,13 @@ struct csdr_decoder {
     size_t cache_layer_stride = 0;   // elements
     int kv_dtype = CSDR_DTYPE_F32;   // fp32 as the reference computes, or fp16 / bf16 (half the cache traffic; sums stay fp32)
     size_t kv_es = 4;
+    // CSDR_KV_Q4: the paged 4-bit cache in place of the two above, each sequence with pages of its own, and the batch
+    // that the pass being run is for it
+    std::unique_ptr<csdr_kv_cache, KvFree> kv4;
+    DevPtr kv_first, kv_length, kv_pages;
+    csdr_kv_batch kv_batch{};
+    uint32_t kv_pages_per_seq = 0;
+    DevPtr score_logits;             // rows of logits that csdr_decoder_score takes at a time
     std::vector<int32_t> pos_host;
     // token selection of the reference's generation loop (off: plain argmax): temperature and a
     // bitmap of the tokens each sequence has produced, [max_batch][seen_words]
@@ -177,8 +196,10 @@ DevPtr load_vector(csdr_decoder* d, const std::string& name, uint32_t n) {
 // dictionary (col_shard: the output and down projections - their input is the rank's slice of
 // the heads / intermediate width; every rank projects its slice, the partial projections are
 // summed over the ranks, and every rank gathers all rows into its copy of the hidden state).
+// A stored-raw tensor in q4_0 or q4_k blocks stays packed where it is only multiplied by (`packed`) and its rows
+// start on whole blocks.
 Linear load_linear(csdr_decoder* d, const std::string& name, uint32_t rows, uint32_t cols, bool row_shard,
-                   bool col_shard) {
+                   bool col_shard, bool packed = true) {
     csdr_segment_header h{};
     int rc = csdr_archive_find(d->ar, name.c_str(), &h);
     if (rc == CSDR_ERR_NOT_FOUND) throw Error(CSDR_ERR_NOT_FOUND, "decoder: tensor not in archive: " + name);
@@ -235,9 +256,17 @@ Linear load_linear(csdr_decoder* d, const std::string& name, uint32_t rows, uint
             rethrow_last(csdr_archive_load_segment(d->ar, name.c_str(), bytes.data(), bytes.size(), &nbytes));
             if (dequant_output_count(id, nbytes) < want)
                 throw Error(CSDR_ERR_GEOMETRY, "tensor '" + name + "' is smaller than the decoder config needs");
-            DevPtr packed = upload(d->ctx, bytes.data(), nbytes);
+            const bool q4_0 = fmt == "q4_0", q4_k = fmt == "q4_k";
+            if (packed && ((q4_0 && cols % 32u == 0) || (q4_k && cols % 256u == 0))) {
+                csdr_q4_weight* w = nullptr;
+                const size_t whole = static_cast<size_t>(rows) * cols / (q4_0 ? 32u : 256u) * (q4_0 ? 18u : 144u);
+                rethrow_last(csdr_q4_create(d->ctx, fmt.c_str(), bytes.data(), whole, rows, cols, &w));
+                l.q4.reset(w, Q4Free{});
+                return l;
+            }
+            DevPtr source = upload(d->ctx, bytes.data(), nbytes);
             l.raw = dev_alloc(d->ctx, dequant_output_count(id, nbytes) * 4);
-            launch_dequantize_inference(d->ctx, id, static_cast<const uint8_t*>(packed->ptr), nbytes,
+            launch_dequantize_inference(d->ctx, id, static_cast<const uint8_t*>(source->ptr), nbytes,
                                         dequant_output_count(id, nbytes), F(l.raw));
         }
         CSDR_CUDA(cudaStreamSynchronize(d->ctx->stream));
@@ -249,7 +278,10 @@ Linear load_linear(csdr_decoder* d, const std::string& name, uint32_t rows, uint
 
 // y (T x rows_local) = x (T x cols) * W^T, token-major both sides.
 void linear(csdr_decoder* d, const Linear& l, const float* x, uint32_t T, float* y) {
-    if (l.raw) {
+    if (l.q4) {
+        rethrow_last(csdr_q4_matmul_device_async(d->ctx, l.q4.get(), x, CSDR_DTYPE_F32, CSDR_LAYOUT_TOKEN_MAJOR, T, y,
+                                                 CSDR_LAYOUT_TOKEN_MAJOR, nullptr));
+    } else if (l.raw) {
         MatmulArgs a;
         a.x = x;
         a.x_layout = CSDR_LAYOUT_TOKEN_MAJOR;
@@ -267,7 +299,7 @@ void linear(csdr_decoder* d, const Linear& l, const float* x, uint32_t T, float*
 void linear_group(csdr_decoder* d, std::initializer_list<const Linear*> ls, const float* x, uint32_t T,
                   std::initializer_list<float*> ys) {
     bool all_hsdr = true;
-    for (const Linear* l : ls) all_hsdr = all_hsdr && !l->raw;
+    for (const Linear* l : ls) all_hsdr = all_hsdr && !l->stored_raw();
     if (!all_hsdr) {
         auto y = ys.begin();
         for (const Linear* l : ls) linear(d, *l, x, T, *y++);
@@ -305,6 +337,14 @@ void sum_over_ranks(csdr_decoder* d, float* from, size_t floats) {
 void attend(csdr_decoder* d, uint32_t li, uint32_t T, float* out, __nv_bfloat16* hi = nullptr, __nv_bfloat16* lo = nullptr) {
     const csdr_decoder_config& c = d->cfg;
     csdr_context* ctx = d->ctx;
+    if (d->kv4) {
+        float* to = out ? out : F(d->att);
+        rethrow_last(csdr_kv_cache_append_device_async(d->kv4.get(), li, &d->kv_batch, F(d->k), F(d->v), 0, CSDR_DTYPE_F32, 1, F(d->q), 0,
+                                                       d->QH_l, F(d->q), 0));
+        rethrow_last(csdr_kv_cache_attention_device_async(d->kv4.get(), li, &d->kv_batch, F(d->q), 0, CSDR_DTYPE_F32, d->QH_l, 0.0f, to, 0));
+        if (hi) op_planes(ctx, to, static_cast<size_t>(T) * d->QD_l, hi, lo);
+        return;
+    }
     void* kc = static_cast<char*>(d->kcache->ptr) + li * d->cache_layer_stride * d->kv_es;
     void* vc = static_cast<char*>(d->vcache->ptr) + li * d->cache_layer_stride * d->kv_es;
     if (d->distinct_seqs && ctx->attention_rope_fold && attention_step_supported(c.head_dim)) {
@@ -617,6 +657,42 @@ void copy_out(csdr_context* ctx, void* dst, const void* src, size_t bytes) {
     else CSDR_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToHost, ctx->stream));
 }
 
+// The blocks over n_tokens new positions of a sequence, up to the final normalisation; the sequence's position moves on with
+// advance().
+uint32_t run_tokens(csdr_decoder* d, uint32_t seq, const int32_t* tokens, size_t n_tokens) {
+    const csdr_decoder_config& c = d->cfg;
+    if (!tokens || n_tokens == 0) throw Error(CSDR_ERR_INVALID_ARG, "no tokens");
+    if (seq >= c.max_batch) throw Error(CSDR_ERR_INVALID_ARG, "sequence index out of range");
+    const int32_t p0 = d->pos_host[seq];
+    if (n_tokens > d->T_max || p0 + n_tokens > c.max_seq)
+        throw Error(CSDR_ERR_LIMIT, "sequence would exceed the KV-cache capacity (max_seq)");
+    for (size_t i = 0; i < n_tokens; ++i)
+        if (tokens[i] < 0 || static_cast<uint32_t>(tokens[i]) >= c.vocab)
+            throw Error(CSDR_ERR_INVALID_ARG, "token id outside the vocabulary");
+    csdr_context* ctx = d->ctx;
+    const uint32_t T = static_cast<uint32_t>(n_tokens);
+    std::vector<int32_t> so(T, static_cast<int32_t>(seq)), po(T);
+    for (uint32_t t = 0; t < T; ++t) po[t] = p0 + static_cast<int32_t>(t);
+    CSDR_CUDA(cudaMemcpyAsync(d->tokens_dev->ptr, tokens, T * 4, cudaMemcpyHostToDevice, ctx->stream));
+    CSDR_CUDA(cudaMemcpyAsync(d->seq_of->ptr, so.data(), T * 4, cudaMemcpyHostToDevice, ctx->stream));
+    CSDR_CUDA(cudaMemcpyAsync(d->pos_of->ptr, po.data(), T * 4, cudaMemcpyHostToDevice, ctx->stream));
+    if (d->kv4) {
+        const int32_t first[2] = {0, static_cast<int32_t>(T)}, length = p0 + static_cast<int32_t>(T);
+        CSDR_CUDA(cudaMemcpyAsync(d->kv_first->ptr, first, 8, cudaMemcpyHostToDevice, ctx->stream));
+        CSDR_CUDA(cudaMemcpyAsync(d->kv_length->ptr, &length, 4, cudaMemcpyHostToDevice, ctx->stream));
+        d->kv_batch = {1, T, d->kv_pages_per_seq, I32(d->kv_first), I32(d->kv_length),
+                       I32(d->kv_pages) + static_cast<size_t>(seq) * d->kv_pages_per_seq};
+    }
+    embed(d, T);
+    d->distinct_seqs = T == 1u;
+    run_blocks(d, T);
+    return T;
+}
+void advance(csdr_decoder* d, uint32_t seq, uint32_t T) {
+    d->pos_host[seq] += static_cast<int32_t>(T);
+    CSDR_CUDA(cudaMemcpyAsync(I32(d->pos_dev) + seq, &d->pos_host[seq], 4, cudaMemcpyHostToDevice, d->ctx->stream));
+}
+
 void need(csdr_decoder* d) {
     if (!d) throw Error(CSDR_ERR_INVALID_ARG, "decoder is null");
     require_ctx(d->ctx);
@@ -689,7 +765,7 @@ int csdr_decoder_create(csdr_archive* ar, const csdr_decoder_config* cfg, csdr_d
         d->I_l = c.inter / d->P;
         d->H_l = H;   // the residual stream is replicated on every rank
         d->V_l = c.vocab / d->P;
-        d->emb = load_linear(d.get(), "token_embd.weight", c.vocab, H, false, false);
+        d->emb = load_linear(d.get(), "token_embd.weight", c.vocab, H, false, false, false);
         {
             csdr_segment_header h{};
             const char* head = csdr_archive_find(ar, "output.weight", &h) == CSDR_OK ? "output.weight"
@@ -716,8 +792,24 @@ int csdr_decoder_create(csdr_archive* ar, const csdr_decoder_config* cfg, csdr_d
         d->T_max = std::max(c.max_seq, c.max_batch);
         const size_t T = d->T_max;
         d->cache_layer_stride = static_cast<size_t>(c.max_batch) * c.max_seq * d->KVD_l;
-        if (c.kv_dtype != CSDR_DTYPE_F32 && c.kv_dtype != CSDR_DTYPE_BF16 && c.kv_dtype != CSDR_DTYPE_F16)
-            throw Error(CSDR_ERR_INVALID_ARG, "decoder: kv_dtype must be CSDR_DTYPE_F32, CSDR_DTYPE_F16 or CSDR_DTYPE_BF16");
+        if (c.kv_dtype == CSDR_KV_Q4) {
+            if (d->P > 1) throw Error(CSDR_ERR_UNSUPPORTED, "decoder: the 4-bit KV cache is for a single GPU");
+            constexpr uint32_t kPage = 64;
+            d->kv_pages_per_seq = (c.max_seq + kPage - 1) / kPage;
+            const uint64_t pages = static_cast<uint64_t>(c.max_batch) * d->kv_pages_per_seq;
+            if (pages > 0x7FFFFFFFu) throw Error(CSDR_ERR_LIMIT, "decoder: KV cache too large");
+            csdr_kv_cache* cache = nullptr;
+            rethrow_last(csdr_kv_cache_create(ctx, c.n_layers, static_cast<uint32_t>(pages), kPage, d->KVH_l, HD, c.rope_theta, &cache));
+            d->kv4.reset(cache);
+            std::vector<int32_t> table(pages);
+            for (size_t i = 0; i < table.size(); ++i) table[i] = static_cast<int32_t>(i);
+            d->kv_pages = upload(ctx, table.data(), table.size() * 4u);
+            d->kv_first = dev_alloc(ctx, (static_cast<size_t>(c.max_batch) + 1) * 4);
+            d->kv_length = dev_alloc(ctx, static_cast<size_t>(c.max_batch) * 4);
+            CSDR_CUDA(cudaStreamSynchronize(ctx->stream));
+            d->cache_layer_stride = 0;
+        } else if (c.kv_dtype != CSDR_DTYPE_F32 && c.kv_dtype != CSDR_DTYPE_BF16 && c.kv_dtype != CSDR_DTYPE_F16)
+            throw Error(CSDR_ERR_INVALID_ARG, "decoder: kv_dtype must be CSDR_DTYPE_F32, CSDR_DTYPE_F16, CSDR_DTYPE_BF16 or CSDR_KV_Q4");
         d->kv_dtype = static_cast<int>(c.kv_dtype);
         d->kv_es = d->kv_dtype == CSDR_DTYPE_F32 ? 4 : 2;
         d->kcache = dev_alloc(ctx, d->cache_layer_stride * c.n_layers * d->kv_es);
@@ -741,13 +833,13 @@ int csdr_decoder_create(csdr_archive* ar, const csdr_decoder_config* cfg, csdr_d
         {
             // the planes path needs every block linear (and the head) to be an HSDR image the
             // grouped tensor-core path takes
-            bool ok = !d->lm_head.raw;
+            bool ok = !d->lm_head.stored_raw();
             uint32_t widest = 0;   // atoms of the largest group
             auto atoms = [](const Linear& l) { return l.use() ? l.use()->g.n_atoms : 0u; };
             for (const Layer& L : d->layers) {
                 const Linear* all[7] = {&L.q, &L.k, &L.v, &L.o, &L.gate, &L.up, &L.down};
                 for (const Linear* l : all) {
-                    if (l->raw || !l->use()) {
+                    if (l->stored_raw() || !l->use()) {
                         ok = false;
                         continue;
                     }
@@ -768,7 +860,7 @@ int csdr_decoder_create(csdr_archive* ar, const csdr_decoder_config* cfg, csdr_d
                 for (const Layer& L : d->layers) {
                     const Linear* all[7] = {&L.q, &L.k, &L.v, &L.o, &L.gate, &L.up, &L.down};
                     for (const Linear* l : all) {
-                        if (l->raw || !l->use()) {
+                        if (l->stored_raw() || !l->use()) {
                             q_ok = false;
                             continue;
                         }
@@ -776,7 +868,7 @@ int csdr_decoder_create(csdr_archive* ar, const csdr_decoder_config* cfg, csdr_d
                                               CSDR_LAYOUT_TOKEN_MAJOR, nullptr};
                         q_ok = q_ok && gemv_queue_supported(ctx, &probe, 1);
                     }
-                    q_ok = q_ok && !L.gate.raw && !L.up.raw && L.gate.rows_local == L.up.rows_local;
+                    q_ok = q_ok && !L.gate.stored_raw() && !L.up.stored_raw() && L.gate.rows_local == L.up.rows_local;
                 }
                 d->queue_capable = q_ok;
             }
@@ -786,7 +878,7 @@ int csdr_decoder_create(csdr_archive* ar, const csdr_decoder_config* cfg, csdr_d
                     bool f_ok = true;
                     for (const Layer& L : d->layers) {
                         const Linear* all[7] = {&L.q, &L.k, &L.v, &L.o, &L.gate, &L.up, &L.down};
-                        for (const Linear* l : all) f_ok = f_ok && !l->raw && l->use();
+                        for (const Linear* l : all) f_ok = f_ok && !l->stored_raw() && l->use();
                         if (!f_ok) break;
                         FusedGlue norm, mlp, none;
                         norm.norm_w = mlp.norm_w = F(L.attn_norm);
@@ -955,25 +1047,9 @@ int csdr_decoder_forward(csdr_decoder* d, uint32_t seq, const int32_t* tokens, s
                          float* logits_out, float* hidden_out) {
     return guard([&] {
         need(d);
+        const uint32_t T = run_tokens(d, seq, tokens, n_tokens);
         const csdr_decoder_config& c = d->cfg;
-        if (!tokens || n_tokens == 0) throw Error(CSDR_ERR_INVALID_ARG, "no tokens");
-        if (seq >= c.max_batch) throw Error(CSDR_ERR_INVALID_ARG, "sequence index out of range");
-        const int32_t p0 = d->pos_host[seq];
-        if (n_tokens > d->T_max || p0 + n_tokens > c.max_seq)
-            throw Error(CSDR_ERR_LIMIT, "sequence would exceed the KV-cache capacity (max_seq)");
-        for (size_t i = 0; i < n_tokens; ++i)
-            if (tokens[i] < 0 || static_cast<uint32_t>(tokens[i]) >= c.vocab)
-                throw Error(CSDR_ERR_INVALID_ARG, "token id outside the vocabulary");
         csdr_context* ctx = d->ctx;
-        const uint32_t T = static_cast<uint32_t>(n_tokens);
-        std::vector<int32_t> so(T, static_cast<int32_t>(seq)), po(T);
-        for (uint32_t t = 0; t < T; ++t) po[t] = p0 + static_cast<int32_t>(t);
-        CSDR_CUDA(cudaMemcpyAsync(d->tokens_dev->ptr, tokens, T * 4, cudaMemcpyHostToDevice, ctx->stream));
-        CSDR_CUDA(cudaMemcpyAsync(d->seq_of->ptr, so.data(), T * 4, cudaMemcpyHostToDevice, ctx->stream));
-        CSDR_CUDA(cudaMemcpyAsync(d->pos_of->ptr, po.data(), T * 4, cudaMemcpyHostToDevice, ctx->stream));
-        embed(d, T);
-        d->distinct_seqs = T == 1u;
-        run_blocks(d, T);
         if (hidden_out) {
             materialise_normed(d, T);
         }
@@ -983,8 +1059,61 @@ int csdr_decoder_forward(csdr_decoder* d, uint32_t seq, const int32_t* tokens, s
                                       cudaMemcpyDeviceToHost, ctx->stream));
         }
         if (hidden_out) copy_out(ctx, hidden_out, d->normed->ptr, static_cast<size_t>(T) * c.hidden * 4);
-        d->pos_host[seq] = p0 + static_cast<int32_t>(T);
-        CSDR_CUDA(cudaMemcpyAsync(I32(d->pos_dev) + seq, &d->pos_host[seq], 4, cudaMemcpyHostToDevice, ctx->stream));
+        advance(d, seq, T);
+        CSDR_CUDA(cudaStreamSynchronize(ctx->stream));
+    });
+}
+
+int csdr_decoder_score(csdr_decoder* d, uint32_t seq, const int32_t* tokens, size_t n_tokens, const int32_t* targets, float* logprobs,
+                       float* entropy, uint32_t top, int32_t* top_ids, float* top_logprobs) {
+    return guard([&] {
+        need(d);
+        const csdr_decoder_config& c = d->cfg;
+        if (d->P > 1) throw Error(CSDR_ERR_UNSUPPORTED, "decoder: scoring is for a single GPU");
+        if (top > kMaxTop) throw Error(CSDR_ERR_LIMIT, "at most 32 alternatives");
+        if (top > c.vocab) throw Error(CSDR_ERR_INVALID_ARG, "more alternatives than the vocabulary has tokens");
+        if (!logprobs || (top && (!top_ids || !top_logprobs))) throw Error(CSDR_ERR_INVALID_ARG, "null argument");
+        const uint32_t T = run_tokens(d, seq, tokens, n_tokens);
+        csdr_context* ctx = d->ctx;
+        // as many rows of logits at a time as 64 MB hold, 64 at most
+        const uint32_t rows = static_cast<uint32_t>(std::min<size_t>(64, std::max<size_t>(1, (64u << 20) / (static_cast<size_t>(c.vocab) * 4))));
+        if (!d->score_logits) d->score_logits = dev_alloc(ctx, static_cast<size_t>(rows) * c.vocab * 4);
+        std::vector<int32_t> next(T, -1);
+        for (uint32_t t = 0; t < T; ++t) next[t] = targets ? targets[t] : t + 1 < T ? tokens[t + 1] : -1;
+        const size_t k = top;
+        DevPtr want = upload(ctx, next.data(), static_cast<size_t>(T) * 4), out = dev_alloc(ctx, static_cast<size_t>(T) * (2 + 2 * k) * 4);
+        float* lp = F(out);
+        float* ent = lp + T;
+        int32_t* ids = reinterpret_cast<int32_t*>(ent + T);
+        float* alt = reinterpret_cast<float*>(ids + T * k);
+        struct Swap {      // the logits of a step stay where captured steps left them
+            csdr_decoder* d;
+            explicit Swap(csdr_decoder* x) : d(x) { std::swap(d->logits, d->score_logits); }
+            ~Swap() { std::swap(d->logits, d->score_logits); }
+        } swapped(d);
+        for (uint32_t t0 = 0; t0 < T; t0 += rows) {
+            const uint32_t n = std::min(rows, T - t0);
+            run_logits(d, T, t0, n);
+            LogprobArgs a{};
+            a.logits = d->logits->ptr;
+            a.stride = c.vocab;
+            a.rows = n;
+            a.vocab = c.vocab;
+            a.targets = I32(want) + t0;
+            a.logprob = lp + t0;
+            a.entropy = ent + t0;
+            a.top = top;
+            a.top_ids = ids + t0 * k;
+            a.top_logprobs = alt + t0 * k;
+            launch_logprobs(ctx, CSDR_DTYPE_F32, a);
+        }
+        advance(d, seq, T);
+        copy_out(ctx, logprobs, lp, static_cast<size_t>(T) * 4);
+        if (entropy) copy_out(ctx, entropy, ent, static_cast<size_t>(T) * 4);
+        if (top) {
+            copy_out(ctx, top_ids, ids, T * k * 4);
+            copy_out(ctx, top_logprobs, alt, T * k * 4);
+        }
         CSDR_CUDA(cudaStreamSynchronize(ctx->stream));
     });
 }
@@ -1003,6 +1132,10 @@ int csdr_decoder_step_device_async(csdr_decoder* d, const int32_t* tokens_dev, s
         if (tokens_dev != I32(d->tokens_dev))
             CSDR_CUDA(cudaMemcpyAsync(d->tokens_dev->ptr, tokens_dev, B * 4, cudaMemcpyDeviceToDevice, ctx->stream));
         op_step_positions(ctx, I32(d->pos_dev), B, I32(d->seq_of), I32(d->pos_of));
+        if (d->kv4) {
+            op_step_lengths(ctx, I32(d->pos_of), B, I32(d->kv_first), I32(d->kv_length));
+            d->kv_batch = {B, B, d->kv_pages_per_seq, I32(d->kv_first), I32(d->kv_length), I32(d->kv_pages)};
+        }
         embed(d, B);
         d->distinct_seqs = true;
         run_blocks(d, B);

@@ -728,6 +728,20 @@ __global__ void mark_seen_kernel(uint32_t* __restrict__ seen_row, const int32_t*
     }
 }
 
+__global__ void step_lengths_kernel(const int32_t* __restrict__ pos_of, uint32_t B, int32_t* __restrict__ first, int32_t* __restrict__ length) {
+    pdl_enter();
+    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i <= B) first[i] = static_cast<int32_t>(i);
+    if (i < B) length[i] = pos_of[i] + 1;
+}
+
+__global__ void __launch_bounds__(256)
+planes_kernel(const float* __restrict__ x, size_t n, __nv_bfloat16* __restrict__ hi, __nv_bfloat16* __restrict__ lo) {
+    pdl_enter();
+    const size_t stride = static_cast<size_t>(gridDim.x) * 256u;
+    for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += stride) store_planes(hi, lo, i, x[i]);
+}
+
 // positions: pos_of[t] = pos[b] for a batched step, then pos[b] += 1 (all on the device, so a
 // captured step replays without host involvement).
 __global__ void step_positions_kernel(int32_t* __restrict__ pos, uint32_t B, int32_t* __restrict__ seq_of,
@@ -936,6 +950,18 @@ void op_step_positions(csdr_context* ctx, int32_t* pos, uint32_t B, int32_t* seq
     LaunchScope ls(ctx, KC_DECODER_OP);
     step_positions_kernel<<<(B + 127) / 128, 128, 0, ctx->stream>>>(pos, B, seq_of, pos_of);
     ls.done("step_positions_kernel");
+}
+
+void op_step_lengths(csdr_context* ctx, const int32_t* pos_of, uint32_t B, int32_t* first, int32_t* length) {
+    LaunchScope ls(ctx, KC_DECODER_OP);
+    launch_pdl(ctx, step_lengths_kernel, dim3((B + 128) / 128), dim3(128), pos_of, B, first, length);
+    ls.done("step_lengths_kernel");
+}
+
+void op_planes(csdr_context* ctx, const float* x, size_t n, __nv_bfloat16* hi, __nv_bfloat16* lo) {
+    LaunchScope ls(ctx, KC_DECODER_OP);
+    launch_pdl(ctx, planes_kernel, dim3(grid_for(n, ctx)), dim3(256), x, n, hi, lo);
+    ls.done("planes_kernel");
 }
 
 }  // namespace csdr

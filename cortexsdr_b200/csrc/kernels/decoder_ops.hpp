@@ -64,5 +64,8 @@ void op_select(csdr_context* ctx, const float* logits, uint32_t rows, uint32_t V
                uint32_t* seen, uint32_t seen_words);
 void op_mark_seen(csdr_context* ctx, uint32_t* seen_row, const int32_t* tokens_dev, uint32_t n, uint32_t V);
 void op_step_positions(csdr_context* ctx, int32_t* pos, uint32_t B, int32_t* seq_of, int32_t* pos_of);
+// A decode step as a batch of the paged cache: sequence i has row i, its token at pos_of[i] the last.
+void op_step_lengths(csdr_context* ctx, const int32_t* pos_of, uint32_t B, int32_t* first, int32_t* length);
+void op_planes(csdr_context* ctx, const float* x, size_t n, __nv_bfloat16* hi, __nv_bfloat16* lo);
 
 }  // namespace csdr

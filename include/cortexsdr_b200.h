@@ -55,6 +55,7 @@ enum {
 };
 
 enum { CSDR_DTYPE_F32 = 0, CSDR_DTYPE_BF16 = 1,
+       CSDR_KV_Q4 = 16 /* csdr_decoder_config.kv_dtype only */,
        CSDR_DTYPE_F16 = 2 /* KV caches and the operators that say so; elsewhere activations are fp32 or bf16 */ };
 enum { CSDR_LAYOUT_FEATURE_MAJOR = 0, CSDR_LAYOUT_TOKEN_MAJOR = 1 };
 enum { CSDR_KIND_HSDR = 0, CSDR_KIND_HSDC = 1 };
@@ -441,7 +442,9 @@ typedef struct {
     /* KV cache element type: CSDR_DTYPE_F32 (0, default: the reference's arithmetic),
      * CSDR_DTYPE_F16 or CSDR_DTYPE_BF16 (keys and values rounded to 16 bits when they enter
      * the cache, scores and sums in fp32; half the cache bytes per step; fp16 keeps three more
-     * mantissa bits and wants |k|, |v| < 65504). No counterpart in the reference. */
+     * mantissa bits and wants |k|, |v| < 65504), or CSDR_KV_Q4 (keys and values in 4 bits, see the
+     * paged cache below: 0.28 of the bytes of 16 bits; rotary angles in 64 bits; a single GPU, head_dim
+     * 64, 128 or 256). No counterpart in the reference. */
     uint32_t kv_dtype;
 } csdr_decoder_config;
 
@@ -477,6 +480,13 @@ CSDR_API int csdr_decoder_seek(csdr_decoder* d, uint32_t seq, uint32_t position)
  * position (n_tokens x hidden, host). */
 CSDR_API int csdr_decoder_forward(csdr_decoder* d, uint32_t seq, const int32_t* tokens,
                                   size_t n_tokens, float* logits_out, float* hidden_out);
+/* As csdr_decoder_forward, with a score for every new position instead of the last one's logits: the log
+ * probability of targets[t] after tokens[0 .. t] (targets NULL: of tokens[t + 1]; none for the last, NaN), the
+ * entropy there (may be NULL), and `top` alternatives (at most 32; ids and log probabilities, n_tokens x top,
+ * largest first), as csdr_token_logprobs_device_async has them. Host arrays. A single GPU. */
+CSDR_API int csdr_decoder_score(csdr_decoder* d, uint32_t seq, const int32_t* tokens, size_t n_tokens,
+                                const int32_t* targets, float* logprobs, float* entropy, uint32_t top,
+                                int32_t* top_ids, float* top_logprobs);
 /* One decode step for `batch` sequences at once (sequence b gets tokens[b]); writes the
  * greedy next token of each to next_out (host). logits_out may be NULL, else
  * (batch x vocab) host fp32. */
