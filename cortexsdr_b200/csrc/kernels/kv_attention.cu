@@ -65,7 +65,8 @@ struct Seq {
     // blocks of 128 keys that a tile of rows sees; at least one, so that rows that see nothing are written too
     template <uint32_t TILE>
     __device__ __forceinline__ int64_t keys(uint32_t tile, uint32_t group) const {
-        const uint32_t last = min(n_new - 1u, static_cast<uint32_t>((static_cast<uint64_t>(TILE) * (tile + 1u) - 1u) / group));
+        // TILE (tiles + 1) fits 32 bits (launch_kv_attention)
+        const uint32_t last = tile + 1u == tiles ? n_new - 1u : (TILE * (tile + 1u) - 1u) / group;
         return min(max(base + last + 1, static_cast<int64_t>(0)), cap);
     }
     template <uint32_t TILE>
@@ -85,13 +86,29 @@ struct Seq {
         n_new = static_cast<uint32_t>(r1 - r0);
         base = static_cast<int64_t>(p.b.length[s]) - f1 + r0;
         cap = min(static_cast<int64_t>(p.b.pages_per_seq) << p.kv.page_shift, static_cast<int64_t>(0x7FFFFF00));
-        tiles = static_cast<uint32_t>((static_cast<uint64_t>(n_new) * p.group + TILE - 1u) / TILE);
+        tiles = (n_new * p.group + TILE - 1u) / TILE;
         pair_weight = mid_weight = 0;
         if (!tiles) return;
+        if (tiles == 1u) {
+            mid_weight = blocks<TILE>(0, p.group);
+            return;
+        }
         const uint32_t a = blocks<TILE>(0, p.group), z = blocks<TILE>(tiles - 1u, p.group);
         // rounding to blocks and the last tile's missing rows: two blocks at most
         pair_weight = tiles == 2u ? a + z : base + n_new > cap ? 2u * z : a + z + 2u;
         if (tiles & 1u) mid_weight = blocks<TILE>(tiles / 2u, p.group);
+    }
+    // As lane `from` of the warp has it.
+    __device__ __forceinline__ Seq of_lane(uint32_t from) const {
+        Seq q;
+        q.base = __shfl_sync(0xFFFFFFFFu, base, from);
+        q.cap = __shfl_sync(0xFFFFFFFFu, cap, from);
+        q.row0 = __shfl_sync(0xFFFFFFFFu, row0, from);
+        q.n_new = __shfl_sync(0xFFFFFFFFu, n_new, from);
+        q.tiles = __shfl_sync(0xFFFFFFFFu, tiles, from);
+        q.pair_weight = __shfl_sync(0xFFFFFFFFu, pair_weight, from);
+        q.mid_weight = __shfl_sync(0xFFFFFFFFu, mid_weight, from);
+        return q;
     }
     __device__ __forceinline__ uint64_t head_weight() const { return static_cast<uint64_t>(tiles / 2u) * pair_weight + mid_weight; }
 };
@@ -592,64 +609,94 @@ kv_attention_kernel(AttnParams p) {
     op_enter();
     asm volatile("fence.proxy.async;" ::: "memory");
 
-    // ---- this CTA's share of the work ----
-    const uint32_t per = (p.b.n_seqs + kThreads - 1u) / kThreads;
-    const uint32_t s_lo = min(tid * per, p.b.n_seqs), s_hi = min(s_lo + per, p.b.n_seqs);
-    uint64_t mine = 0;
-    uint32_t blocks = 0, units = 0;
-    for (uint32_t s = s_lo; s < s_hi; ++s) {
-        Seq q;
-        q.load<TILE>(p, s);
-        mine += q.head_weight() * p.kv.kv_heads;
-        if (q.tiles) blocks = max(blocks, q.blocks<TILE>(q.tiles - 1u, p.group));
-        units += q.tiles * p.kv.kv_heads;
-    }
-    atomicMax(&longest, blocks);
-    atomicAdd(&n_units, units);
-    uint64_t upto = mine;
+    // ---- this CTA's share of the work: places x0 to x1 - 1 ----
+    uint64_t total, x0 = 0, x1 = 0, ctas = 0;
+    auto share = [&](uint32_t longest_unit, uint32_t units) {
+        // Joining n pieces costs a CTA about a sixteenth of a block's time each: no unit is cut finer than both together take.
+        const uint64_t least_blocks = 1u + static_cast<uint32_t>(sqrtf(static_cast<float>(longest_unit) / 16.0f));
+        ctas = min(static_cast<uint64_t>(gridDim.x), max(quotient(total, least_blocks), static_cast<uint64_t>(1)));
+        // Units that are all as long, one a CTA, where sharing them evenly would save less than the joins cost (two blocks' time;
+        // 16 sequences of 1024 with 32 heads: 39.7 -> 33.9 us)
+        if (units <= gridDim.x && total == static_cast<uint64_t>(units) * longest_unit && longest_unit <= quotient(total, ctas) + 2u) {
+            ctas = units;
+            x0 = static_cast<uint64_t>(blockIdx.x) * longest_unit;
+            x1 = x0 + longest_unit;
+        } else {
+            x0 = quotient(blockIdx.x * total, ctas);
+            x1 = quotient((blockIdx.x + 1u) * total, ctas);
+        }
+    };
+    auto scan_up = [&](uint64_t v) {
 #pragma unroll
-    for (uint32_t o = 1; o < 32u; o <<= 1) {
-        const uint64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-        if (lane >= o) upto += v;
-    }
-    if (lane == 31u) scan[warp] = upto;
-    __syncthreads();
-    uint64_t total = 0, before = 0;
+        for (uint32_t o = 1; o < 32u; o <<= 1) {
+            const uint64_t w = __shfl_up_sync(0xFFFFFFFFu, v, o);
+            if (lane >= o) v += w;
+        }
+        return v;
+    };
+    uint32_t s;
+    uint64_t seq_at;
+    Seq sq;
+    if (p.b.n_seqs <= 32u) {
+        // every warp for itself, a lane a sequence
+        Seq q{};
+        if (lane < p.b.n_seqs) q.load<TILE>(p, lane);
+        const uint64_t w = q.head_weight() * p.kv.kv_heads, upto = scan_up(w);
+        total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        if (!total) return;
+        share(__reduce_max_sync(0xFFFFFFFFu, q.tiles ? q.blocks<TILE>(q.tiles - 1u, p.group) : 0u),
+              __reduce_add_sync(0xFFFFFFFFu, q.tiles * p.kv.kv_heads));
+        if (blockIdx.x >= ctas) return;
+        s = __ffs(__ballot_sync(0xFFFFFFFFu, x0 >= upto - w && x0 < upto)) - 1u;
+        seq_at = __shfl_sync(0xFFFFFFFFu, upto - w, s);
+        sq = q.of_lane(s);
+    } else {
+        const uint32_t per = (p.b.n_seqs + kThreads - 1u) / kThreads;
+        const uint32_t s_lo = min(tid * per, p.b.n_seqs), s_hi = min(s_lo + per, p.b.n_seqs);
+        uint64_t mine = 0;
+        uint32_t blocks = 0, units = 0;
+        for (uint32_t i = s_lo; i < s_hi; ++i) {
+            Seq q;
+            q.load<TILE>(p, i);
+            mine += q.head_weight() * p.kv.kv_heads;
+            if (q.tiles) blocks = max(blocks, q.blocks<TILE>(q.tiles - 1u, p.group));
+            units += q.tiles * p.kv.kv_heads;
+        }
+        atomicMax(&longest, blocks);
+        atomicAdd(&n_units, units);
+        const uint64_t upto = scan_up(mine);
+        if (lane == 31u) scan[warp] = upto;
+        __syncthreads();
+        uint64_t before = 0;
+        total = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kWarps; ++i) {
-        if (i < warp) before += scan[i];
-        total += scan[i];
-    }
-    if (!total) return;
-    // Joining n pieces costs a CTA about a ninth of a block's time each: no unit is cut finer than both together take.
-    const uint64_t least_blocks = 1u + static_cast<uint32_t>(sqrtf(static_cast<float>(longest) / 16.0f));
-    uint64_t ctas = min(static_cast<uint64_t>(gridDim.x), max(quotient(total, least_blocks), static_cast<uint64_t>(1)));
-    // Units that are all as long, one a CTA, where sharing them evenly would save less than the joins cost (two blocks' time;
-    // 16 sequences of 1024 with 32 heads: 39.7 -> 33.9 us)
-    if (n_units <= gridDim.x && total == static_cast<uint64_t>(n_units) * longest && longest <= quotient(total, ctas) + 2u) ctas = n_units;
-    if (blockIdx.x >= ctas) return;
-    const uint64_t x0 = quotient(blockIdx.x * total, ctas), x1 = quotient((blockIdx.x + 1u) * total, ctas);
-    {
+        for (uint32_t i = 0; i < kWarps; ++i) {
+            if (i < warp) before += scan[i];
+            total += scan[i];
+        }
+        if (!total) return;
+        share(longest, n_units);
+        if (blockIdx.x >= ctas) return;
         uint64_t at = before + upto - mine;
         if (x0 >= at && x0 < at + mine) {
-            for (uint32_t s = s_lo; s < s_hi; ++s) {
+            for (uint32_t i = s_lo; i < s_hi; ++i) {
                 Seq q;
-                q.load<TILE>(p, s);
+                q.load<TILE>(p, i);
                 const uint64_t w = q.head_weight() * p.kv.kv_heads;
                 if (x0 < at + w) {
-                    found = s;
+                    found = i;
                     found_at = at;
                     break;
                 }
                 at += w;
             }
         }
+        __syncthreads();
+        s = found;
+        seq_at = found_at;
+        sq.load<TILE>(p, s);
     }
-    __syncthreads();
-    uint32_t s = found;
-    uint64_t seq_at = found_at, x = x0;
-    Seq sq;
-    sq.load<TILE>(p, s);
+    uint64_t x = x0;
     uint32_t turn = 0;       // stages filled so far
     bool live = true;
     Warp rows;
@@ -684,7 +731,11 @@ kv_attention_kernel(AttnParams p) {
         const uint64_t z = y - kvh * hw;
         uint32_t tile, b0;
         uint64_t next = seq_at + kvh * hw;       // where the next unit starts
-        if (z < pairs) {
+        if (sq.tiles == 1u) {
+            tile = 0u;
+            b0 = static_cast<uint32_t>(z);
+            next += hw;
+        } else if (z < pairs) {
             const uint32_t pr = static_cast<uint32_t>(quotient(z, sq.pair_weight)), o = static_cast<uint32_t>(z - static_cast<uint64_t>(pr) * sq.pair_weight);
             const uint32_t n = sq.blocks<TILE>(pr, p.group);
             next += static_cast<uint64_t>(pr) * sq.pair_weight;
@@ -899,7 +950,8 @@ void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim,
     const size_t es = dtype == CSDR_DTYPE_F32 ? 4 : 2;
     p.vec = (reinterpret_cast<uintptr_t>(a.q) | a.q_stride * es) % 16u == 0;
     p.vec_out = (reinterpret_cast<uintptr_t>(a.out) | a.out_stride * es) % 16u == 0;
-    const uint64_t rows = static_cast<uint64_t>(b.n_tokens) * p.group / b.n_seqs;
+    const uint64_t all_rows = static_cast<uint64_t>(b.n_tokens) * p.group, rows = all_rows / b.n_seqs;
+    if (all_rows > 0xFFFFFF00u) throw Error(CSDR_ERR_LIMIT, "attention: more query rows of a kv head than 2^32");
     LaunchScope ls(ctx, KC_KV_ATTENTION);
     with_dtype(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -248,6 +248,25 @@ def test_attention_matches_the_definition(ctx, shape, dtype):
     assert (out[at:] == 7).all()             # rows behind the last sequence
 
 
+@pytest.mark.parametrize("n,most_new,dtype", [(33, 1, "f32"), (150, 1, "bf16"), (300, 1, "f32"), (40, 9, "f16"), (140, 30, "bf16")])
+def test_attention_of_many_sequences(ctx, n, most_new, dtype):
+    rng = np.random.default_rng(n)
+    fresh = [0 if i % 9 == 4 else int(rng.integers(1, most_new + 1)) for i in range(n)]
+    lengths = [f + int(rng.integers(0, 200)) for f in fresh]
+    c = Case(ctx, lengths, fresh, 2, 64, 16, seed=n, dtype=dtype)
+    c.store()
+    qh = 6
+    q = [c.values((f, qh, 64)) for f in fresh]
+    out = c.attend(c.rows(q), qh)
+    k, v = c.held()
+    at = 0
+    for s, f in enumerate(fresh):
+        if f:
+            want = ref.attention(q[s].to(torch.float64).numpy(), k[s], v[s], lengths[s] - f + np.arange(f), 0.125)
+            close(out[at:at + f], want, c.tdtype, max(1.0, np.abs(v[s]).max()))
+        at += f
+
+
 def test_attention_sees_what_has_a_place(ctx):
     # a page that is not there inside a sequence, a length past the table, a length that is less than the new rows
     c = Case(ctx, [100, 64, 2, 0], [1, 1, 5, 3], 2, 64, 16, seed=8)
