@@ -182,83 +182,102 @@ kv_append_kernel(KvView kv, KvBatchView b, KvAppend a, uint32_t tokens) {
     }
     const uint32_t nq = (a.q ? a.q_heads : 0u) * G, nk = kv.kv_heads * G, units = nq + 2u * nk, fours = (units + 3u) / 4u;
     Eight<T> ahead;
-    // a warp's i-th four: token and group of this lane
-    auto fetch = [&](uint32_t i) {
-        const uint32_t j = i / fours, u = i % fours * 4u + (lane >> 3), t = t0 + j;
+    const uint32_t sub = lane >> 3, step = gridDim.y * kWarps;
+    // a warp's place: four f of token j; the next one `step` fours on
+    auto move = [&](uint32_t& j, uint32_t& f) {
+        while (f >= fours && j < n_tok) {
+            f -= fours;
+            ++j;
+        }
+    };
+    auto fetch = [&](uint32_t j, uint32_t f) {
+        const uint32_t u = f * 4u + sub, t = t0 + j;
         if (u >= units || !places.own[j]) return;
         if (u < nq) ahead.load(static_cast<const T*>(a.q) + t * a.q_stride + u * 64u + 8u * l, a.q_vec);
         else if (places.page[j] < 0) return;
         else if (u < nq + nk) ahead.load(static_cast<const T*>(a.k) + t * a.kv_stride + (u - nq) * 64u + 8u * l, a.kv_vec);
         else ahead.load(static_cast<const T*>(a.v) + t * a.kv_stride + (u - nq - nk) * 64u + 8u * l, a.kv_vec);
     };
-    const uint32_t step = gridDim.y * kWarps, n_fours = n_tok * fours;
-    uint32_t i = blockIdx.y * kWarps + warp;
-    if (i < n_fours) fetch(i);
-    for (; i < n_fours; i += step) {
-        const uint32_t j = i / fours, u0 = i % fours * 4u, u = u0 + (lane >> 3), t = t0 + j;
-        const int32_t pos = places.pos[j], page = places.page[j];
-        const uint32_t at = static_cast<uint32_t>(pos) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
+    const uint32_t head_bytes = (1u << (kv.page_shift - 4u)) * kv.block_bytes;      // of a page
+    uint32_t j = 0, f = blockIdx.y * kWarps + warp;
+    move(j, f);
+    if (j < n_tok) fetch(j, f);
+    while (j < n_tok) {
+        const uint32_t u0 = f * 4u, u = u0 + sub, t = t0 + j, jn = j;
         const Eight<T> raw = ahead;
-        if (i + step < n_fours) fetch(i + step);
-        if (!places.own[j]) continue;
+        f += step;
+        move(j, f);
+        if (j < n_tok) fetch(j, f);
+        if (!places.own[jn]) continue;
+        const int32_t page = places.page[jn];
         const bool is_q = u < nq, is_v = u >= nq + nk, there = u < units && (is_q || page >= 0);
         const uint32_t gr = is_q ? u : is_v ? u - nq - nk : u - nq, d = gr % G * 64u + 8u * l;
         const bool rotate = a.freq && !is_v;
-        float x[8], wide = 0.0f;      // wide: the most that a rotated value can be
+        float x[8];
+        uint32_t wide = 0;      // |x0| + |x1| of the pairs, as bits: a NaN counts as more than infinity
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) x[e] = there ? raw[e] : 0.0f;
-        if (rotate) {
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; e += 2u) {
-                const float2 r = turns[j][d / 2u + e / 2u];
-                const float y0 = fmaf(x[e], r.x, -x[e + 1] * r.y), y1 = fmaf(x[e], r.y, x[e + 1] * r.x);
-                wide = fmaxf(wide, fabsf(x[e]) + fabsf(x[e + 1]));
+        for (uint32_t e = 0; e < 8u; e += 2u) wide = max(wide, __float_as_uint(fabsf(x[e]) + fabsf(x[e + 1])) & 0x7FFFFFFFu);
+        if (rotate) {
+            const float4* r = reinterpret_cast<const float4*>(&turns[jn][d / 2u]);
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; e += 4u) {
+                const float4 c = r[e / 4u];
+                const float y0 = fmaf(x[e], c.x, -x[e + 1] * c.y), y1 = fmaf(x[e], c.y, x[e + 1] * c.x);
+                const float y2 = fmaf(x[e + 2], c.z, -x[e + 3] * c.w), y3 = fmaf(x[e + 2], c.w, x[e + 3] * c.z);
                 x[e] = y0;
                 x[e + 1] = y1;
+                x[e + 2] = y2;
+                x[e + 3] = y3;
             }
         }
         if (there && is_q) store8(static_cast<T*>(a.q_out) + t * a.q_out_stride + gr * 64u + 8u * l, a.q_out_vec, x);
         if (u0 + 4u <= nq || page < 0) continue;       // for the whole warp
         // ---- the group: fp32, and what its error leaves open ----
-        float lo = x[0], hi = x[0];
-        bool fine = true;
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            lo = fminf(lo, x[i]);
-            hi = fmaxf(hi, x[i]);
-            fine = fine && fabsf(x[i]) <= 65504.0f;      // what saturates or is not finite: slowly
-        }
+        float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+        float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         lo = over_group<float>(lo, least);
         hi = over_group<float>(hi, most);
-        wide = over_group<float>(wide, most);
+#pragma unroll
+        for (uint32_t o = 4; o; o >>= 1) wide = max(wide, __shfl_xor_sync(0xFFFFFFFFu, wide, o));
+        bool fine = wide <= 0x477FE000u || is_q;      // 65504: what saturates or is not finite goes slowly
         // rotation: cos and sin are 2^-24.9 off, a product and the sum round: 2.6 2^-24 (|x0| + |x1|)
-        const float err = wide * 0x1p-22f;
+        const float err = rotate ? __uint_as_float(wide) * 0x1p-22f : 0.0f;
         const float width = hi - lo, step15 = width * (1.0f / 15.0f), step_err = fmaf(step15, 0x1p-22f, err * 0.134f);
         __half mn, st;
-        fine = fine && settled(lo - err, lo + err, mn);
-        fine = fine && settled(step15 - step_err, step15 + step_err, st);
+        fine = (settled(lo - err, lo + err, mn) || is_q) && fine;
+        fine = (settled(step15 - step_err, step15 + step_err, st) || is_q) && fine;
         const float m = __half2float(mn), s = __half2float(st);
         uint32_t c[8];
         {
             // (x - m) / s: three roundings of 2^-24 on at most 16. What lies outside 0 .. 15 by less than half a code falls to
             // the same side whatever its error
-            const float by = s > 0.0f ? 1.0f / s : 0.0f, open = 0.5f - fmaf(err, by, 17.0f * 0x1p-22f);
+            const float by = s > 0.0f ? __frcp_rn(s) : 0.0f, open = 0.5f - fmaf(err, by, 17.0f * 0x1p-22f);
             constexpr float kWhole = 12582912.0f;      // 1.5 2^23: adding it rounds to a whole number, which its low bits are
+            const f32x2 less = pack2(-m, -m), times = pack2(by, by), whole = pack2(kWhole, kWhole), back = pack2(-kWhole, -kWhole), minus = pack2(-1.0f, -1.0f);
+            float off = 0.0f;
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) {
-                const float q = fminf(fmaxf((x[e] - m) * by, 0.0f), 15.0f), r = q + kWhole;
-                fine = fine && fabsf(q - (r - kWhole)) < open;
-                c[e] = __float_as_uint(r) & 15u;
+            for (uint32_t e = 0; e < 8u; e += 2u) {
+                const float2 q = unpack2(mul2(add2(pack2(x[e], x[e + 1]), less), times));
+                const f32x2 p = pack2(fminf(fmaxf(q.x, 0.0f), 15.0f), fminf(fmaxf(q.y, 0.0f), 15.0f));
+                const f32x2 r = add2(p, whole);
+                const float2 w = unpack2(fma2(add2(r, back), minus, p)), b = unpack2(r);
+                off = fmaxf(off, fmaxf(fabsf(w.x), fabsf(w.y)));
+                c[e] = __float_as_uint(b.x) & 15u;
+                c[e + 1] = __float_as_uint(b.y) & 15u;
             }
+            fine = fine && (off < open || is_q);
         }
         if (!__all_sync(0xFFFFFFFFu, fine)) {
             float v[8];
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e) v[e] = there ? raw[e] : 0.0f;
-            quantise_slowly(v, rotate, pos, a.freq ? a.freq + d / 2u : nullptr, c, mn, st);
+            quantise_slowly(v, rotate, places.pos[jn], a.freq ? a.freq + d / 2u : nullptr, c, mn, st);
         }
         if (there && !is_q) {
-            uint8_t* block = kv.base + kv.block_at(page, gr / G, at);
+            const uint32_t at = static_cast<uint32_t>(places.pos[jn]) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
+            uint8_t* block = kv.base + (static_cast<size_t>(page) * kv.kv_heads + gr / G) * head_bytes + (at >> 4) * kv.block_bytes;
             const uint32_t h0 = pack_codes(c[0], c[1], c[2], c[3]), h1 = pack_codes(c[4], c[5], c[6], c[7]);
             if (is_v) {
                 uint16_t* to = reinterpret_cast<uint16_t*>(block + value_offset<HD>(tok, d));
@@ -282,9 +301,15 @@ kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restric
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, l = lane & 7u;
     locate(kv, b, t0, n_tok, places);
     const uint32_t nk = kv.kv_heads * G, units = 2u * nk, fours = (units + 3u) / 4u;
-#pragma unroll 2
-    for (uint32_t f = blockIdx.y * kWarps + warp; f < n_tok * fours; f += gridDim.y * kWarps) {
-        const uint32_t j = f / fours, u = f % fours * 4u + (lane >> 3), t = t0 + j;
+    const uint32_t head_bytes = (1u << (kv.page_shift - 4u)) * kv.block_bytes;      // of a page
+    uint32_t j = 0, f = blockIdx.y * kWarps + warp;
+    for (;; f += gridDim.y * kWarps) {      // the limit is n_tok
+        while (f >= fours && j < n_tok) {
+            f -= fours;
+            ++j;
+        }
+        if (j >= n_tok) break;
+        const uint32_t u = f * 4u + (lane >> 3), t = t0 + j;
         if (u >= units || !places.own[j]) continue;
         const int32_t page = places.page[j];
         const uint32_t at = static_cast<uint32_t>(places.pos[j]) & ((1u << kv.page_shift) - 1u), tok = at & 15u;
@@ -294,7 +319,7 @@ kv_read_kernel(KvView kv, KvBatchView b, float* __restrict__ k, float* __restric
 #pragma unroll
         for (uint32_t i = 0; i < 8u; ++i) x[i] = 0.0f;
         if (page >= 0) {
-            const uint8_t* block = kv.base + kv.block_at(page, gr / G, at);
+            const uint8_t* block = kv.base + (static_cast<size_t>(page) * kv.kv_heads + gr / G) * head_bytes + (at >> 4) * kv.block_bytes;
             uint32_t h[2];
             if (is_v) {
                 const uint16_t* from = reinterpret_cast<const uint16_t*>(block + value_offset<HD>(tok, d));
