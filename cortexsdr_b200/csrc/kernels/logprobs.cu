@@ -170,7 +170,7 @@ __device__ __noinline__ void best_of(const u64* from, uint32_t n, u64* to, uint3
 }
 
 template <typename T, bool TOP, uint32_t kThreads>
-__global__ void __launch_bounds__(kThreads, 768 / kThreads)
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 logprob_kernel(LogprobArgs a) {
     constexpr uint32_t kWarps = kThreads / 32;
     __shared__ Shared<kWarps> sh;
@@ -430,7 +430,8 @@ void launch_logprobs(csdr_context* ctx, int dtype, const LogprobArgs& a) {
     LaunchScope ls(ctx, KC_LOGPROB);
     with_dtype(dtype, [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        // three CTAs of 256 threads an SM; where a row is cut because there are few, one of 512
+        // four CTAs of 256 threads an SM (three: 140 us instead of 133 for 2048 rows of 151936); where a row is cut because
+        // there are few, 512
         uint32_t ranks = 1;
         while (ranks < 8u && static_cast<uint64_t>(a.rows) * ranks * 2u <= static_cast<uint64_t>(ctx->sm_count) &&
                a.vocab / (ranks * 2u) >= 512u * Vec<T>::N)
