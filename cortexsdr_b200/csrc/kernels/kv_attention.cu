@@ -718,7 +718,7 @@ kv_attention_kernel(AttnParams p) {
         if (second) copy(SB, pg1, sub + 1u, second);
     };
 
-    while (x < x1 && live) {
+    while (x < x1) {      // without the keys once a wait has run out: who joins a unit counts on everyone
         // ---- the unit that holds place x ----
         uint64_t w = sq.head_weight() * p.kv.kv_heads;
         while (x >= seq_at + w) {
@@ -769,7 +769,7 @@ kv_attention_kernel(AttnParams p) {
         if constexpr (KEYS) {
             // a warp's i-th piece is number 4 (b0 + i) + warp; the pages of sixteen pieces at a time, a lane a block
             const uint32_t first = 4u * b0 + warp;
-            const uint32_t n = 2u * first >= subs ? 0u : min(b1 - b0, (subs - 2u * first + 7u) / 8u);
+            const uint32_t n = !live || 2u * first >= subs ? 0u : min(b1 - b0, (subs - 2u * first + 7u) / 8u);
             int32_t page_of = -1;
             uint32_t there = 0;      // two bits a stage: the piece's blocks have pages
             auto issue = [&](uint32_t i) {
@@ -790,8 +790,11 @@ kv_attention_kernel(AttnParams p) {
             if constexpr (Warp::kShared) __syncthreads();
             for (uint32_t i = 0; i < n; ++i) {
                 const uint32_t k = turn0 + i, st = k % kStages;
-                live = live && mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
-                if (!live) break;
+                live = mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
+                if (!live) {
+                    for (uint32_t j = k; j < turn; ++j) mbar_wait(my_bar + 8u * (j % kStages), (j / kStages) & 1u, kDrainRounds);
+                    break;
+                }
                 rows.piece(my_ring + st * kStageBytes, static_cast<int32_t>((first + 4u * i) * kPiece), there >> 2u * st & 3u, lane, my_q, my_meta);
                 __syncwarp();
                 if (i + kStages < n) issue(i + kStages);
@@ -800,7 +803,8 @@ kv_attention_kernel(AttnParams p) {
             rows.store(rows_of(warp), lane);
         } else {
             // All warps see every piece. Warp 0 copies: a stage when all are through with it, one piece behind their work
-            const uint32_t first = 4u * b0, n = min(4u * (b1 - b0), (max(subs, 2u * first) - 2u * first + 1u) / 2u), turn0 = turn;
+            const uint32_t first = 4u * b0, n = live ? min(4u * (b1 - b0), (max(subs, 2u * first) - 2u * first + 1u) / 2u) : 0u, turn0 = turn;
+            uint32_t issued = 0;
             int32_t page_of = -1;
             auto issue = [&](uint32_t i) {
                 if ((i & 15u) == 0u) {
@@ -811,7 +815,9 @@ kv_attention_kernel(AttnParams p) {
                 const int32_t pg0 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u)), pg1 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u) + 1u);
                 const uint32_t k = turn0 + i, st = k % kStages;
                 if (k >= kStages) live = live && mbar_wait(smem_u32(&empty[st]), (k / kStages - 1u) & 1u, p.spin);
-                if (live && lane == 0) {
+                if (!live) return;
+                ++issued;
+                if (lane == 0) {
                     there_s[st] = (pg0 >= 0 ? 1u : 0u) | (pg1 >= 0 ? 2u : 0u);
                     fetch(my_ring + st * kStageBytes, my_bar + 8u * st, 2u * (first + i), pg0, pg1);
                 }
@@ -830,6 +836,9 @@ kv_attention_kernel(AttnParams p) {
                 if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[st])) : "memory");
                 if (warp == 0 && i >= 1u && i - 1u + kStages < n) issue(i - 1u + kStages);
             }
+            if (!live)      // warp 0 has copied
+                for (uint32_t j = max(issued, kStages) - kStages; j < issued; ++j)
+                    mbar_wait(my_bar + 8u * ((turn0 + j) % kStages), ((turn0 + j) / kStages) & 1u, kDrainRounds);
             turn += n;
         }
         live = __syncthreads_and(live);

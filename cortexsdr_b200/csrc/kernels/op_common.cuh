@@ -52,6 +52,8 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return done != 0u;
 }
+// How long a kernel that has given up waits for its own copies, which write into its shared memory until they are done.
+constexpr uint32_t kDrainRounds = 4000000u;
 // The whole warp waits, and gives up as one.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
     if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
