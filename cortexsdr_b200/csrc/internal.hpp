@@ -129,6 +129,7 @@ struct csdr_context {
     static constexpr int kEncoderScratch = 8, kScratchSlots = 13;
     csdr::DevPtr scratch[kScratchSlots];
     void* scratch_get(int slot, size_t bytes);
+    std::vector<csdr::DevPtr> held;             // scratch that captured 4-bit products use: a larger call moves the slot, not these
     void encoder_scratch_trim() noexcept;       // at the end of an encoder call: keeps up to 256 MB a slot
     // What a segment keeps although there is a form that does without it (a rebuilt weight, coefficient
     // entries). Null where all of them together would pass the budget or the device has no room.

@@ -288,14 +288,17 @@ q4_matmul_kernel(Q4Params p) {
             stage<T, FMT, NT>(p, u0, u1, tok0, n_tok, xs, tid, kThreads);
             return;
         }
-        if (tid == 0) {
+        if (tid == 0 && live) {
             const uint32_t bytes = (u1 - u0) * S::kStageBytes;
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&bar)), "r"(bytes) : "memory");
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(xs)),
                          "l"(p.planes + (static_cast<size_t>(blockIdx.y) * p.w.n_units + u0) * S::kStageBytes), "r"(bytes), "r"(smem_u32(&bar))
                          : "memory");
         }
-        live = live && mbar_wait(smem_u32(&bar), copies & 1u, p.spin);
+        if (live && !mbar_wait(smem_u32(&bar), copies & 1u, p.spin)) {
+            live = false;
+            if (warp == 0) mbar_wait(smem_u32(&bar), copies & 1u, kDrainRounds);
+        }
         ++copies;
     };
     if (staged_once && u_end > u_begin) {
@@ -486,7 +489,10 @@ void launch(csdr_context* ctx, Q4Params p) {
     const size_t items = static_cast<size_t>(p.units_rank) * std::min<size_t>(p.a.batch, S::kTokens) * S::kGroups * 4u;
     size_t each = std::max<size_t>(1, std::min<size_t>(tiles, (16u << 20) / tile_bytes));
     bool ahead = items > 2u * kThreads;
-    if (ahead && (!ctx->scratch[5] || ctx->scratch[5]->bytes < each * tile_bytes) && ctx->capturing()) ahead = false;
+    if (ahead && ctx->capturing()) {
+        if (!ctx->scratch[5] || ctx->scratch[5]->bytes < each * tile_bytes) ahead = false;
+        else if (ctx->held.empty() || ctx->held.back() != ctx->scratch[5]) ctx->held.push_back(ctx->scratch[5]);      // for the graph
+    }
     if (!ahead) each = tiles;
     const Q4Args all = p.a;
     for (size_t t0 = 0; t0 < tiles; t0 += each) {

@@ -2,6 +2,7 @@
 // and log probabilities of given tokens. Argument checks here, arithmetic in kernels/.
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <limits>
 #include <vector>
 
@@ -19,6 +20,13 @@ void need_dtype(int dtype) {
         throw Error(CSDR_ERR_INVALID_ARG, "unknown dtype");
 }
 
+// Elements of `bytes` bytes are read and written whole.
+void need_whole(size_t bytes, std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) % bytes) throw Error(CSDR_ERR_INVALID_ARG, "a pointer is not on a whole element");
+}
+size_t dtype_bytes(int dtype) { return dtype == CSDR_DTYPE_F32 ? 4u : 2u; }
+
 void need_cache(csdr_kv_cache* c, uint32_t layer) {
     if (!c) throw Error(CSDR_ERR_INVALID_ARG, "cache is null");
     require_ctx(c->ctx);
@@ -31,6 +39,7 @@ KvBatchView view_of(const csdr_kv_batch* b) {
         throw Error(CSDR_ERR_INVALID_ARG, "batch: null array");
     if (b->n_tokens > 0x7FFFFFFFu || b->n_seqs > 0x7FFFFFFEu || b->pages_per_seq == 0)
         throw Error(CSDR_ERR_INVALID_ARG, "batch: counts out of range");
+    need_whole(4, {b->first_dev, b->length_dev, b->pages_dev});
     return {b->first_dev, b->length_dev, b->pages_dev, b->n_seqs, b->n_tokens, b->pages_per_seq};
 }
 
@@ -56,6 +65,8 @@ int csdr_kv_cache_create(csdr_context* ctx, uint32_t n_layers, uint32_t n_pages,
         if (head_dim != 64 && head_dim != 128 && head_dim != 256)
             throw Error(CSDR_ERR_UNSUPPORTED, "cache: head_dim must be 64, 128 or 256");
         if (!std::isfinite(rope_theta)) throw Error(CSDR_ERR_INVALID_ARG, "cache: rope_theta is not finite");
+        if (rope_theta > 0.0f && rope_theta < 1.0f)
+            throw Error(CSDR_ERR_INVALID_ARG, "cache: rope_theta must be at least 1, or none (<= 0)");
         auto c = std::make_unique<csdr_kv_cache>();
         c->ctx = ctx;
         c->n_layers = n_layers;
@@ -114,12 +125,15 @@ int csdr_kv_cache_append_device_async(csdr_kv_cache* c, uint32_t layer, const cs
         a.q = q_dev;
         a.q_out = q_out_dev;
         a.kv_stride = row_stride(kv_stride, static_cast<size_t>(c->kv_heads) * c->head_dim, "k and v");
+        need_whole(dtype_bytes(dtype), {k_dev, v_dev, q_dev, q_dev ? q_out_dev : nullptr});
         if (q_dev) {
             if (!q_heads || q_heads > 65535u) throw Error(CSDR_ERR_INVALID_ARG, "q: head count out of range");
             if (!q_out_dev) throw Error(CSDR_ERR_INVALID_ARG, "q_out is null");
             a.q_heads = q_heads;
             a.q_stride = row_stride(q_stride, static_cast<size_t>(q_heads) * c->head_dim, "q");
             a.q_out_stride = row_stride(q_out_stride, static_cast<size_t>(q_heads) * c->head_dim, "q_out");
+            if (q_out_dev == q_dev && a.q_stride != a.q_out_stride && b.n_tokens > 1u)
+                throw Error(CSDR_ERR_INVALID_ARG, "q_out is q, but its stride is another");
         }
         if (rotate && !c->freq) throw Error(CSDR_ERR_INVALID_ARG, "the cache was made without a rotation (rope_theta <= 0)");
         if (rotate) a.freq = static_cast<const double*>(c->freq->ptr);
@@ -133,6 +147,7 @@ int csdr_kv_cache_read_device_async(csdr_kv_cache* c, uint32_t layer, const csdr
     return guard([&] {
         need_cache(c, layer);
         const KvBatchView b = view_of(batch);
+        need_whole(4, {k_dev, v_dev});
         if (!b.n_tokens || !b.n_seqs) return;
         if (!k_dev || !v_dev) throw Error(CSDR_ERR_INVALID_ARG, "null argument");
         launch_kv_read(c->ctx, c->layer(layer), c->head_dim, b, k_dev, v_dev);
@@ -149,6 +164,7 @@ int csdr_kv_cache_attention_device_async(csdr_kv_cache* c, uint32_t layer, const
         if (!q_heads || q_heads > 65535u || q_heads % c->kv_heads)
             throw Error(CSDR_ERR_INVALID_ARG, "q_heads must be a multiple of the cache's kv_heads");
         if (!std::isfinite(scale)) throw Error(CSDR_ERR_INVALID_ARG, "scale is not finite");
+        need_whole(dtype_bytes(dtype), {q_dev, out_dev});
         KvAttend a{};
         a.q = q_dev;
         a.out = out_dev;
@@ -210,6 +226,8 @@ int csdr_q4_matmul_device_async(csdr_context* ctx, const csdr_q4_weight* w, cons
         if ((x_layout != CSDR_LAYOUT_FEATURE_MAJOR && x_layout != CSDR_LAYOUT_TOKEN_MAJOR) ||
             (y_layout != CSDR_LAYOUT_FEATURE_MAJOR && y_layout != CSDR_LAYOUT_TOKEN_MAJOR))
             throw Error(CSDR_ERR_INVALID_ARG, "unknown dtype or layout");
+        need_whole(dtype_bytes(x_dtype), {x_dev});
+        need_whole(4, {y_dev, bias_dev});
         if (!batch) return;
         Q4Args a{};
         a.x = x_dev;
@@ -245,6 +263,8 @@ int csdr_token_logprobs_device_async(csdr_context* ctx, const void* logits_dev, 
         a.top = top;
         a.top_ids = top_ids_dev;
         a.top_logprobs = top_logprobs_dev;
+        need_whole(dtype_bytes(dtype), {logits_dev});
+        need_whole(4, {targets_dev, logprobs_dev, entropy_dev, top_ids_dev, top_logprobs_dev});
         if (!rows) return;
         if (!logits_dev || (logprobs_dev && !targets_dev) || (top && (!top_ids_dev || !top_logprobs_dev)))
             throw Error(CSDR_ERR_INVALID_ARG, "null argument");

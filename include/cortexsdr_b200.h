@@ -501,8 +501,8 @@ CSDR_API int csdr_decoder_step_device_async(csdr_decoder* d, const int32_t* toke
  * number of sequences through page tables. Each group of 64 values of a head is held as 4-bit codes with
  * an fp16 minimum and an fp16 step: minimum + step * code, step = (max - min) / 15 (4.5 bits a value with
  * head_dim 64, 128 or 256; 0.28 of an fp16 cache). A group that holds a value that is not finite reads
- * back as NaN; values past 65504 saturate. rope_theta > 0: the rotary embedding that
- * csdr_kv_cache_append_device_async applies on request. */
+ * back as NaN; values past 65504 saturate. rope_theta at least 1: the rotary embedding that
+ * csdr_kv_cache_append_device_async applies on request; 0 or less: none. */
 CSDR_API int csdr_kv_cache_create(csdr_context* ctx, uint32_t n_layers, uint32_t n_pages,
                                   uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim,
                                   float rope_theta, csdr_kv_cache** out);
@@ -556,7 +556,9 @@ CSDR_API int csdr_q4_create(csdr_context* ctx, const char* format, const void* p
                             uint32_t rows, uint32_t cols, csdr_q4_weight** out);
 CSDR_API int csdr_q4_destroy(csdr_q4_weight* weight);
 /* y = W x (+ bias), fp32 out; dtypes (CSDR_DTYPE_F16 too) and layouts as csdr_matmul_device_async. Products and sums
- * are those of fp32 activations. Asynchronous on the context's stream. */
+ * are those of fp32 activations; an activation that is not finite leaves its token's results not finite. y must not
+ * overlap x. Products of several tokens share scratch of the context: they run one after the other, graphs that were
+ * captured from them too. Asynchronous on the context's stream. */
 CSDR_API int csdr_q4_matmul_device_async(csdr_context* ctx, const csdr_q4_weight* weight,
                                          const void* x_dev, int x_dtype, int x_layout, size_t batch,
                                          float* y_dev, int y_layout, const float* bias_dev);

@@ -442,3 +442,57 @@ def test_refusals(ctx, lib):
     c.cache.attention(cs.KVBatch(1, 0, 0, 0, 0, 1), 0, 0, 4, 0)
     assert ctx.launch_count == before
     assert lib.csdr_kv_cache_read_device_async(None, 0, b._ref, p, p) == _lib.ERR_INVALID_ARG
+
+
+def test_refuses_pointers_inside_an_element_and_angles_without_a_bound(ctx):
+    c = Case(ctx, [16], [16], 2, 64, 16)
+    b = c.batch([16], [16])
+    x = torch.zeros(16, 5, 64, device="cuda")
+    p = x.data_ptr()
+    off = cs.KVBatch(1, 16, p + 2, p, p, 1)
+    for call in [
+        lambda: c.cache.append(b, p + 2, p, 0), lambda: c.cache.append(b, p, p + 1, 1), lambda: c.cache.append(b, p, p + 1, 2),
+        lambda: c.cache.append(b, p, p, 0, q_ptr=p + 2, q_heads=4, q_out_ptr=p),
+        lambda: c.cache.append(b, p, p, 0, q_ptr=p, q_heads=4, q_out_ptr=p + 3),
+        lambda: c.cache.append(off, p, p, 0), lambda: c.cache.read(off, p, p), lambda: c.cache.read(b, p + 2, p),
+        lambda: c.cache.attention(b, p + 2, 0, 4, p), lambda: c.cache.attention(b, p, 1, 4, p + 1), lambda: c.cache.attention(off, p, 0, 4, p),
+    ]:
+        with pytest.raises(ValueError, match="whole element"):
+            call()
+    with pytest.raises(ValueError, match="stride is another"):
+        c.cache.append(b, p, p, 0, q_ptr=p, q_stride=256, q_heads=4, q_out_ptr=p, q_out_stride=260)
+    with pytest.raises(ValueError, match="at least 1"):
+        cs.KVCache(4, 16, 1, 64, rope_theta=0.5, ctx=ctx)
+    c.cache.close()
+
+
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_negative_scale(ctx, fresh):
+    c = Case(ctx, [150, 40], [fresh, fresh], 2, 128, 32, seed=5)
+    c.store(rotate=False)
+    qs = [c.values((fresh, 4, 128)) for _ in range(2)]
+    got = c.attend(c.rows(qs), 4, scale=-0.05)
+    hk, hv = c.held()
+    want = np.concatenate([ref.attention(q.to(torch.float64).numpy(), k, v, np.arange(n - fresh, n), -0.05) for q, k, v, n in zip(qs, hk, hv, c.lengths)])
+    close(got, want, torch.float32, 16.0)
+
+
+@pytest.mark.parametrize("dtype,fresh", [("f32", 1), ("bf16", 200)])
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_cache_usable(dtype, fresh):
+    """The shortest limit: whether it runs out or not, a later call with the usual one is right."""
+    own = cs.Context(0)
+    c = Case(own, [9000, 500, 2000], [fresh] * 3, 2, 128, 64, seed=6, dtype=dtype)
+    c.store(rotate=False)
+    q = c.rows([c.values((fresh, 8, 128)) for _ in range(3)])
+    want = c.attend(q, 8)
+    own.set_wait_limits(barrier_rounds=1)
+    for _ in range(3):
+        try:
+            got = c.attend(q, 8)
+        except cs.CudaError:
+            continue
+        assert torch.equal(got, want)
+    own.set_wait_limits()
+    assert torch.equal(c.attend(q, 8), want)
+    c.cache.close()
+    own.close()

@@ -125,3 +125,37 @@ def test_refusals(ctx):
     before = ctx.launch_count
     cs.token_logprobs_device(p, 0, 0, 10, 0, 0, ctx=ctx)
     assert ctx.launch_count == before
+
+
+def test_refuses_pointers_inside_an_element(ctx):
+    p = torch.zeros(2, 10, device="cuda").data_ptr()
+    for args in [(p + 2, 0, 2, 8, p, p), (p + 1, 1, 2, 8, p, p), (p, 0, 2, 8, p + 2, p), (p, 0, 2, 8, p, p + 1), (p, 0, 2, 8, p, p, p + 3),
+                 (p, 0, 2, 8, p, p, 0, 2, p + 2, p), (p, 0, 2, 8, p, p, 0, 2, p, p + 2)]:
+        with pytest.raises(ValueError, match="whole element"):
+            cs.token_logprobs_device(*args, ctx=ctx)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 50000), (700, 1000)])
+def test_on_a_stream_of_its_own_captured_and_replayed(rows, vocab):
+    side = torch.cuda.Stream()
+    own = cs.Context(0, side.cuda_stream)
+    x = torch.zeros(rows, vocab, device="cuda", dtype=torch.bfloat16)
+    t = torch.randint(0, vocab, (rows,), dtype=torch.int32, device="cuda")
+    lp, ids, alt = torch.zeros(rows, device="cuda"), torch.zeros(rows, 4, dtype=torch.int32, device="cuda"), torch.zeros(rows, 4, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            cs.token_logprobs_device(x.data_ptr(), 1, rows, vocab, t.data_ptr(), lp.data_ptr(), 0, 4, ids.data_ptr(), alt.data_ptr(), ctx=own)
+        for seed in range(2):
+            torch.manual_seed(seed)
+            x.copy_(torch.randn(rows, vocab, device="cuda") * 3)
+            g.replay()
+            side.synchronize()
+            want = torch.log_softmax(x.double(), -1)
+            # 2e-5: an fp32 sum of `vocab` terms and the logarithm's own rounding, next to values of about 10
+            assert (lp.double() - want.gather(1, t.long()[:, None])[:, 0]).abs().max() < 2e-5
+            order = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :4]
+            assert torch.equal(ids.long(), order)
+    del g
+    own.close()

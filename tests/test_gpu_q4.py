@@ -167,3 +167,70 @@ def test_refusals(ctx):
     before = ctx.launch_count
     w.matmul_device(x.data_ptr(), 0, 1, 0, y.data_ptr(), 1)
     assert ctx.launch_count == before
+
+
+def test_refuses_pointers_inside_an_element(ctx):
+    payload, _ = ref.q4_weight(np.random.default_rng(0), 4, 256, "q4_0")
+    w = cs.Q4Weight.from_payload(payload, "q4_0", 4, 256, ctx)
+    x, y = torch.zeros(300, device="cuda").data_ptr(), torch.zeros(8, device="cuda").data_ptr()
+    for args in [(x + 2, 0, 1, 1, y, 1), (x + 1, 1, 1, 1, y, 1), (x + 1, 2, 1, 1, y, 1), (x, 0, 1, 1, y + 2, 1), (x, 0, 1, 1, y, 1, y + 1)]:
+        with pytest.raises(ValueError, match="whole element"):
+            w.matmul_device(*args)
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("warm", [False, True])
+def test_a_captured_wide_product(layout, warm):
+    """Captured first of all in its context, and behind one that sized the scratch; then replayed after a larger product
+    has moved that scratch."""
+    rng = np.random.default_rng(11)
+    side = torch.cuda.Stream()
+    own = cs.Context(0, side.cuda_stream)
+    payload, dense = ref.q4_weight(rng, 300, 4096, "q4_k")
+    w = cs.Q4Weight.from_payload(payload, "q4_k", 300, 4096, own)
+    big, _ = ref.q4_weight(rng, 64, 16384, "q4_0")
+    larger = cs.Q4Weight.from_payload(big, "q4_0", 64, 16384, own)
+    x = torch.tensor(rng.normal(0, 1, (40, 4096)), dtype=torch.float32).cuda()
+    given = x.t().contiguous() if layout == 0 else x
+    y = torch.zeros(40, 300, device="cuda")
+    x2, y2 = torch.zeros(128, 16384, device="cuda"), torch.empty(128, 64, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        if warm:
+            w.matmul_device(given.data_ptr(), 0, layout, 40, y.data_ptr(), 1)
+            side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            w.matmul_device(given.data_ptr(), 0, layout, 40, y.data_ptr(), 1)
+        for _ in range(2):
+            y.zero_()
+            g.replay()
+            side.synchronize()
+            check(y.to(torch.float64).cpu().numpy(), x.cpu(), dense)
+            larger.matmul_device(x2.data_ptr(), 0, 1, 128, y2.data_ptr(), 1)
+    side.synchronize()
+    assert (y2 == 0).all()
+    del g
+    w.close()
+    larger.close()
+    own.close()
+
+
+def test_a_wait_that_runs_out_is_reported():
+    own = cs.Context(0)
+    rng = np.random.default_rng(12)
+    payload, dense = ref.q4_weight(rng, 512, 8192, "q4_0")
+    w = cs.Q4Weight.from_payload(payload, "q4_0", 512, 8192, own)
+    x = torch.tensor(rng.normal(0, 1, (48, 8192)), dtype=torch.float32)
+    want = run(w, x, 1, 512, own)
+    own.set_wait_limits(barrier_rounds=1)
+    for _ in range(3):
+        try:
+            got = run(w, x, 1, 512, own)
+        except cs.CudaError:
+            continue
+        np.testing.assert_array_equal(got, want)
+    own.set_wait_limits()
+    np.testing.assert_array_equal(run(w, x, 1, 512, own), want)
+    w.close()
+    own.close()
