@@ -17,7 +17,7 @@ SOURCES = [
     "kernels/gemv_queue.cu",
     "kernels/decoder_ops.cu", "kernels/attention_prompt.cu",
     "kernels/gemm_tcgen05.cu", "kernels/gemm_tma.cu", "kernels/gemm_simt.cu", "kernels/gather_mma.cu",
-    "kernels/kv_cache.cu", "kernels/kv_attention.cu", "kernels/q4_matmul.cu", "kernels/logprobs.cu",
+    "kernels/kv_cache.cu", "kernels/kv_attention.cu", "kernels/kv_attention_tc.cu", "kernels/q4_matmul.cu", "kernels/logprobs.cu",
     "operators.cu",
     "decoder.cu",
     "kernels/encode.cu",

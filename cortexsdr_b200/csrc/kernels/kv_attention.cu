@@ -11,107 +11,25 @@
 // Rounding and rest carry 22 bits, sums are fp32's. A row's q is scaled by a power of two to use fp16's range, p step
 // likewise by the largest step met. The 8 comes off in every piece (by one more product, of p step with eights): the
 // matrix units cut sums off instead of rounding them, and sums of one sign drift (1e-5 of an output over 5000 keys).
-// tcgen05 would want the codes widened into shared memory first, which costs more than the products here.
+// tcgen05 wants the codes widened into shared memory first, which pays for prompts whose outputs round coarsely: bf16
+// (kv_attention_tc.cu).
 //
 // Work is cut evenly, whatever the lengths: units are (sequence, tile of query rows, kv head), their length in 128 keys
 // is known on the device, and CTA c of G takes the c-th G-th of all of it. A unit that is cut leaves partial
 // (maximum, sum, output) pieces; the last CTA to arrive at it joins them, in the order of the keys. Nothing depends on the
 // host knowing lengths, so a captured call follows its sequences as they grow.
 #include <algorithm>
-#include <cfloat>
 #include <type_traits>
 
 #include "codes4.cuh"
-#include "kv_cache.hpp"
-#include "op_common.cuh"
+#include "kv_attention.cuh"
 
 namespace csdr {
 
 namespace {
 
-constexpr uint32_t kWarps = 4, kThreads = kWarps * 32, kPiece = 32, kBlockKeys = kWarps * kPiece;
-constexpr float kSlack = 6.0f;
-template <int HD>
-constexpr uint32_t kPitch = HD + 4;      // of a row of outputs with its maximum and sum
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-struct AttnParams {
-    KvView kv;
-    KvBatchView b;
-    KvAttend a;
-    uint32_t group;          // query heads of a kv head
-    uint32_t vec, vec_out;   // rows of q, of the result start on 16 bytes
-    float* part;             // [CTA][2][rows][HD + 4]
-    uint32_t* counters;      // [CTA]: arrivals at the unit that starts in a CTA's share and is cut
-    int* status;
-    uint32_t spin;
-};
-
-__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
-    return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-}
-
-// A sequence as the schedule sees it.
-struct Seq {
-    int64_t base;            // position of its first new token
-    int64_t cap;             // keys that its table can hold
-    uint32_t row0, n_new, tiles;
-    uint32_t pair_weight, mid_weight;
-    // blocks of 128 keys that a tile of rows sees; at least one, so that rows that see nothing are written too
-    template <uint32_t TILE>
-    __device__ __forceinline__ int64_t keys(uint32_t tile, uint32_t group) const {
-        // TILE (tiles + 1) fits 32 bits (launch_kv_attention)
-        const uint32_t last = tile + 1u == tiles ? n_new - 1u : (TILE * (tile + 1u) - 1u) / group;
-        return min(max(base + last + 1, static_cast<int64_t>(0)), cap);
-    }
-    template <uint32_t TILE>
-    __device__ __forceinline__ uint32_t blocks(uint32_t tile, uint32_t group) const {
-        return max(1u, static_cast<uint32_t>((keys<TILE>(tile, group) + kBlockKeys - 1) / kBlockKeys));
-    }
-    // Causal tiles grow along a prompt: the first and the last tile make a pair, the second and the last but one,
-    // whose blocks add up to nearly the same, so that a place in the work is found by a division. What a pair
-    // has less than the weight is empty.
-    template <uint32_t TILE>
-    __device__ __forceinline__ void load(const AttnParams& p, uint32_t s) {
-        const int32_t f0 = p.b.first[s], f1 = p.b.first[s + 1];
-        const int64_t most = p.b.n_tokens;
-        const int64_t r0 = min(max(static_cast<int64_t>(f0), static_cast<int64_t>(0)), most);
-        const int64_t r1 = min(max(static_cast<int64_t>(f1), r0), most);
-        row0 = static_cast<uint32_t>(r0);
-        n_new = static_cast<uint32_t>(r1 - r0);
-        base = static_cast<int64_t>(p.b.length[s]) - f1 + r0;
-        cap = min(static_cast<int64_t>(p.b.pages_per_seq) << p.kv.page_shift, static_cast<int64_t>(0x7FFFFF00));
-        tiles = (n_new * p.group + TILE - 1u) / TILE;
-        pair_weight = mid_weight = 0;
-        if (!tiles) return;
-        if (tiles == 1u) {
-            mid_weight = blocks<TILE>(0, p.group);
-            return;
-        }
-        const uint32_t a = blocks<TILE>(0, p.group), z = blocks<TILE>(tiles - 1u, p.group);
-        // rounding to blocks and the last tile's missing rows: two blocks at most
-        pair_weight = tiles == 2u ? a + z : base + n_new > cap ? 2u * z : a + z + 2u;
-        if (tiles & 1u) mid_weight = blocks<TILE>(tiles / 2u, p.group);
-    }
-    // As lane `from` of the warp has it.
-    __device__ __forceinline__ Seq of_lane(uint32_t from) const {
-        Seq q;
-        q.base = __shfl_sync(0xFFFFFFFFu, base, from);
-        q.cap = __shfl_sync(0xFFFFFFFFu, cap, from);
-        q.row0 = __shfl_sync(0xFFFFFFFFu, row0, from);
-        q.n_new = __shfl_sync(0xFFFFFFFFu, n_new, from);
-        q.tiles = __shfl_sync(0xFFFFFFFFu, tiles, from);
-        q.pair_weight = __shfl_sync(0xFFFFFFFFu, pair_weight, from);
-        q.mid_weight = __shfl_sync(0xFFFFFFFFu, mid_weight, from);
-        return q;
-    }
-    __device__ __forceinline__ uint64_t head_weight() const { return static_cast<uint64_t>(tiles / 2u) * pair_weight + mid_weight; }
-};
+constexpr uint32_t kWarps = 4, kThreads = kWarps * 32, kPiece = 32;
+static_assert(kBlockKeys == kWarps * kPiece, "a block is a piece a warp");
 
 // A warp's query rows, 8 H of them: fragments, running maxima and sums, outputs. Lane (g, t) = (lane / 4, lane % 4) has the
 // scores of rows g + 8 h for keys 2t, 2t + 1 of every eight, and the outputs of rows 8 h + 2t, + 2t + 1 for values
@@ -186,7 +104,7 @@ struct Rows {
             const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : kTop;
             // the scale's sign goes with q: the largest score / factor is the largest score
             const float up = copysignf(power_of_two(kTop - e), p.a.scale);
-            factor[h] = fabsf(p.a.scale) * 1.4426950408889634f * power_of_two(min(e - kTop + kCodeShift, 127));
+            factor[h] = fmaxf(fabsf(p.a.scale) * 1.4426950408889634f * power_of_two(min(e - kTop + kCodeShift, 127)), FLT_MIN);
 #pragma unroll
             for (uint32_t g = 0; g < G; ++g) sum_q[h][g] = 0.0f;
 #pragma unroll
@@ -519,48 +437,6 @@ struct Rows {
     }
 };
 
-// Joins n pieces of a row (outputs, maximum, sum), eight values of it. `get` reads four floats of a piece.
-template <int HD, typename F>
-__device__ __forceinline__ void join(uint32_t n, uint32_t d, F&& get, float (&o)[8], float& m, float& l) {
-    m = -FLT_MAX;
-    l = 0.0f;
-#pragma unroll
-    for (uint32_t j = 0; j < 8u; ++j) o[j] = 0.0f;
-#pragma unroll 4
-    for (uint32_t i = 0; i < n; ++i) m = fmaxf(m, get(i, HD).x);
-#pragma unroll 4
-    for (uint32_t i = 0; i < n; ++i) {
-        const float4 st = get(i, HD), a = get(i, d), b = get(i, d + 4u);
-        const float f = ex2(st.x - m);
-        l = fmaf(f, st.y, l);
-        o[0] = fmaf(f, a.x, o[0]);
-        o[1] = fmaf(f, a.y, o[1]);
-        o[2] = fmaf(f, a.z, o[2]);
-        o[3] = fmaf(f, a.w, o[3]);
-        o[4] = fmaf(f, b.x, o[4]);
-        o[5] = fmaf(f, b.y, o[5]);
-        o[6] = fmaf(f, b.z, o[6]);
-        o[7] = fmaf(f, b.w, o[7]);
-    }
-}
-
-// Eight results, as one or two 128-bit pieces where rows start on 16 bytes.
-template <typename T>
-__device__ __forceinline__ void store_row(T* to, const float (&v)[8], float by, bool vec) {
-    T r[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i) r[i] = op_narrow<T>(v[i] * by);
-    if (vec) {
-        const uint4* from = reinterpret_cast<const uint4*>(r);
-        uint4* at = reinterpret_cast<uint4*>(to);
-        at[0] = from[0];
-        if constexpr (sizeof(T) == 4) at[1] = from[1];
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) to[i] = r[i];
-    }
-}
-
 // CTAs an SM: what the registers of the outputs leave room for.
 template <int HD, int H>
 __host__ __device__ constexpr int ctas() { return HD > 128 ? 2 : HD * H > 128 ? 3 : 4; }
@@ -589,9 +465,8 @@ kv_attention_kernel(AttnParams p) {
     __shared__ uint64_t bars[kWarps * kStages];
     __shared__ uint64_t empty[kStages];      // where the warps share stages: all are through with one
     __shared__ uint32_t there_s[kStages];
-    __shared__ uint64_t scan[kWarps];
-    __shared__ uint64_t found_at;
-    __shared__ uint32_t found, flag, longest, n_units;
+    __shared__ ScheduleShared<kThreads> sched;
+    __shared__ uint32_t flag;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     uint8_t* my_meta = meta_s + warp * Warp::kMetaBytes;
     uint4* my_q = reinterpret_cast<uint4*>(meta_s + kWarps * Warp::kMetaBytes + (KEYS ? 0u : warp) * (HD / 16u) * 512u);
@@ -603,100 +478,16 @@ kv_attention_kernel(AttnParams p) {
         for (uint32_t i = 0; i < kWarps * kStages; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&bars[i])));
         for (uint32_t i = 0; i < kStages; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&empty[i])), "r"(kWarps));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        longest = n_units = 0;
+        sched.longest = sched.n_units = 0;
     }
     __syncthreads();
     op_enter();
     asm volatile("fence.proxy.async;" ::: "memory");
 
-    // ---- this CTA's share of the work: places x0 to x1 - 1 ----
-    uint64_t total, x0 = 0, x1 = 0, ctas = 0;
-    auto share = [&](uint32_t longest_unit, uint32_t units) {
-        // Joining n pieces costs a CTA about a sixteenth of a block's time each: no unit is cut finer than both together take.
-        const uint64_t least_blocks = 1u + static_cast<uint32_t>(sqrtf(static_cast<float>(longest_unit) / 16.0f));
-        ctas = min(static_cast<uint64_t>(gridDim.x), max(quotient(total, least_blocks), static_cast<uint64_t>(1)));
-        // Units that are all as long, one a CTA, where sharing them evenly would save less than the joins cost (two blocks' time;
-        // 16 sequences of 1024 with 32 heads: 39.7 -> 33.9 us)
-        if (units <= gridDim.x && total == static_cast<uint64_t>(units) * longest_unit && longest_unit <= quotient(total, ctas) + 2u) {
-            ctas = units;
-            x0 = static_cast<uint64_t>(blockIdx.x) * longest_unit;
-            x1 = x0 + longest_unit;
-        } else {
-            x0 = quotient(blockIdx.x * total, ctas);
-            x1 = quotient((blockIdx.x + 1u) * total, ctas);
-        }
-    };
-    auto scan_up = [&](uint64_t v) {
-#pragma unroll
-        for (uint32_t o = 1; o < 32u; o <<= 1) {
-            const uint64_t w = __shfl_up_sync(0xFFFFFFFFu, v, o);
-            if (lane >= o) v += w;
-        }
-        return v;
-    };
-    uint32_t s;
-    uint64_t seq_at;
-    Seq sq;
-    if (p.b.n_seqs <= 32u) {
-        // every warp for itself, a lane a sequence
-        Seq q{};
-        if (lane < p.b.n_seqs) q.load<TILE>(p, lane);
-        const uint64_t w = q.head_weight() * p.kv.kv_heads, upto = scan_up(w);
-        total = __shfl_sync(0xFFFFFFFFu, upto, 31);
-        if (!total) return;
-        share(__reduce_max_sync(0xFFFFFFFFu, q.tiles ? q.blocks<TILE>(q.tiles - 1u, p.group) : 0u),
-              __reduce_add_sync(0xFFFFFFFFu, q.tiles * p.kv.kv_heads));
-        if (blockIdx.x >= ctas) return;
-        s = __ffs(__ballot_sync(0xFFFFFFFFu, x0 >= upto - w && x0 < upto)) - 1u;
-        seq_at = __shfl_sync(0xFFFFFFFFu, upto - w, s);
-        sq = q.of_lane(s);
-    } else {
-        const uint32_t per = (p.b.n_seqs + kThreads - 1u) / kThreads;
-        const uint32_t s_lo = min(tid * per, p.b.n_seqs), s_hi = min(s_lo + per, p.b.n_seqs);
-        uint64_t mine = 0;
-        uint32_t blocks = 0, units = 0;
-        for (uint32_t i = s_lo; i < s_hi; ++i) {
-            Seq q;
-            q.load<TILE>(p, i);
-            mine += q.head_weight() * p.kv.kv_heads;
-            if (q.tiles) blocks = max(blocks, q.blocks<TILE>(q.tiles - 1u, p.group));
-            units += q.tiles * p.kv.kv_heads;
-        }
-        atomicMax(&longest, blocks);
-        atomicAdd(&n_units, units);
-        const uint64_t upto = scan_up(mine);
-        if (lane == 31u) scan[warp] = upto;
-        __syncthreads();
-        uint64_t before = 0;
-        total = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kWarps; ++i) {
-            if (i < warp) before += scan[i];
-            total += scan[i];
-        }
-        if (!total) return;
-        share(longest, n_units);
-        if (blockIdx.x >= ctas) return;
-        uint64_t at = before + upto - mine;
-        if (x0 >= at && x0 < at + mine) {
-            for (uint32_t i = s_lo; i < s_hi; ++i) {
-                Seq q;
-                q.load<TILE>(p, i);
-                const uint64_t w = q.head_weight() * p.kv.kv_heads;
-                if (x0 < at + w) {
-                    found = i;
-                    found_at = at;
-                    break;
-                }
-                at += w;
-            }
-        }
-        __syncthreads();
-        s = found;
-        seq_at = found_at;
-        sq.load<TILE>(p, s);
-    }
-    uint64_t x = x0;
+    Schedule<TILE, kThreads> sch;
+    if (!sch.begin(p, sched)) return;
+    const uint64_t x1 = sch.x1;
+    uint64_t x = sch.x0;
     uint32_t turn = 0;       // stages filled so far
     bool live = true;
     Warp rows;
@@ -719,50 +510,17 @@ kv_attention_kernel(AttnParams p) {
     };
 
     while (x < x1) {      // without the keys once a wait has run out: who joins a unit counts on everyone
-        // ---- the unit that holds place x ----
-        uint64_t w = sq.head_weight() * p.kv.kv_heads;
-        while (x >= seq_at + w) {
-            seq_at += w;
-            sq.load<TILE>(p, ++s);
-            w = sq.head_weight() * p.kv.kv_heads;
+        Unit un;
+        if (!sch.at(p, x, un)) {
+            x = un.next;
+            continue;
         }
-        const uint64_t hw = sq.head_weight(), y = x - seq_at, pairs = static_cast<uint64_t>(sq.tiles / 2u) * sq.pair_weight;
-        const uint32_t kvh = static_cast<uint32_t>(quotient(y, hw));
-        const uint64_t z = y - kvh * hw;
-        uint32_t tile, b0;
-        uint64_t next = seq_at + kvh * hw;       // where the next unit starts
-        if (sq.tiles == 1u) {
-            tile = 0u;
-            b0 = static_cast<uint32_t>(z);
-            next += hw;
-        } else if (z < pairs) {
-            const uint32_t pr = static_cast<uint32_t>(quotient(z, sq.pair_weight)), o = static_cast<uint32_t>(z - static_cast<uint64_t>(pr) * sq.pair_weight);
-            const uint32_t n = sq.blocks<TILE>(pr, p.group);
-            next += static_cast<uint64_t>(pr) * sq.pair_weight;
-            tile = pr;
-            b0 = o;
-            if (o >= n) {
-                tile = sq.tiles - 1u - pr;
-                b0 = o - n;
-                next += sq.pair_weight;
-                if (b0 >= sq.blocks<TILE>(tile, p.group)) {    // the empty end of a pair
-                    x = next;
-                    continue;
-                }
-            } else {
-                next += n;
-            }
-        } else {
-            tile = sq.tiles / 2u;
-            b0 = static_cast<uint32_t>(z - pairs);
-            next += hw;
-        }
-        const uint32_t n_blocks = sq.blocks<TILE>(tile, p.group);
-        const uint64_t start = x - b0;
-        const uint32_t b1 = static_cast<uint32_t>(min(static_cast<uint64_t>(n_blocks), static_cast<uint64_t>(b0) + (x1 - x)));
-        const int32_t keys = static_cast<int32_t>(sq.keys<TILE>(tile, p.group));
+        const Seq& sq = sch.sq;
+        const uint32_t kvh = un.kvh, tile = un.tile, b0 = un.b0, b1 = un.b1, n_blocks = un.n_blocks;
+        const uint64_t start = un.start, next = un.next;
+        const int32_t keys = un.keys;
         head_base = p.kv.base + p.kv.block_at(0u, kvh, 0u);
-        const int32_t* table = p.b.pages + static_cast<size_t>(s) * p.b.pages_per_seq;
+        const int32_t* table = p.b.pages + static_cast<size_t>(sch.s) * p.b.pages_per_seq;
 
         // ---- its keys from block b0 to b1, in pieces of 32 ----
         const uint32_t subs = static_cast<uint32_t>(keys + 15) / 16u;      // blocks of sixteen that exist
@@ -775,7 +533,7 @@ kv_attention_kernel(AttnParams p) {
             auto issue = [&](uint32_t i) {
                 if ((i & 15u) == 0u) {
                     const uint32_t sub = 2u * (first + 4u * (i + (lane >> 1))) + (lane & 1u);
-                    page_of = sub < subs ? __ldg(table + (sub >> (p.kv.page_shift - 4u))) : -1;
+                    page_of = sub < subs ? table[sub >> (p.kv.page_shift - 4u)] : -1;
                     if (static_cast<uint32_t>(page_of) >= p.kv.n_pages) page_of = -1;
                 }
                 const int32_t pg0 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u)), pg1 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u) + 1u);
@@ -809,7 +567,7 @@ kv_attention_kernel(AttnParams p) {
             auto issue = [&](uint32_t i) {
                 if ((i & 15u) == 0u) {
                     const uint32_t sub = 2u * (first + i) + lane;
-                    page_of = sub < subs ? __ldg(table + (sub >> (p.kv.page_shift - 4u))) : -1;
+                    page_of = sub < subs ? table[sub >> (p.kv.page_shift - 4u)] : -1;
                     if (static_cast<uint32_t>(page_of) >= p.kv.n_pages) page_of = -1;
                 }
                 const int32_t pg0 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u)), pg1 = __shfl_sync(0xFFFFFFFFu, page_of, 2u * (i & 15u) + 1u);
@@ -848,7 +606,7 @@ kv_attention_kernel(AttnParams p) {
 
         // ---- out, or a piece of it ----
         const bool whole = b0 == 0u && b1 == n_blocks;
-        float* slot = p.part + (static_cast<size_t>(blockIdx.x) * 2u + (start >= x0 ? 1u : 0u)) * TILE * kPitch<HD>;
+        float* slot = p.part + (static_cast<size_t>(blockIdx.x) * 2u + (start >= sch.x0 ? 1u : 0u)) * TILE * kPitch<HD>;
         auto write = [&](uint32_t r, uint32_t d, const float(&o)[8], float l) {
             const uint32_t rr = tile * TILE + r, tok = rr / p.group, head = kvh * p.group + rr % p.group;
             if (tok >= sq.n_new) return;
@@ -878,9 +636,7 @@ kv_attention_kernel(AttnParams p) {
                 lane, [&](uint32_t r, uint32_t d, const float(&v)[8], float sum) { write(warp * 8u * H + r, d, v, sum); }, [](uint32_t, float, float) {});
         }
         if (!whole) {
-            // CTA c has place v if floor(c total / ctas) <= v < floor((c + 1) total / ctas)
-            const uint32_t c0 = static_cast<uint32_t>(quotient((start + 1u) * ctas - 1u, total));
-            const uint32_t c1 = static_cast<uint32_t>(quotient((start + n_blocks) * ctas - 1u, total));
+            const uint32_t c0 = sch.holder(start), c1 = sch.holder(start + n_blocks - 1u);
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -928,13 +684,17 @@ void launch(csdr_context* ctx, AttnParams& p) {
 
 template <typename T, int HD>
 void launch_rows(csdr_context* ctx, uint64_t rows, AttnParams& p) {
-    // query rows of a sequence and kv head, on average. Less than two tiles of eight: the warps share the rows; more: the keys
+    // query rows of a sequence and kv head, on average. Less than two tiles of eight: the warps share the rows; more: the keys.
+    // bf16 prompts go to tcgen05 (8 sequences of 2048, 8 kv heads of 128: 62 us for 16 rows, 64 for 128, 107 for 512; by warps 70,
+    // 90, 222; heads of 64 39, 41, 74 and 35, 64, 137); fp16 outputs are eight times as fine and keep the codes as they are.
     if (rows < 16u) {
         launch<T, HD, true, 1>(ctx, p);
     } else if constexpr (std::is_same<T, float>::value || HD > 128) {
         launch<T, HD, false, 1>(ctx, p);
-    } else {
+    } else if constexpr (std::is_same<T, __half>::value) {
         launch<T, HD, false, 2>(ctx, p);
+    } else {
+        launch_kv_attention_tc(ctx, HD, p);
     }
 }
 
@@ -942,7 +702,7 @@ void launch_rows(csdr_context* ctx, uint64_t rows, AttnParams& p) {
 
 size_t kv_attention_counters(const csdr_context* ctx) { return static_cast<size_t>(ctx->sm_count) * 4u; }
 size_t kv_attention_workspace(const csdr_context* ctx, uint32_t head_dim) {
-    // two pieces of a tile of at most 64 rows (32 for the widest heads) a CTA, at most four CTAs an SM
+    // two pieces of a tile of at most 64 rows (32 for the widest heads) a CTA, at most four CTAs an SM; or 128 rows and two CTAs
     return kv_attention_counters(ctx) * (4u + 2u * (head_dim > 128u ? 32u : 64u) * (head_dim + 4u) * 4u);
 }
 

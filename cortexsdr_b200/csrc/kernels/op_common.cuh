@@ -17,7 +17,7 @@ __device__ __forceinline__ void op_enter() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// The kernel must begin with op_enter(). cluster: CTAs of a cluster along x (1: none).
+// The kernel must begin with op_enter(), or have its two halves in an order of its own. cluster: CTAs of a cluster along x (1: none).
 template <typename... KArgs, typename... Args>
 void launch_op(csdr_context* ctx, void (*kern)(KArgs...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, Args... args) {
     cudaLaunchConfig_t cfg{};

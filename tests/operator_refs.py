@@ -46,6 +46,26 @@ def attention(q, k, v, pos, scale):
     return out
 
 
+def widened_bound(q, k, v, pos, scale):
+    """What fp16 operands cost attention(): keys off by half a step each (2^-11 of themselves) move a score by at most
+    d = 2^-11 |scale| sum |q k|, all weights together by a factor of e^(2 d) at most; values and weights are off by 2^-11 of
+    themselves, weights under 2^-14 of the largest by 2^-25 of it (the largest is at least 1 before the division by a sum of at
+    least that), where values are finite."""
+    group = q.shape[1] // k.shape[1]
+    out = np.zeros(q.shape)
+    for t in range(q.shape[0]):
+        n = pos[t] + 1
+        if n <= 0:
+            continue
+        kk, vv = (np.repeat(a[:n], group, axis=1) for a in (k, v))
+        s = np.einsum("hd,lhd->hl", q[t].astype(np.float64), kk) * scale
+        d = 2.0 ** -11 * abs(scale) * np.einsum("hd,lhd->hl", np.abs(q[t]).astype(np.float64), np.abs(kk)).max(1)
+        e = np.exp(s - s.max(1, keepdims=True))
+        size = np.einsum("hl,lhd->hd", e / e.sum(1, keepdims=True), np.abs(vv))
+        out[t] = np.expm1(2 * d + 2.0 ** -10)[:, None] * size + 2.0 ** -25 * np.abs(vv).sum(0)
+    return out
+
+
 def q4_pack(codes, steps, fmt, mins=None):
     """Blocks of a stored tensor. q4_0: codes (n, 32), steps (n,) fp16. q4_k: codes (n, 256), steps (n, 8) and mins (n, 8)
     6-bit, `steps[1]` is (n, 2) fp16 (d, dmin)."""

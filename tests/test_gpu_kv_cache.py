@@ -73,17 +73,30 @@ class Case:
         return out
 
 
-def close(out, want, tdtype, largest):
+def close(out, want, tdtype, largest, widened=None):
     """fp32 arithmetic: a score's error is at most sum |q k| scale 2^-21 (two 11-bit halves of q, fp32 sums), here
     under 64 * 16 * 2^-21 / 8 < 1e-4 of a weight for the loudest rows, an output that times the largest value; and
-    half a step of the output's type."""
+    half a step of the output's type. `widened` (bf16 prompts, whose keys, values and weights are operands in fp16): what their
+    roundings come to, operator_refs.widened_bound; on the whole such an output is bf16's: its roundings are spread over
+    half a step, 2^-8 / sqrt(3) of the value at most, and a quarter of that again."""
     half = 2.0 ** -24 if tdtype == torch.float32 else torch.finfo(tdtype).eps / 2
     bound = half * np.abs(want) + 1e-4 * largest
+    if widened is not None:
+        bound = bound + (1 + half) * widened
     err = np.abs(out.to(torch.float64).cpu().numpy() - want)
     assert (err <= bound).all(), f"off by up to {np.nanmax(err - bound)} past the bound"
     if tdtype == torch.float32:
         # the errors of many terms do not all point one way: over all rows, fp32's own
         assert np.linalg.norm(err) <= 4e-6 * np.linalg.norm(want) + 1e-30
+    if widened is not None:
+        assert np.linalg.norm(err) <= 1.25 * 2.0 ** -8 / 3 ** 0.5 * np.linalg.norm(want)
+
+
+def bound_of(c, fresh, qh, hd, q, k, v, pos, scale):
+    """widened_bound where the call's operands are widened: bf16, heads of at most 128, sixteen query rows of a kv head a sequence."""
+    if c.tdtype != torch.bfloat16 or hd > 128 or sum(fresh) * (qh // c.kvh) // len(fresh) < 16:
+        return None
+    return ref.widened_bound(q.to(torch.float64).numpy(), k, v, pos, scale)
 
 
 SHAPES = [
@@ -242,8 +255,9 @@ def test_attention_matches_the_definition(ctx, shape, dtype):
     at = 0
     for s, n in enumerate(fresh):
         if n:
-            want = ref.attention(q[s].to(torch.float64).numpy(), k[s], v[s], lengths[s] - n + np.arange(n), hd ** -0.5)
-            close(out[at:at + n], want, c.tdtype, np.abs(v[s]).max())
+            pos = lengths[s] - n + np.arange(n)
+            want = ref.attention(q[s].to(torch.float64).numpy(), k[s], v[s], pos, hd ** -0.5)
+            close(out[at:at + n], want, c.tdtype, np.abs(v[s]).max(), bound_of(c, fresh, qh, hd, q[s], k[s], v[s], pos, hd ** -0.5))
         at += n
     assert (out[at:] == 7).all()             # rows behind the last sequence
 
@@ -262,8 +276,9 @@ def test_attention_of_many_sequences(ctx, n, most_new, dtype):
     at = 0
     for s, f in enumerate(fresh):
         if f:
-            want = ref.attention(q[s].to(torch.float64).numpy(), k[s], v[s], lengths[s] - f + np.arange(f), 0.125)
-            close(out[at:at + f], want, c.tdtype, max(1.0, np.abs(v[s]).max()))
+            pos = lengths[s] - f + np.arange(f)
+            want = ref.attention(q[s].to(torch.float64).numpy(), k[s], v[s], pos, 0.125)
+            close(out[at:at + f], want, c.tdtype, max(1.0, np.abs(v[s]).max()), bound_of(c, fresh, qh, 64, q[s], k[s], v[s], pos, 0.125))
         at += f
 
 
@@ -496,3 +511,105 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_cache_usable(dtype, fre
     assert torch.equal(c.attend(q, 8), want)
     c.cache.close()
     own.close()
+
+
+def prompts(c, qh, scale=None, keep=None, **kw):
+    """The call's rows against the definition; keep: positions of sequence 0 that have a page."""
+    hd = c.hd
+    scale = hd ** -0.5 if scale is None else scale
+    qs = [c.values((f, qh, hd)) for f in c.fresh]
+    out = c.attend(c.rows(qs, c.tail), qh, scale=scale, **kw)
+    k, v = c.held()
+    at = 0
+    for s, (n, f) in enumerate(zip(c.lengths, c.fresh)):
+        pos = n - f + np.arange(f)
+        kk, vv = k[s], v[s]
+        if s == 0 and keep is not None:
+            kk, vv, pos = kk[keep], vv[keep], np.array([(keep <= t).sum() - 1 for t in pos])
+        if f:
+            want = ref.attention(qs[s].to(torch.float64).numpy(), kk, vv, pos, scale)
+            close(out[at:at + f], want, c.tdtype, max(1.0, np.nanmax(np.abs(vv), initial=0)), bound_of(c, c.fresh, qh, hd, qs[s], kk, vv, pos, scale))
+        at += f
+    assert (out[at:] == 7).all()
+    return out
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lengths,fresh,kvh,qh,page", [
+    ([128], [128], 1, 1, 16),                      # a tile of rows, two blocks of keys
+    ([129, 1, 0, 64], [129, 1, 0, 64], 2, 6, 32),  # whole prompts, an idle sequence
+    ([70, 400, 65], [17, 130, 65], 1, 7, 64),      # rows that end inside a tile, keys inside a block
+    ([3000], [24], 2, 8, 256),                     # few tiles, cut along the keys
+    ([40] * 70, [3] * 70, 2, 16, 16),              # more sequences than a warp has lanes
+])
+def test_bf16_prompts(ctx, lengths, fresh, kvh, qh, page, hd):
+    c = Case(ctx, lengths, fresh, kvh, hd, page, seed=len(lengths) + hd, dtype="bf16", spare=1, tail=5)
+    c.store()
+    prompts(c, qh)
+    prompts(c, qh, scale=-0.03)
+
+
+def test_bf16_prompts_see_what_has_a_place(ctx):
+    c = Case(ctx, [300, 64], [100, 64], 2, 128, 16, seed=21, dtype="bf16", tail=2)
+    c.store()
+    c.pages[0, 2], c.pages[0, 7], c.pages[0, 13] = -1, c.n_pages + 5, -9
+    keep = np.array([t for t in range(300) if t // 16 not in (2, 7, 13)])
+    prompts(c, 8, keep=keep)
+    # lengths that are less than the new rows: the first see nothing
+    c.lengths, c.fresh = [20, 0], [50, 30]
+    q = [c.values((f, 8, 128)) for f in c.fresh]
+    out = c.attend(c.rows(q), 8)
+    assert (out[:30] == 0).all() and (out[50:] == 0).all() and (out[30:50] != 0).any(-1).all()
+
+
+def test_bf16_prompts_do_not_see_later_tokens(ctx):
+    # NaN among values that some rows of a tile see and others do not, in one group of 64; then among keys
+    c = Case(ctx, [150], [150], 1, 128, 64, seed=22, dtype="bf16")
+    c.v[0][100, 0, 70] = float("nan")
+    c.k[0][120, 0, 3] = float("inf")
+    c.store()
+    k, v = c.held()
+    q = [c.values((150, 4, 128))]
+    out = c.attend(c.rows(q), 4)
+    want = ref.attention(q[0][:100].to(torch.float64).numpy(), k[0], v[0], np.arange(100), 128 ** -0.5)
+    close(out[:100], want, torch.bfloat16, np.abs(v[0][:100]).max(), ref.widened_bound(q[0][:100].to(torch.float64).numpy(), k[0], v[0], np.arange(100), 128 ** -0.5))
+    assert torch.isfinite(out[100:120, :, :64]).all() and torch.isnan(out[100:, :, 64:]).all() and torch.isnan(out[120:]).all()
+
+
+@pytest.mark.parametrize("vscale", [1e-6, 3000.0, 65504.0])
+def test_bf16_prompts_of_any_magnitude(ctx, vscale):
+    c = Case(ctx, [200], [60], 2, 64, 32, seed=23, dtype="bf16")
+    c.v[0] = (c.v[0] / c.v[0].abs().max() * vscale).to(torch.bfloat16)
+    c.k[0] = c.k[0] / 1024
+    c.store()
+    q = [c.values((60, 8, 64)) * 1e20, c.values((60, 8, 64)) * 0]
+    k, v = c.held()
+    for x in q:
+        out = c.attend(c.rows([x]), 8, scale=1e-18)
+        pos = 140 + np.arange(60)
+        want = ref.attention(x.to(torch.float64).numpy(), k[0], v[0], pos, 1e-18)
+        bound = ref.widened_bound(x.to(torch.float64).numpy(), k[0], v[0], pos, 1e-18) + 2.0 ** -8 * np.abs(want) + 2.0 ** -24
+        assert (np.abs(out.to(torch.float64).cpu().numpy() - want) <= bound).all()
+
+
+def test_bf16_prompts_strides_layers_and_odd_offsets(ctx):
+    c = Case(ctx, [90, 40], [70, 40], 2, 64, 16, seed=24, layers=2, dtype="bf16")
+    c.store(layer=1)
+    rows = torch.zeros(110 * 6 * 64 + 200, dtype=torch.bfloat16, device="cuda")
+    out = torch.full_like(rows, 7.0)
+    q = c.values((110, 4, 64)).cuda()
+    k, v = c.held()
+    for off, stride in ((0, 6 * 64), (1, 4 * 64 + 1)):
+        rows[off:off + 110 * stride].view(110, stride)[:, :256] = q.view(110, 256)
+        torch.cuda.synchronize()
+        c.cache.attention(c.batch(c.lengths, c.fresh), rows.data_ptr() + 2 * off, 1, 4, out.data_ptr() + 2 * off, q_stride=stride, out_stride=stride, layer=1)
+        ctx.synchronize()
+        got = out[off:off + 110 * stride].view(110, stride)
+        at = 0
+        for s, f in enumerate(c.fresh):
+            pos = c.lengths[s] - f + np.arange(f)
+            x = q[at:at + f].cpu().to(torch.float64).numpy()
+            close(got[at:at + f, :256].reshape(f, 4, 64), ref.attention(x, k[s], v[s], pos, 0.125), torch.bfloat16, 16.0, ref.widened_bound(x, k[s], v[s], pos, 0.125))
+            at += f
+        assert (got[:, 256:] == 7).all()
+        out.fill_(7.0)
