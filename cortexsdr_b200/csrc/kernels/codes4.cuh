@@ -45,6 +45,11 @@ __device__ __forceinline__ void widen_codes(uint32_t w, uint32_t (&r)[4]) {
 }
 constexpr int kCodeShift = 18;
 constexpr uint32_t kEights = 0x02000200u;      // code 8, twice
+// Widened codes without their 8: exact.
+__device__ __forceinline__ uint32_t less_eight(uint32_t codes) {
+    const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&codes), __half2half2(__ushort_as_half(0x8200)));
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 // Pairs of fp32 values, one packed operation each.
 typedef unsigned long long f32x2;

@@ -9,8 +9,10 @@
 //            of query rows and eight of what the roundings left
 //   output   sum over groups of (p step) . (code - 8) + sum p (minimum + 8 step)   transposed, p step: 8 columns
 // Rounding and rest carry 22 bits, sums are fp32's. A row's q is scaled by a power of two to use fp16's range, p step
-// likewise by the largest step met. The 8 comes off in every piece (by one more product, of p step with eights): the
-// matrix units cut sums off instead of rounding them, and sums of one sign drift (1e-5 of an output over 5000 keys).
+// likewise by the largest step met. The matrix units cut sums off instead of rounding them, and sums of one sign drift (1e-5 of an
+// output over 5000 keys): so the 8 comes off. For 16-bit outputs that is one more product a piece, of p step with eights; for
+// fp32 ones it comes off every code, keys' too, and a piece's sums stand by themselves until they are added, rounded (16 sequences
+// of 1024: 4.4e-7 of an output and 33.3 us, against 1.2e-6 and 31.0 as 16-bit outputs have it).
 // tcgen05 wants the codes widened into shared memory first, which pays for prompts whose outputs round coarsely: bf16
 // (kv_attention_tc.cu).
 //
@@ -41,6 +43,7 @@ struct Rows {
     static constexpr uint32_t W = HD / 32, G = HD / 64;
     static constexpr bool kFine = std::is_same<T, float>::value;
     static constexpr bool kOnce = H == 2 || std::is_same<T, __nv_bfloat16>::value;      // bf16 rounds eight times as coarsely as p step
+    static_assert(!kFine || H == 1, "sixteen rows are for 16-bit outputs");
     static constexpr float kOdd = kFine ? 1.0f : 16.0f;      // odd pairs of codes count one in kOdd
     static constexpr bool kShared = HD >= 128;     // q fragments in shared memory: the registers go to the outputs
     static constexpr uint32_t kMetaBytes = 2u * G * 16u * 16u;      // of a piece, widened
@@ -178,7 +181,7 @@ struct Rows {
         {
             const uint32_t pr = lane & 15u, of_values = lane >> 4;
             const uint8_t* from = block + (pr >> 3) * (18u * HD) + (16u + of_values) * HD + (pr & 7u) * 8u;
-            const float mid = of_values ? 8.0f : 0.0f;
+            const float mid = kFine || of_values ? 8.0f : 0.0f;
 #pragma unroll
             for (uint32_t u = 0; u < G; ++u) {
                 uint2 w = *reinterpret_cast<const uint2*>(from + 64u * u);
@@ -224,6 +227,10 @@ struct Rows {
                 for (uint32_t nt = 0; nt < 4u; ++nt) {
                     uint32_t r[4];
                     widen_codes<kFine>(i ? w[nt].y : w[nt].x, r);
+                    if constexpr (kFine) {
+#pragma unroll
+                        for (uint32_t n = 0; n < 4u; ++n) r[n] = less_eight(r[n]);
+                    }
                     if (i == 0u) mma16816_first(acc[nt], f[0][0], f[0][1], f[0][2], f[0][3], r[0], r[1]);
                     else mma16816(acc[nt], f[0][0], f[0][1], f[0][2], f[0][3], r[0], r[1]);
                     mma16816(acc[nt], f[1][0], f[1][1], f[1][2], f[1][3], r[2], r[3]);
@@ -337,7 +344,7 @@ struct Rows {
                 }
             }
 #pragma unroll
-            for (uint32_t h = 0; h < H; ++h) {
+            for (uint32_t h = 0; h < (kFine ? 0u : H); ++h) {
                 mma16816_first(eight[h], kEights, kEights, kEights, kEights, hi[h][0], hi[h][1]);
                 mma16816(eight[h], kEights, kEights, kEights, kEights, hi[h][2], hi[h][3]);
                 if constexpr (!kOnce) {
@@ -345,20 +352,44 @@ struct Rows {
                     mma16816(eight[h], kEights, kEights, kEights, kEights, lo[2], lo[3]);
                 }
             }
+            if constexpr (kFine) {
+                // a piece's sums by themselves: what is cut off is cut off them, and they are added rounded
+                float z[4][4];
+#pragma unroll
+                for (uint32_t b = 0; b < 2u; ++b) {
+                    uint32_t r[4][4];
+                    values_at(block, b, u, t, g, r);
+#pragma unroll
+                    for (uint32_t k = 0; k < 4u; ++k)
+#pragma unroll
+                        for (uint32_t n = 0; n < 4u; ++n) r[k][n] = less_eight(r[k][n]);
+#pragma unroll
+                    for (uint32_t n = 0; n < 4u; ++n) {
+                        if (b == 0u) mma16816_first(z[n], r[0][n], r[1][n], r[2][n], r[3][n], lo[2u * b], lo[2u * b + 1u]);
+                        else mma16816(z[n], r[0][n], r[1][n], r[2][n], r[3][n], lo[2u * b], lo[2u * b + 1u]);
+                        mma16816(z[n], r[0][n], r[1][n], r[2][n], r[3][n], hi[0][2u * b], hi[0][2u * b + 1u]);
+                    }
+                }
+#pragma unroll
+                for (uint32_t n = 0; n < 4u; ++n) {
+                    const float2 x = unpack2(add2(pack2(o[0][u][n][0], o[0][u][n][1]), pack2(z[n][0], z[n][1])));
+                    const float2 y = unpack2(add2(pack2(o[0][u][n][2], o[0][u][n][3]), pack2(z[n][2], z[n][3])));
+                    o[0][u][n][0] = x.x;
+                    o[0][u][n][1] = x.y;
+                    o[0][u][n][2] = y.x;
+                    o[0][u][n][3] = y.y;
+                }
+                continue;
+            }
 #pragma unroll
             for (uint32_t b = 0; b < 2u; ++b) {
-                const uint8_t* v0 = block + b * (18u * HD) + 8u * HD + t * HD + g * (HD / 8) + 8u * u;
-                const uint2 w0 = *reinterpret_cast<const uint2*>(v0), w1 = *reinterpret_cast<const uint2*>(v0 + 4u * HD);
-                uint32_t r0[4], r1[4], r2[4], r3[4];
-                widen_codes<kFine>(w0.x, r0);
-                widen_codes<kFine>(w0.y, r1);
-                widen_codes<kFine>(w1.x, r2);
-                widen_codes<kFine>(w1.y, r3);
+                uint32_t r[4][4];
+                values_at(block, b, u, t, g, r);
 #pragma unroll
                 for (uint32_t n = 0; n < 4u; ++n) {
 #pragma unroll
-                    for (uint32_t h = 0; h < H; ++h) mma16816(o[h][u][n], r0[n], r1[n], r2[n], r3[n], hi[h][2u * b], hi[h][2u * b + 1u]);
-                    if constexpr (!kOnce) mma16816(o[0][u][n], r0[n], r1[n], r2[n], r3[n], lo[2u * b], lo[2u * b + 1u]);
+                    for (uint32_t h = 0; h < H; ++h) mma16816(o[h][u][n], r[0][n], r[1][n], r[2][n], r[3][n], hi[h][2u * b], hi[h][2u * b + 1u]);
+                    if constexpr (!kOnce) mma16816(o[0][u][n], r[0][n], r[1][n], r[2][n], r[3][n], lo[2u * b], lo[2u * b + 1u]);
                 }
             }
 #pragma unroll
@@ -368,6 +399,15 @@ struct Rows {
                 for (uint32_t h = 0; h < H; ++h) add_tile(o[h][u][n], pack2(eight[h][0], eight[h][1]), pack2(times, times));
             }
         }
+    }
+    // Words of block b's pairs of tokens 2t, 2t + 8 as pairs of codes: values 64 u + 8 g + n and + 4 + n.
+    static __device__ __forceinline__ void values_at(const uint8_t* block, uint32_t b, uint32_t u, uint32_t t, uint32_t g, uint32_t (&r)[4][4]) {
+        const uint8_t* v0 = block + b * (18u * HD) + 8u * HD + t * HD + g * (HD / 8) + 8u * u;
+        const uint2 w0 = *reinterpret_cast<const uint2*>(v0), w1 = *reinterpret_cast<const uint2*>(v0 + 4u * HD);
+        widen_codes<kFine>(w0.x, r[0]);
+        widen_codes<kFine>(w0.y, r[1]);
+        widen_codes<kFine>(w1.x, r[2]);
+        widen_codes<kFine>(w1.y, r[3]);
     }
     __device__ __forceinline__ void piece(const uint8_t* block, int32_t tok0, uint32_t there, uint32_t lane, const uint4* shared, uint8_t* meta) {
         if (there != 3u || tok0 + 32 > least) keys32<true>(block, tok0, there, lane, shared, meta);

@@ -11,8 +11,9 @@
 // instead of 128). Two CTAs an SM fill what is left. Work is cut as there (kv_attention.cuh).
 //
 // 3 sequences of 2048 with 512 new tokens, 32 query heads over 8 of 128: 114 us, 332 TFLOP/s (by warps 245 us). The products
-// are 42 of it (a product of 64 columns takes 75 cycles, of 128 columns 121), widening and exponentials as much again each; a
-// block passes through the three one after the other, and two CTAs overlap them only in part. Tried and slower: 256 rows a CTA
+// are 42 of it (one of 64 columns takes 75 cycles, of 128 columns 121: 1080 a block); a warp widens its part of a block in 1400
+// cycles and has a row's weights in 960. A block passes through the three one after the other, and two CTAs overlap them only
+// in part. Tried and slower: 256 rows a CTA
 // (129 us: one CTA's phases have nobody beside them), keys published before values (122 us).
 #include "codes4.cuh"
 #include "kv_attention.cuh"
