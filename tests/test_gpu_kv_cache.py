@@ -613,3 +613,49 @@ def test_bf16_prompts_strides_layers_and_odd_offsets(ctx):
             at += f
         assert (got[:, 256:] == 7).all()
         out.fill_(7.0)
+
+
+def test_captured_bf16_prompts_follow_new_lengths():
+    """A graph of append and attention for pieces of prompts, replayed back to back as sequences grow; two caches' graphs in turn."""
+    side = torch.cuda.Stream()
+    own = cs.Context(0, side.cuda_stream)
+    kvh, qh, hd, page, piece, n = 2, 8, 128, 64, 48, 3
+    rng = np.random.default_rng(31)
+    runs = []
+    for _ in range(2):
+        per = 4
+        cache = cs.KVCache(n * per, page, kvh, hd, rope_theta=THETA, ctx=own)
+        first = torch.tensor([0, piece, piece, 2 * piece], dtype=torch.int32, device="cuda")      # the second sequence idles
+        length = torch.zeros(n, dtype=torch.int32, device="cuda")
+        pages = torch.tensor(rng.permutation(n * per).reshape(n, per), dtype=torch.int32, device="cuda")
+        b = cs.KVBatch(n, 2 * piece, first.data_ptr(), length.data_ptr(), pages.data_ptr(), per)
+        k, v, q = (torch.zeros(2 * piece, h, hd, dtype=torch.bfloat16, device="cuda") for h in (kvh, kvh, qh))
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+            cache.append(b, k.data_ptr(), v.data_ptr(), 1, rotate=False)
+            cache.attention(b, q.data_ptr(), 1, qh, out.data_ptr())
+        runs.append((cache, b, first, length, pages, k, v, q, out, g, [], []))
+    for step in range(4):
+        for cache, b, first, length, pages, k, v, q, out, g, ks, vs in runs:
+            with torch.cuda.stream(side):
+                for t in (k, v, q):
+                    t.copy_(torch.tensor(rng.normal(0, 1, t.shape), dtype=torch.bfloat16))
+                length.copy_(torch.tensor([piece * (step + 1), 0, piece * (step + 1)], dtype=torch.int32))
+                g.replay()
+            ks.append(k.cpu())
+            vs.append(v.cpu())
+        own.synchronize()
+        for cache, b, first, length, pages, k, v, q, out, g, ks, vs in runs:
+            for i in range(2):
+                rows = slice(i * piece, (i + 1) * piece)
+                hk, hv = (ref.held(torch.cat([t[rows] for t in src]).to(torch.float64).numpy()) for src in (ks, vs))
+                pos = piece * step + np.arange(piece)
+                x = q[rows].cpu().to(torch.float64).numpy()
+                close(out[rows], ref.attention(x, hk, hv, pos, hd ** -0.5), torch.bfloat16, 5.0, ref.widened_bound(x, hk, hv, pos, hd ** -0.5))
+    for cache, *_, g, _, _ in runs:
+        del g
+        cache.close()
+    runs.clear()
+    own.close()
