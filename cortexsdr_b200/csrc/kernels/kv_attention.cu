@@ -724,12 +724,16 @@ void launch(csdr_context* ctx, AttnParams& p) {
 
 template <typename T, int HD>
 void launch_rows(csdr_context* ctx, uint64_t rows, AttnParams& p) {
-    // query rows of a sequence and kv head, on average. Less than two tiles of eight: the warps share the rows; more: the keys.
-    // bf16 prompts go to tcgen05 (8 sequences of 2048, 8 kv heads of 128: 62 us for 16 rows, 64 for 128, 107 for 512; by warps 70,
-    // 90, 222; heads of 64 39, 41, 74 and 35, 64, 137); fp16 outputs are eight times as fine and keep the codes as they are.
-    if (rows < 16u) {
+    // query rows of a sequence and kv head, on average. Few: the warps share eight rows and have keys of their own, so that a
+    // tile's keys are spread over four warps. Many: each has rows of its own and keys are shared. 4 sequences of 2048, 8 kv heads
+    // of 128, us for 64, 128, 512, 2048 rows:
+    //   fp32   49, 72, 203, 680 and 51, 81, 212, 647 (heads of 256: 74, 119, 388, 1358 and 96, 141, 401, 1286)
+    //   fp16   43, 64, 177, 585 and 57, 75, 147, 363
+    //   bf16   41, 58, 160, 526 and, on tcgen05, 51, 53, 76, 164 (fp16 outputs are eight times as fine and keep their codes)
+    constexpr bool kWide = std::is_same<T, float>::value || HD > 128;
+    if (rows < (kWide ? 1024u : std::is_same<T, __half>::value ? 192u : 96u)) {
         launch<T, HD, true, 1>(ctx, p);
-    } else if constexpr (std::is_same<T, float>::value || HD > 128) {
+    } else if constexpr (kWide) {
         launch<T, HD, false, 1>(ctx, p);
     } else if constexpr (std::is_same<T, __half>::value) {
         launch<T, HD, false, 2>(ctx, p);

@@ -541,9 +541,9 @@ CSDR_API int csdr_kv_cache_read_device_async(csdr_kv_cache* cache, uint32_t laye
  * out = softmax(scale * q k^T) v (multi_head_attention, kernels/attention_kernels.cpp:26-113), a new token
  * seeing every token up to its own position. q and out: n_tokens x q_heads x head_dim of `dtype`, strides
  * as above; out must not overlap q; scale 0: 1 / sqrt(head_dim). A token that sees nothing gets zeros.
- * Scores, weights and sums in fp32; bf16 rows, sixteen and more of a kv head a sequence on average and heads of 64 or
- * 128, take keys, values and weights as operands in fp16 (2^-11 of themselves; sums in fp32). Calls on one cache share its workspace: they run one after
- * the other, graphs that were captured from them too. */
+ * Scores, weights and sums in fp32; of bf16 prompts (heads of 64 or 128, 96 query rows and more of a kv head a
+ * sequence on average) keys, values and weights are operands in fp16, 2^-11 of themselves, and sums fp32. Calls on one cache
+ * share its workspace: they run one after the other, graphs that were captured from them too. */
 CSDR_API int csdr_kv_cache_attention_device_async(csdr_kv_cache* cache, uint32_t layer,
                                                   const csdr_kv_batch* batch, const void* q_dev,
                                                   size_t q_stride, int dtype, uint32_t q_heads, float scale,

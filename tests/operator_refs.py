@@ -66,6 +66,25 @@ def widened_bound(q, k, v, pos, scale):
     return out
 
 
+def steps_bound(q, k, v, pos, scale):
+    """What it costs attention() to round a weight times a step to fp16 (2^-11 of itself): an output is a sum of these times
+    (code - 8), |code - 8| <= 8, and a group's fifteen steps are at most twice its largest value: 2^-11 16 / 15 of that, weighted.
+    (Half as much again: a step is rounded up by 2^-11 at most, held values may lie inside the range.)"""
+    group = q.shape[1] // k.shape[1]
+    out = np.zeros(q.shape)
+    most = np.abs(v.reshape(*v.shape[:2], -1, 64)).max(-1, keepdims=True)
+    most = np.broadcast_to(most, (*most.shape[:3], 64)).reshape(v.shape)
+    for t in range(q.shape[0]):
+        n = pos[t] + 1
+        if n <= 0:
+            continue
+        kk, mm = (np.repeat(a[:n], group, axis=1) for a in (k, most))
+        s = np.einsum("hd,lhd->hl", q[t].astype(np.float64), kk) * scale
+        e = np.exp(s - s.max(1, keepdims=True))
+        out[t] = 1.5 * 2.0 ** -11 * 16 / 15 * np.einsum("hl,lhd->hd", e / e.sum(1, keepdims=True), mm)
+    return out
+
+
 def q4_pack(codes, steps, fmt, mins=None):
     """Blocks of a stored tensor. q4_0: codes (n, 32), steps (n,) fp16. q4_k: codes (n, 256), steps (n, 8) and mins (n, 8)
     6-bit, `steps[1]` is (n, 2) fp16 (d, dmin)."""
