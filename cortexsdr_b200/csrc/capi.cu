@@ -212,7 +212,7 @@ void* csdr_context::scratch_get(int slot, size_t bytes) {
 }
 
 void csdr_context::encoder_scratch_trim() noexcept {
-    for (int slot = kEncoderScratch; slot < kScratchSlots; ++slot)
+    for (int slot = kEncoderScratch; slot < kQ4Scratch; ++slot)
         if (scratch[slot] && scratch[slot]->bytes > (256u << 20)) {
             (void)cudaStreamSynchronize(stream);   // work of a call that ended early may still use it
             scratch[slot].reset();

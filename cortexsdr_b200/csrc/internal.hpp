@@ -125,11 +125,11 @@ struct csdr_context {
     // call needs more: 0 Dx, 1 tile products, 2 materialised W, 3 host staging, 4 fused-GEMV partials,
     // 5 activation planes / wait self-test, 6 GEMV queue, 7 dense product before re-tiling. The rest is the
     // encoder's, which no graph holds: 8 dictionary, 9 codes and small arrays, 10 projections, 11 the
-    // matrix, 12 its tiles.
-    static constexpr int kEncoderScratch = 8, kScratchSlots = 13;
+    // matrix, 12 its tiles. But 13: the fragments of 4-bit products, which move their own slot only.
+    static constexpr int kEncoderScratch = 8, kQ4Scratch = 13, kScratchSlots = 14;
     csdr::DevPtr scratch[kScratchSlots];
     void* scratch_get(int slot, size_t bytes);
-    std::vector<csdr::DevPtr> held;             // scratch that captured 4-bit products use: a larger call moves the slot, not these
+    std::vector<csdr::DevPtr> held;             // kQ4Scratch as captured products use it: a larger call moves the slot, not these
     void encoder_scratch_trim() noexcept;       // at the end of an encoder call: keeps up to 256 MB a slot
     // What a segment keeps although there is a form that does without it (a rebuilt weight, coefficient
     // entries). Null where all of them together would pass the budget or the device has no room.

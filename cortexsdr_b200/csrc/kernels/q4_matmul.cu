@@ -490,8 +490,9 @@ void launch(csdr_context* ctx, Q4Params p) {
     size_t each = std::max<size_t>(1, std::min<size_t>(tiles, (16u << 20) / tile_bytes));
     bool ahead = items > 2u * kThreads;
     if (ahead && ctx->capturing()) {
-        if (!ctx->scratch[5] || ctx->scratch[5]->bytes < each * tile_bytes) ahead = false;
-        else if (ctx->held.empty() || ctx->held.back() != ctx->scratch[5]) ctx->held.push_back(ctx->scratch[5]);      // for the graph
+        const DevPtr& now = ctx->scratch[csdr_context::kQ4Scratch];
+        if (!now || now->bytes < each * tile_bytes) ahead = false;
+        else if (ctx->held.empty() || ctx->held.back() != now) ctx->held.push_back(now);      // for the graph
     }
     if (!ahead) each = tiles;
     const Q4Args all = p.a;
@@ -501,7 +502,7 @@ void launch(csdr_context* ctx, Q4Params p) {
         p.a.y = all.y + tok * all.y_token;
         p.a.batch = std::min(all.batch - tok, n * S::kTokens);
         if (ahead) {
-            p.planes = static_cast<uint8_t*>(ctx->scratch_get(5, each * tile_bytes));
+            p.planes = static_cast<uint8_t*>(ctx->scratch_get(csdr_context::kQ4Scratch, each * tile_bytes));
             constexpr uint32_t kUnits = 2;
             LaunchScope ls(ctx, KC_Q4);
             launch_op(ctx, q4_stage_kernel<T, FMT, NT>, dim3((p.w.n_units + kUnits - 1u) / kUnits, static_cast<unsigned>(n)), kThreads, 0, 1, p, kUnits);

@@ -5,6 +5,7 @@ import torch
 
 import cortexsdr_b200 as cs
 from tests import operator_refs as ref
+from tests import synth
 
 pytestmark = pytest.mark.gpu
 DTYPES = {"f32": (torch.float32, 0), "bf16": (torch.bfloat16, 1), "f16": (torch.float16, 2)}
@@ -233,4 +234,35 @@ def test_a_wait_that_runs_out_is_reported():
     own.set_wait_limits()
     np.testing.assert_array_equal(run(w, x, 1, 512, own), want)
     w.close()
+    own.close()
+
+
+def test_a_captured_product_of_another_kind_keeps_its_scratch():
+    """A graph of a product with a compressed weight, whose activations go through scratch of the context; then the largest 4-bit
+    product so far, whose fragments take up to 16 MB; then the graph again."""
+    rng = np.random.default_rng(13)
+    side = torch.cuda.Stream()
+    own = cs.Context(0, side.cuda_stream)
+    seg = cs.Segment.from_payload(synth.hsdr_payload(384, 1024, n_atoms=128, k=6, seed=4), own)
+    big, dense = ref.q4_weight(rng, 64, 16384, "q4_0")
+    larger = cs.Q4Weight.from_payload(big, "q4_0", 64, 16384, own)
+    x, y = torch.tensor(rng.normal(0, 1, (16, 1024)), dtype=torch.float32).cuda(), torch.zeros(16, 384, device="cuda")
+    x2, y2 = torch.tensor(rng.normal(0, 1, (128, 16384)), dtype=torch.float32).cuda(), torch.empty(128, 64, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        seg.matmul_device(x.data_ptr(), 0, 1, 16, y.data_ptr(), 1)
+        side.synchronize()
+        first = y.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            seg.matmul_device(x.data_ptr(), 0, 1, 16, y.data_ptr(), 1)
+        larger.matmul_device(x2.data_ptr(), 0, 1, 128, y2.data_ptr(), 1)
+        y.zero_()
+        g.replay()
+    side.synchronize()
+    assert torch.equal(y, first)
+    check(y2.to(torch.float64).cpu().numpy(), x2.cpu(), dense)
+    del g
+    larger.close()
+    seg.close()
     own.close()
