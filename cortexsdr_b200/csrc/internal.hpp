@@ -3,8 +3,10 @@
 
 #include <cuda_runtime.h>
 
+#include <array>
 #include <atomic>
 #include <cstdint>
+#include <map>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -176,6 +178,8 @@ struct csdr_context {
     // to a device; a process may hold contexts on several).
     void opt_in_smem(const void* kernel, size_t bytes);               // raises the opt-in when bytes needs it
     std::unordered_map<const void*, std::pair<size_t, int>> occupancy; // kernel -> (smem asked, CTAs per SM)
+    uint32_t q4_resident[2][8] = {};                                   // 4-bit products: [CTAs an SM - 1][cluster size - 1] -> clusters resident
+    std::map<std::array<size_t, 3>, std::array<uint32_t, 6>> q4_cuts;  // and how they are cut, by sizes (q4_matmul.cu)
     bool tma_attrs_set = false;
     int tma_max_cluster = 8;
     std::unordered_map<uint64_t, int> cluster_fit;                    // (cluster size, smem) -> clusters resident

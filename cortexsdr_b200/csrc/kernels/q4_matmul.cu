@@ -3,6 +3,8 @@
 //   q4_k   W = (d sc) code - dmin mn, (sc, mn) 6 bits for 32 columns, (d, dmin) fp16 for 256
 // as decodeSupportedGGUFQuantized reads them (SparseInferenceEngine.cpp:276-469).
 #include <algorithm>
+#include <array>
+#include <cmath>
 
 #include <cooperative_groups.h>
 
@@ -100,8 +102,6 @@ struct Q4Shape {
     static constexpr uint32_t kStageBytes = kBacksAt + kColumns * 4u;
     // partial results of all ranks (runs of 32, so up to a run a rank more than there are), twice
     static constexpr uint32_t kSums = kRowsBlock * kTokens + 8u * 32u, kSumBytes = 2u * kSums * 4u;
-    // units whose activations fit beside the partial results, with n CTAs an SM
-    static constexpr uint32_t staged(uint32_t n) { return ((n == 2u ? 104u : 208u) * 1024u - kSumBytes) / kStageBytes; }
 };
 
 // Eight neighbouring columns of a token as they lie in memory; what lies behind the matrix is zero.
@@ -451,57 +451,117 @@ q4_matmul_kernel(Q4Params p) {
     if (!live && lane == 0) atomicExch(p.status, 1);      // results are wrong, and said to be
 }
 
-template <typename T, int FMT, int NT, bool ONE = false>
-void launch(csdr_context* ctx, Q4Params p) {
-    using S = Q4Shape<FMT, NT, std::is_same<T, float>::value>;
-    p.n_blocks = (p.w.rows + kRowsBlock - 1u) / kRowsBlock;
-    // Cut the columns so that the CTA with most to do has least: blocks in turn, each its units and about two more for the
-    // join. Two CTAs an SM, or one with all of the shared memory (half the warps: a CTA alone is little faster); activations that
-    // do not fit at a time are staged anew for every block.
-    uint32_t ranks = 1, per_sm = 2;
-    float least = 1e30f;
-    for (uint32_t n = 2; n >= 1; --n) {
-        const uint32_t slots = static_cast<uint32_t>(ctx->sm_count) * n, fits = S::staged(n);
-        for (uint32_t r = 1; r <= 8u && r <= p.w.n_units; ++r) {
-            const uint32_t units = (p.w.n_units + r - 1u) / r, clusters = slots / r, turns = (p.n_blocks + clusters - 1u) / clusters;
-            const float cost = static_cast<float>(turns * (units * (units > fits ? 4u : 1u) + 2u)) * (n == 2u ? 1.0f : 0.9f);
-            if (cost < least) {
-                least = cost;
-                ranks = r;
-                per_sm = n;
-            }
-        }
+// Sizes of Q4Shape as the host has them.
+struct Sizes {
+    uint32_t tokens, stage_bytes, sum_bytes, groups;
+    constexpr Sizes(bool split, int format, uint32_t nt)
+        : tokens(nt * (split ? 4u : 8u)), stage_bytes(q4_unit_cols(format) / 32u * nt * 8u * 68u + nt * 32u),
+          sum_bytes(2u * (kRowsBlock * tokens + 8u * 32u) * 4u), groups(q4_unit_cols(format) / 32u) {}
+    // units whose activations fit beside the partial results, with n CTAs an SM
+    uint32_t staged(uint32_t n) const { return ((n == 2u ? 104u : 208u) * 1024u - sum_bytes) / stage_bytes; }
+};
+
+// Clusters of r CTAs that are resident at once, n CTAs an SM (GPCs do not divide by every r).
+uint32_t resident(csdr_context* ctx, uint32_t n, uint32_t r) {
+    uint32_t& known = ctx->q4_resident[n - 1u][r - 1u];
+    if (!known && r == 1u) known = static_cast<uint32_t>(ctx->sm_count) * n;
+    if (!known) {
+        auto kern = q4_matmul_kernel<float, 0, 1, false>;
+        const size_t smem = (n == 2u ? 104u : 208u) * 1024u;
+        ctx->opt_in_smem(reinterpret_cast<const void*>(kern), smem);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(r * static_cast<uint32_t>(ctx->sm_count));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = r;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        CSDR_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
+        known = static_cast<uint32_t>(std::max(clusters, 1));
     }
-    p.units_rank = (p.w.n_units + ranks - 1u) / ranks;
-    p.units_staged = std::min(p.units_rank, S::staged(per_sm));
+    return known;
+}
+
+// Token tiles a launch whose fragments are made ahead: what 16 MB hold.
+size_t tiles_ahead(size_t tiles, size_t tile_bytes) { return std::max<size_t>(1, std::min<size_t>(tiles, (16u << 20) / tile_bytes)); }
+
+// How a product is cut: token tiles of nt times eight operand columns, the columns of a block of 128 rows over `ranks` CTAs of a
+// cluster, the row blocks over `clusters` of these in turn; `ahead`: a launch makes the activations' fragments for all.
+//
+// The cut with the least estimated time, microseconds. A CTA's unit of 128 columns takes 0.5, 0.8 or 1.7 for one, two or four
+// eights (three times that for 256 of q4_k, whose groups are twice as many and have minima), the join of a row block 0.6, over
+// a cluster 1.1; 256 items of staging 0.5 for a CTA itself, anew for every row block where they do not all fit, or 1.5 for a launch
+// and 0.03 a unit; whatever does not fit the GPU at a time waits (and clusters fit less well beside what a launch in front has
+// left running). Against all of its cuts the one chosen is 1.0 % off the fastest on average and 18 % at most (396 products:
+// 21 weights from 256 x 256 to 151936 x 896, 1 to 1024 tokens, fp32 and bf16). One cut for a single token tile whatever the batch
+// was 29 % off: 4864 x 896, 1024 fp32 tokens, 406 us, and 130 with the row blocks uncut; 256 x 256 q4_k, 16 tokens, 7.7 and 3.2
+// with four tiles of four tokens instead of one.
+struct Cut {
+    uint32_t nt = 0, ranks = 0, units_rank = 0, units_staged = 0, clusters = 0;
+    bool ahead = false;
+};
+Cut cut_of(csdr_context* ctx, const Q4View& w, bool split, size_t batch, bool may_stage_ahead) {
+    const uint32_t blocks = (w.rows + kRowsBlock - 1u) / kRowsBlock;
+    Cut best;
+    float least = 0.0f;
+    for (uint32_t nt = 1; nt <= 4u; nt *= 2u) {
+        const Sizes sz(split, w.format, nt);
+        if (nt > 1u && sz.tokens >= 2u * batch) break;
+        const size_t tiles = (batch + sz.tokens - 1u) / sz.tokens;
+        if (tiles > 65535u) continue;      // of a grid
+        const float unit = (nt == 1u ? 0.5f : nt == 2u ? 0.8f : 1.7f) * (w.format ? 3.0f : 1.0f);
+        for (uint32_t n = 2; n >= 1u; --n)
+            for (uint32_t r = 1; r <= 8u && r <= w.n_units; ++r) {
+                const uint32_t fit = resident(ctx, n, r), units = (w.n_units + r - 1u) / r, fits = sz.staged(n);
+                const uint32_t most = std::min(blocks, std::max(1u, static_cast<uint32_t>(ctx->sm_count) * n / r));
+                const uint32_t fewer = std::min<uint32_t>(most, std::max<uint32_t>(1u, static_cast<uint32_t>(ctx->sm_count * n / r / tiles)));
+                const float items = static_cast<float>((units * std::min<size_t>(batch, sz.tokens) * sz.groups * 4u + kThreads - 1u) / kThreads);
+                // two CTAs an SM where shared memory lets them
+                const uint32_t at_once = n == 2u || sz.sum_bytes + std::min(units, fits) * sz.stage_bytes <= 104u * 1024u ? resident(ctx, 2, r) : fit;
+                for (uint32_t c : {most, fewer})
+                    for (bool ahead : {false, true}) {
+                        if (ahead && !may_stage_ahead) continue;
+                        const float turns = static_cast<float>((blocks + c - 1u) / c), staging = ahead ? 0.03f * units : 0.5f * items;
+                        float waves = std::max(1.0f, static_cast<float>(tiles) * c / (at_once * (ahead ? 0.95f : 1.0f)));
+                        if (waves < 6.0f) waves = std::ceil(waves);
+                        const float cta = 0.8f + turns * (units * unit + (r > 1u ? 1.1f : 0.6f)) + staging * (units > fits ? turns : 1.0f);
+                        const float cost = (ahead ? 1.5f : 0.0f) + waves * cta;
+                        if (best.nt && cost >= least) continue;
+                        least = cost;
+                        best = {nt, r, units, std::min(units, fits), c, ahead};
+                    }
+            }
+    }
+    return best;
+}
+
+template <typename T, int FMT, int NT, bool ONE>
+void launch(csdr_context* ctx, Q4Params p, const Cut& cut) {
+    using S = Q4Shape<FMT, NT, std::is_same<T, float>::value>;
+    constexpr Sizes kSizes(std::is_same<T, float>::value, FMT, NT);
+    static_assert(kSizes.tokens == S::kTokens && kSizes.stage_bytes == S::kStageBytes && kSizes.sum_bytes == S::kSumBytes && kSizes.groups == S::kGroups, "one size");
+    p.n_blocks = (p.w.rows + kRowsBlock - 1u) / kRowsBlock;
+    p.units_rank = cut.units_rank;
+    p.units_staged = cut.units_staged;
     const size_t smem = S::kSumBytes + static_cast<size_t>(p.units_staged) * S::kStageBytes;
     p.x_vec = p.a.x_col == 1 && (reinterpret_cast<uintptr_t>(p.a.x) | p.a.x_token * sizeof(T)) % 16u == 0;
-    const uint32_t clusters = std::min(p.n_blocks, static_cast<uint32_t>(ctx->sm_count) * per_sm / ranks);
     auto kern = q4_matmul_kernel<T, FMT, NT, ONE>;
     ctx->opt_in_smem(reinterpret_cast<const void*>(kern), smem);
     p.status = ctx->status_word;
     p.spin = ctx->spin_limit_barrier;
-    // A CTA makes its activations' fragments itself while that is a turn or two of its threads (11008 x 4096 q4_0, one token: 9 us,
-    // with a launch before it 10.4); else a launch makes them once for all (11008 x 4096 q4_k, 8 fp16 tokens: 16 us without,
-    // 12.9 with; 32 tokens: 47 and 34). Token tiles a launch: what 16 MB of fragments hold. Where nothing may be allocated, the
-    // CTAs do it.
     const size_t tiles = (p.a.batch + S::kTokens - 1u) / S::kTokens, tile_bytes = static_cast<size_t>(p.w.n_units) * S::kStageBytes;
-    const size_t items = static_cast<size_t>(p.units_rank) * std::min<size_t>(p.a.batch, S::kTokens) * S::kGroups * 4u;
-    size_t each = std::max<size_t>(1, std::min<size_t>(tiles, (16u << 20) / tile_bytes));
-    bool ahead = items > 2u * kThreads;
-    if (ahead && ctx->capturing()) {
-        const DevPtr& now = ctx->scratch[csdr_context::kQ4Scratch];
-        if (!now || now->bytes < each * tile_bytes) ahead = false;
-        else if (ctx->held.empty() || ctx->held.back() != now) ctx->held.push_back(now);      // for the graph
-    }
-    if (!ahead) each = tiles;
+    const size_t each = cut.ahead ? tiles_ahead(tiles, tile_bytes) : tiles;
     const Q4Args all = p.a;
     for (size_t t0 = 0; t0 < tiles; t0 += each) {
         const size_t n = std::min(each, tiles - t0), tok = t0 * S::kTokens;
         p.a.x = static_cast<const T*>(all.x) + tok * all.x_token;
         p.a.y = all.y + tok * all.y_token;
         p.a.batch = std::min(all.batch - tok, n * S::kTokens);
-        if (ahead) {
+        if (cut.ahead) {
             p.planes = static_cast<uint8_t*>(ctx->scratch_get(csdr_context::kQ4Scratch, each * tile_bytes));
             constexpr uint32_t kUnits = 2;
             LaunchScope ls(ctx, KC_Q4);
@@ -509,18 +569,40 @@ void launch(csdr_context* ctx, Q4Params p) {
             ls.done("q4_stage_kernel");
         }
         LaunchScope ls(ctx, KC_Q4);
-        launch_op(ctx, kern, dim3(clusters * ranks, static_cast<unsigned>(n)), kThreads, smem, ranks, p);
+        launch_op(ctx, kern, dim3(cut.clusters * cut.ranks, static_cast<unsigned>(n)), kThreads, smem, cut.ranks, p);
         ls.done("q4_matmul_kernel");
     }
 }
 
 template <typename T, int FMT>
 void launch_tokens(csdr_context* ctx, const Q4Params& p) {
-    const size_t m = p.a.batch * (std::is_same<T, float>::value ? 2u : 1u);
-    if (p.a.batch == 1) launch<T, FMT, 1, true>(ctx, p);
-    else if (m <= 8) launch<T, FMT, 1>(ctx, p);
-    else if (m <= 16) launch<T, FMT, 2>(ctx, p);
-    else launch<T, FMT, 4>(ctx, p);
+    constexpr bool kSplit = std::is_same<T, float>::value;
+    // The same sizes are cut alike: remembered, as there are some hundred cuts to compare.
+    auto remembered = [&](bool may_stage_ahead) {
+        const std::array<size_t, 3> key{(static_cast<size_t>(p.w.rows) << 32) | p.w.cols, p.a.batch,
+                                        static_cast<size_t>(p.w.format) | (kSplit ? 2u : 0u) | (may_stage_ahead ? 4u : 0u)};
+        auto& known = ctx->q4_cuts;
+        auto it = known.find(key);
+        if (it == known.end()) {
+            if (known.size() >= 4096u) known.clear();
+            const Cut c = cut_of(ctx, p.w, kSplit, p.a.batch, may_stage_ahead);
+            it = known.emplace(key, std::array<uint32_t, 6>{c.nt, c.ranks, c.units_rank, c.units_staged, c.clusters, c.ahead ? 1u : 0u}).first;
+        }
+        const auto& v = it->second;
+        return Cut{v[0], v[1], v[2], v[3], v[4], v[5] != 0u};
+    };
+    Cut cut = remembered(true);
+    if (cut.ahead && ctx->capturing()) {      // nothing may be allocated, and what the graph uses stays
+        const Sizes sz(kSplit, FMT, cut.nt);
+        const size_t tile_bytes = static_cast<size_t>(p.w.n_units) * sz.stage_bytes;
+        const DevPtr& now = ctx->scratch[csdr_context::kQ4Scratch];
+        if (!now || now->bytes < tiles_ahead((p.a.batch + sz.tokens - 1u) / sz.tokens, tile_bytes) * tile_bytes) cut = remembered(false);
+        else if (ctx->held.empty() || ctx->held.back() != now) ctx->held.push_back(now);
+    }
+    if (p.a.batch == 1) launch<T, FMT, 1, true>(ctx, p, cut);
+    else if (cut.nt == 1u) launch<T, FMT, 1, false>(ctx, p, cut);
+    else if (cut.nt == 2u) launch<T, FMT, 2, false>(ctx, p, cut);
+    else launch<T, FMT, 4, false>(ctx, p, cut);
 }
 
 }  // namespace

@@ -266,3 +266,106 @@ def test_a_captured_product_of_another_kind_keeps_its_scratch():
     larger.close()
     seg.close()
     own.close()
+
+
+def check_wide(y, x, dense, units):
+    """check() for any width: a product carries 2^-22 + 2^-23, and of q4_0 the 8 of every code as much again; a rank adds up at most
+    `units` partial sums, eight ranks and a bias their sums, each rounded to 2^-24, and matrix units cut off 2^-23 in each of
+    sixteen steps of a unit."""
+    x = x.to(torch.float64).numpy()
+    want, room = x @ dense.T, np.abs(x) @ np.abs(dense).T
+    assert (np.abs(y - want) <= (2.0 ** -20 + (units + 8 + 32) * 2.0 ** -24) * room + 1e-30).all()
+    assert np.linalg.norm(y - want) <= 2e-6 * np.linalg.norm(want) + 1e-30
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt,cols", [("q4_0", 96), ("q4_0", 1152), ("q4_k", 512)])
+@pytest.mark.parametrize("batch", [1, 3, 40])
+def test_more_row_blocks_than_the_gpu_holds(ctx, fmt, cols, batch, dtype):
+    """CTAs take blocks of rows in turn."""
+    rows = 128 * 2 * torch.cuda.get_device_properties(0).multi_processor_count + 128 * 17 + 5      # two CTAs an SM, and some more
+    rng = np.random.default_rng(cols + batch)
+    payload, dense = ref.q4_weight(rng, rows, cols, fmt)
+    w = cs.Q4Weight.from_payload(payload, fmt, rows, cols, ctx)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32).to(DTYPES[dtype][0])
+    bias = torch.tensor(rng.normal(0, 1, rows), dtype=torch.float32).cuda()
+    for layout in (0, 1):
+        got = run(w, x, layout, rows, ctx)
+        check(got, x, dense)
+        np.testing.assert_allclose(run(w, x, layout, rows, ctx, bias), got + bias.cpu().numpy(), rtol=1e-6, atol=1e-5)
+    w.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("fmt,cols", [("q4_0", 99200), ("q4_k", 97280)])
+@pytest.mark.parametrize("batch", [1, 5, 33])
+def test_activations_that_do_not_fit_at_a_time(ctx, fmt, cols, batch, dtype):
+    """An eighth of the columns is more than shared memory holds as fragments: they are brought in parts, by the CTAs themselves
+    and by copies of what a launch has made."""
+    units = -(-cols // (256 if fmt == "q4_k" else 128))
+    assert -(-units // 8) * (4384 if fmt == "q4_k" else 2208) > 208 * 1024 - 6144      # the least that fragments and results are
+    rows, rng = 300, np.random.default_rng(cols + batch)
+    payload, dense = ref.q4_weight(rng, rows, cols, fmt)
+    side = torch.cuda.Stream()
+    own = cs.Context(0, side.cuda_stream)
+    w = cs.Q4Weight.from_payload(payload, fmt, rows, cols, own)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32).to(DTYPES[dtype][0])
+    # captured first of all: without scratch, so by the CTAs themselves
+    xd, y = x.cuda(), torch.zeros(batch, rows, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(g, stream=side):
+            w.matmul_device(xd.data_ptr(), DTYPES[dtype][1], 1, batch, y.data_ptr(), 1)
+        g.replay()
+    side.synchronize()
+    check_wide(y.to(torch.float64).cpu().numpy(), x, dense, units)
+    for layout in (0, 1):
+        check_wide(run(w, x, layout, rows, own), x, dense, units)
+    del g
+    w.close()
+    own.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_fragments_than_a_launch_takes(ctx, dtype):
+    """Token tiles go over several pairs of launches, the last one ragged, all through the same scratch."""
+    rows, cols, batch = 130, 4096, 4099
+    rng = np.random.default_rng(17)
+    payload, dense = ref.q4_weight(rng, rows, cols, "q4_k")
+    w = cs.Q4Weight.from_payload(payload, "q4_k", rows, cols, ctx)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32).to(DTYPES[dtype][0])
+    for x_layout, y_layout in ((0, 0), (1, 1), (1, 0)):
+        before = ctx.launch_count
+        got = run(w, x, x_layout, rows, ctx, y_layout=y_layout)
+        assert ctx.launch_count - before >= 4
+        check(got, x, dense)
+    w.close()
+
+
+def test_packed_products_of_prompts_are_not_slower_than_widened_ones(ctx, tmp_path):
+    """A decoder's stored-raw linears stay packed at any number of tokens: the dense fp32 product of the widened weight, which they
+    were before, must not be the faster one. Device time between events, medians, a fifth to spare."""
+    rows, cols, batch = 4864, 896, 1024
+    rng = np.random.default_rng(18)
+    payload, dense = ref.q4_weight(rng, rows, cols, "q4_0")
+    synth.write_sdr(str(tmp_path / "w.sdr"), [synth.raw_segment("w", dense.astype(np.float32), synth.SEG_ATTENTION, 0)])
+    loader = cs.SDRModelLoader(str(tmp_path / "w.sdr"), ctx)
+    engine = cs.SDRInferenceEngine(loader)
+    w = cs.Q4Weight.from_payload(payload, "q4_0", rows, cols, ctx)
+    x = rng.normal(0, 1, (cols, batch)).astype(np.float32)
+    xd = torch.tensor(x).t().contiguous()
+
+    def median(call):
+        call()
+        took = []
+        for _ in range(7):
+            ctx.profile(True)
+            call()
+            took.append(sum(ms for _, ms in ctx.profile_read().values()))
+            ctx.profile(False)
+        return sorted(took)[3]
+
+    assert median(lambda: run(w, xd, 1, rows, ctx)) <= 1.2 * median(lambda: engine.matmulForLayer("w", x, batch))
+    w.close()
+    loader.close()
