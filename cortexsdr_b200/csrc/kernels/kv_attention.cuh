@@ -120,17 +120,14 @@ __device__ __forceinline__ void join(uint32_t n, uint32_t d, F&& get, float (&o)
 // Eight results, as one or two 128-bit pieces where rows start on 16 bytes.
 template <typename T>
 __device__ __forceinline__ void store_row(T* to, const float (&v)[8], float by, bool vec) {
-    T r[8];
+    Eight128<T> r;
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i) r[i] = op_narrow<T>(v[i] * by);
+    for (uint32_t i = 0; i < 8u; ++i) r.v[i] = op_narrow<T>(v[i] * by);
     if (vec) {
-        const uint4* from = reinterpret_cast<const uint4*>(r);
-        uint4* at = reinterpret_cast<uint4*>(to);
-        at[0] = from[0];
-        if constexpr (sizeof(T) == 4) at[1] = from[1];
+        r.store(to);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) to[i] = r[i];
+        for (uint32_t i = 0; i < 8u; ++i) to[i] = r.v[i];
     }
 }
 

@@ -104,16 +104,14 @@ struct Eight {
 };
 template <typename T>
 __device__ __forceinline__ void store8(T* to, bool vec, const float (&x)[8]) {
-    T r[8];
+    Eight128<T> r;
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i) r[i] = op_narrow<T>(x[i]);
+    for (uint32_t i = 0; i < 8u; ++i) r.v[i] = op_narrow<T>(x[i]);
     if (vec) {
-        const uint4* from = reinterpret_cast<const uint4*>(r);
-        reinterpret_cast<uint4*>(to)[0] = from[0];
-        if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(to)[1] = from[1];
+        r.store(to);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) to[i] = r[i];
+        for (uint32_t i = 0; i < 8u; ++i) to[i] = r.v[i];
     }
 }
 

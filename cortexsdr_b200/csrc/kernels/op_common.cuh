@@ -75,6 +75,17 @@ __device__ __forceinline__ __nv_bfloat16 op_narrow<__nv_bfloat16>(float v) { ret
 template <>
 __device__ __forceinline__ __half op_narrow<__half>(float v) { return __float2half_rn(v); }
 
+// Eight elements that leave in 128-bit pieces.
+template <typename T>
+struct alignas(16) Eight128 {
+    T v[8];
+    __device__ __forceinline__ void store(T* to) const {
+        static_assert(sizeof(*this) % sizeof(uint4) == 0 && alignof(Eight128) >= alignof(uint4), "whole pieces");
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) / 2u; ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(v)[i];
+    }
+};
+
 // Calls f with a null pointer of the element type that a CSDR_DTYPE_* stands for.
 template <typename F>
 void with_dtype(int dtype, F&& f) {
