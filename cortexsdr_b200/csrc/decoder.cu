@@ -794,6 +794,7 @@ int csdr_decoder_create(csdr_archive* ar, const csdr_decoder_config* cfg, csdr_d
         d->cache_layer_stride = static_cast<size_t>(c.max_batch) * c.max_seq * d->KVD_l;
         if (c.kv_dtype == CSDR_KV_Q4) {
             if (d->P > 1) throw Error(CSDR_ERR_UNSUPPORTED, "decoder: the 4-bit KV cache is for a single GPU");
+            if (!(c.rope_theta >= 1.0f)) throw Error(CSDR_ERR_INVALID_ARG, "decoder: the 4-bit KV cache needs a rope_theta of at least 1");
             constexpr uint32_t kPage = 64;
             d->kv_pages_per_seq = (c.max_seq + kPage - 1) / kPage;
             const uint64_t pages = static_cast<uint64_t>(c.max_batch) * d->kv_pages_per_seq;

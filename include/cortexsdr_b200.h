@@ -444,7 +444,7 @@ typedef struct {
      * the cache, scores and sums in fp32; half the cache bytes per step; fp16 keeps three more
      * mantissa bits and wants |k|, |v| < 65504), or CSDR_KV_Q4 (keys and values in 4 bits, see the
      * paged cache below: 0.28 of the bytes of 16 bits; rotary angles in 64 bits; a single GPU, head_dim
-     * 64, 128 or 256). No counterpart in the reference. */
+     * 64, 128 or 256, rope_theta at least 1). No counterpart in the reference. */
     uint32_t kv_dtype;
 } csdr_decoder_config;
 

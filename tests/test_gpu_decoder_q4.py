@@ -161,3 +161,14 @@ def test_refuses_heads_the_cache_does_not_take(ctx, tmp_path_factory, oracle):
     path, _ = _build_model(tmp_path_factory, oracle, "hd32", CFG=cfg, n_atoms=32, kv_atoms=16)
     with pytest.raises(cs.CompressionError, match="head_dim"):
         make_decoder(path, ctx, CFG=cfg, kv_dtype="q4")
+
+
+@pytest.mark.parametrize("theta", [0.0, -1.0, 0.5, float("nan"), float("inf")])
+def test_refuses_rotations_that_the_cache_does_not_have(ctx, model_packed, theta):
+    """When it is made, not at its first step."""
+    loader = cs.SDRModelLoader(model_packed[0], ctx)
+    with pytest.raises(ValueError, match="rope_theta"):
+        cs.Decoder(loader, **CFG, max_seq=64, rms_eps=EPS, rope_theta=theta, kv_dtype="q4")
+    dec = cs.Decoder(loader, **CFG, max_seq=64, rms_eps=EPS, rope_theta=1.0, kv_dtype="q4")
+    assert np.isfinite(dec.forward([1, 2, 3])[0]).all()
+    dec.close()
