@@ -114,7 +114,8 @@ class Context:
         return int(self._lib.csdr_context_launch_count(self._h))
 
     def set_wait_limits(self, gemv_polls: int = 0, barrier_rounds: int = 0, exchange_polls: int = 0):
-        """Iteration limits of the bounded device-side waits; 0 restores a default."""
+        """Iteration limits of the bounded device-side waits; 0 restores a default. barrier_rounds _lib.WAIT_GIVE_UP: the
+        kernels over 4-bit data give up their first wait (tests)."""
         _check(self._lib.csdr_context_set_wait_limits(self._h, gemv_polls, barrier_rounds, exchange_polls))
 
     def wait_selftest(self) -> int:

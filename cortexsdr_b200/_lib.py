@@ -27,6 +27,7 @@ ERR_LIMIT = -12
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 KV_Q4 = 16
+WAIT_GIVE_UP = 0xFFFFFFFF
 FEATURE_MAJOR, TOKEN_MAJOR = 0, 1
 
 

@@ -407,7 +407,8 @@ int csdr_context_set_wait_limits(csdr_context* ctx, uint32_t gemv_polls, uint32_
         require_ctx(ctx);
         const csdr_context fresh{};
         ctx->spin_limit_gemv = gemv_polls ? gemv_polls : fresh.spin_limit_gemv;
-        ctx->spin_limit_barrier = barrier_rounds ? barrier_rounds : fresh.spin_limit_barrier;
+        ctx->operators_give_up = barrier_rounds == static_cast<uint32_t>(CSDR_WAIT_GIVE_UP);
+        ctx->spin_limit_barrier = barrier_rounds && !ctx->operators_give_up ? barrier_rounds : fresh.spin_limit_barrier;
         ctx->spin_limit_exchange = exchange_polls ? exchange_polls : fresh.spin_limit_exchange;
     });
 }

@@ -588,7 +588,7 @@ kv_attention_kernel(AttnParams p) {
             if constexpr (Warp::kShared) __syncthreads();
             for (uint32_t i = 0; i < n; ++i) {
                 const uint32_t k = turn0 + i, st = k % kStages;
-                live = mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
+                live = mbar_wait_first(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
                 if (!live) {
                     for (uint32_t j = k; j < turn; ++j) mbar_wait(my_bar + 8u * (j % kStages), (j / kStages) & 1u, kDrainRounds);
                     break;
@@ -626,7 +626,7 @@ kv_attention_kernel(AttnParams p) {
             __syncwarp();
             for (uint32_t i = 0; i < n && live; ++i) {
                 const uint32_t k = turn0 + i, st = k % kStages;
-                live = mbar_wait(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
+                live = mbar_wait_first(my_bar + 8u * st, (k / kStages) & 1u, p.spin);
                 if (!live) break;
                 const int32_t tok = static_cast<int32_t>(kPiece * (first + i));
                 if (tok < rows.most) rows.piece(my_ring + st * kStageBytes, tok, there_s[st], lane, my_q, my_meta);
@@ -759,7 +759,7 @@ void launch_kv_attention(csdr_context* ctx, const KvView& kv, uint32_t head_dim,
     p.counters = static_cast<uint32_t*>(workspace);
     p.part = reinterpret_cast<float*>(p.counters + kv_attention_counters(ctx));
     p.status = ctx->status_word;
-    p.spin = ctx->spin_limit_barrier;
+    p.spin = ctx->operator_spin();
     const size_t es = dtype == CSDR_DTYPE_F32 ? 4 : 2;
     p.vec = (reinterpret_cast<uintptr_t>(a.q) | a.q_stride * es) % 16u == 0;
     p.vec_out = (reinterpret_cast<uintptr_t>(a.out) | a.out_stride * es) % 16u == 0;

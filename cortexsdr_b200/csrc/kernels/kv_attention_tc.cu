@@ -541,7 +541,7 @@ kv_attention_tc_kernel(AttnParams p) {
                 if (lane == 0u) ctl.there[b][mine] = there ? 1u : 0u;
                 publish(bar(ctl.kv_full[b]), lane);
                 if (warp == 7u) {
-                    if (i == 0u) live = mbar_wait(bar(ctl.q_full), units++ & 1u, p.spin);
+                    if (i == 0u) live = mbar_wait_first(bar(ctl.q_full), units++ & 1u, p.spin);      // the others wait for what comes of it
                     scores(k);
                     if (i) outputs(k - 1u, i == 1u);
                     if (!live) return;

@@ -295,7 +295,7 @@ q4_matmul_kernel(Q4Params p) {
                          "l"(p.planes + (static_cast<size_t>(blockIdx.y) * p.w.n_units + u0) * S::kStageBytes), "r"(bytes), "r"(smem_u32(&bar))
                          : "memory");
         }
-        if (live && !mbar_wait(smem_u32(&bar), copies & 1u, p.spin)) {
+        if (live && !mbar_wait_first(smem_u32(&bar), copies & 1u, p.spin)) {
             live = false;
             if (warp == 0) mbar_wait(smem_u32(&bar), copies & 1u, kDrainRounds);
         }
@@ -552,7 +552,7 @@ void launch(csdr_context* ctx, Q4Params p, const Cut& cut) {
     auto kern = q4_matmul_kernel<T, FMT, NT, ONE>;
     ctx->opt_in_smem(reinterpret_cast<const void*>(kern), smem);
     p.status = ctx->status_word;
-    p.spin = ctx->spin_limit_barrier;
+    p.spin = ctx->operator_spin();
     const size_t tiles = (p.a.batch + S::kTokens - 1u) / S::kTokens, tile_bytes = static_cast<size_t>(p.w.n_units) * S::kStageBytes;
     const size_t each = cut.ahead ? tiles_ahead(tiles, tile_bytes) : tiles;
     const Q4Args all = p.a;

@@ -100,7 +100,10 @@ CSDR_API uint64_t csdr_context_launch_count(const csdr_context* ctx);
  * partial results, the mbarrier waits of the tensor-core kernels, and a tensor-parallel rank's
  * wait for its peers' flags. A wait that runs out records a status word, the kernel returns, and
  * the next csdr_context_synchronize answers CSDR_ERR_TIMEOUT; the context stays usable. 0 keeps
- * or restores a default (1e6 polls, 4e6 rounds, 2e6 polls: of the order of a second each). */
+ * or restores a default (1e6 polls, 4e6 rounds, 2e6 polls: of the order of a second each).
+ * barrier_rounds CSDR_WAIT_GIVE_UP: the kernels over 4-bit data (attention, products) give up their first
+ * wait whatever they find, for tests of what a caller does then; the others keep the default. */
+enum { CSDR_WAIT_GIVE_UP = -1 };
 CSDR_API int csdr_context_set_wait_limits(csdr_context* ctx, uint32_t gemv_polls,
                                           uint32_t barrier_rounds, uint32_t exchange_polls);
 /* Diagnostic: runs the receiving side of a two-rank exchange on a scratch region whose second

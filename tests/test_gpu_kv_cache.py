@@ -673,3 +673,26 @@ def test_long_prompts(ctx, hd, dtype):
     c = Case(ctx, [280, 270], [265, 260], 1, hd, 32, seed=hd, dtype=dtype, tail=2)
     c.store()
     prompts(c, 4)
+
+
+# the kernels whose warps share rows; have rows of their own, eight or sixteen; prompts on the tensor cores
+@pytest.mark.parametrize("dtype,hd,fresh", [("f32", 64, 1), ("f32", 128, 1), ("bf16", 256, 1), ("f16", 128, 1), ("f32", 128, 300), ("f16", 64, 60),
+                                            ("f16", 128, 60), ("bf16", 64, 60), ("bf16", 128, 60), ("bf16", 256, 300)])
+def test_waits_that_are_given_up(dtype, hd, fresh):
+    """Every wait is given up with copies on their way: the call says so, units that CTAs share are arrived at all the same, and
+    the next call finds its counters and the shared memory as it needs them."""
+    own = cs.Context(0)
+    c = Case(own, [9000, 500, 2000], [fresh] * 3, 2, hd, 64, seed=6, dtype=dtype)
+    c.store(rotate=False)
+    q = c.rows([c.values((fresh, 8, hd)) for _ in range(3)])
+    want = c.attend(q, 8)
+    for _ in range(2):
+        own.set_wait_limits(barrier_rounds=_lib.WAIT_GIVE_UP)
+        for _ in range(2):
+            with pytest.raises(cs.CudaError, match="wait ran out"):
+                c.attend(q, 8)
+        own.set_wait_limits()
+        for _ in range(2):
+            assert torch.equal(c.attend(q, 8), want)
+    c.cache.close()
+    own.close()

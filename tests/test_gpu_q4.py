@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import cortexsdr_b200 as cs
+from cortexsdr_b200 import _lib
 from tests import operator_refs as ref
 from tests import synth
 
@@ -369,3 +370,29 @@ def test_packed_products_of_prompts_are_not_slower_than_widened_ones(ctx, tmp_pa
     assert median(lambda: run(w, xd, 1, rows, ctx)) <= 1.2 * median(lambda: engine.matmulForLayer("w", x, batch))
     w.close()
     loader.close()
+
+
+@pytest.mark.parametrize("fmt,rows,cols,batch,copies", [("q4_0", 512, 8192, 48, True), ("q4_k", 300, 8192, 48, False), ("q4_0", 300, 99200, 33, True),
+                                                        ("q4_k", 4096, 4096, 48, True)])
+def test_waits_that_are_given_up(fmt, rows, cols, batch, copies):
+    """Copies of the activations' fragments are given up on their way, in one part and in several. Where CTAs make the fragments
+    themselves nothing waits."""
+    own = cs.Context(0)
+    rng = np.random.default_rng(19)
+    payload, dense = ref.q4_weight(rng, rows, cols, fmt)
+    w = cs.Q4Weight.from_payload(payload, fmt, rows, cols, own)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32)
+    before = own.launch_count
+    want = run(w, x, 1, rows, own)
+    assert own.launch_count - before == (2 if copies else 1)      # the first makes the fragments
+    for _ in range(2):
+        own.set_wait_limits(barrier_rounds=_lib.WAIT_GIVE_UP)
+        if copies:
+            with pytest.raises(cs.CudaError, match="wait ran out"):
+                run(w, x, 1, rows, own)
+        else:
+            np.testing.assert_array_equal(run(w, x, 1, rows, own), want)
+        own.set_wait_limits()
+        np.testing.assert_array_equal(run(w, x, 1, rows, own), want)
+    w.close()
+    own.close()
