@@ -696,3 +696,98 @@ def test_waits_that_are_given_up(dtype, hd, fresh):
             assert torch.equal(c.attend(q, 8), want)
     c.cache.close()
     own.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,kvh,page", [(64, 3, 16), (128, 2, 64), (256, 1, 32)])
+def test_prompts_of_many_tokens_are_held_as_the_definition_says(ctx, hd, kvh, page, dtype):
+    """Enough tokens for a CTA to take four of them: keys, values and queries, with rotation, value for value; a sequence that
+    goes on far behind its start, an idle one, rows of no sequence; then the same without rotation, queries copied."""
+    many = 16 * torch.cuda.get_device_properties(0).multi_processor_count
+    qh, tail, far = 3, 3, 70_001
+    fresh = [many - 700, 0, 650, 59]
+    lengths = [many - 700, 7, far + 650, 59]
+    assert sum(fresh) >= many and sum(fresh) % 4
+    c = Case(ctx, lengths, fresh, kvh, hd, page, seed=hd, dtype=dtype)
+    new = [slice(n - f, n) for n, f in zip(lengths, fresh)]
+    q = [c.values((f, qh, hd)) for f in fresh]
+    dq, dk, dv = c.rows(q, tail, 5.0), c.rows([t[n] for t, n in zip(c.k, new)], tail, 5.0), c.rows([t[n] for t, n in zip(c.v, new)], tail, 5.0)
+    b = c.batch(lengths, fresh, tail)
+    t = sum(fresh)
+    pos = [np.arange(n.start, n.stop) for n in new]
+    half = torch.finfo(c.tdtype).eps / 2
+    for rotate in (True, False):
+        q_out = torch.full_like(dq, 7.0)
+        k_out, v_out = (torch.full(dk.shape, 7.0, dtype=torch.float32, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+        c.cache.append(b, dk.data_ptr(), dv.data_ptr(), c.dtype, rotate=rotate, q_ptr=dq.data_ptr(), q_heads=qh, q_out_ptr=q_out.data_ptr())
+        c.cache.read(b, k_out.data_ptr(), v_out.data_ptr())
+        ctx.synchronize()
+        turned = lambda x, p: ref.rotate(x.to(torch.float64).numpy(), p, THETA) if rotate else x.to(torch.float64).numpy()
+        want_k = np.concatenate([ref.held(turned(x[n], p)) for x, n, p in zip(c.k, new, pos) if len(p)])
+        want_v = np.concatenate([ref.held(x[n].to(torch.float64).numpy()) for x, n, p in zip(c.v, new, pos) if len(p)])
+        np.testing.assert_array_equal(k_out[:t].cpu().numpy(), want_k.astype(np.float32))
+        np.testing.assert_array_equal(v_out[:t].cpu().numpy(), want_v.astype(np.float32))
+        want_q = np.concatenate([turned(x, p) for x, p in zip(q, pos) if len(p)])
+        got_q = q_out[:t].to(torch.float64).cpu().numpy()
+        if rotate:
+            # cos and sin are off by 2^-24.9, two products and their sum round: 2.6 2^-24 (|x0| + |x1|); then half a step of the
+            # type: 2^-11 of a fp16 value, and under 2^-14, where its steps are 2^-24 however small it is, 2^-25
+            smallest = 2.0 ** -25 if c.tdtype == torch.float16 else 0.0
+            x = np.abs(np.concatenate([a.to(torch.float64).numpy() for a in q if len(a)]))
+            both = np.repeat(x[..., 0::2] + x[..., 1::2], 2, axis=-1)
+            assert (np.abs(got_q - want_q) <= np.maximum(half * np.abs(want_q), smallest) + (1 + half) * 2.6 * 2.0 ** -24 * both).all()
+        else:
+            np.testing.assert_array_equal(got_q, want_q)
+        for out in (q_out, k_out, v_out):
+            assert (out[t:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype,prompt,singles", [("bf16", 300, 31), ("bf16", 1100, 31), ("f16", 300, 31), ("f16", 1000, 12), ("f32", 300, 31),
+                                                  ("f32", 1100, 2)])
+def test_a_prompt_among_single_tokens(ctx, dtype, prompt, singles):
+    """One call for both, on either side of the mean of rows that chooses the kernel; an idle sequence counts among them."""
+    rng = np.random.default_rng(prompt + singles)
+    lengths = [prompt + 100] + [int(n) for n in rng.integers(1, 400, singles)] + [50]
+    fresh = [prompt] + [1] * singles + [0]
+    c = Case(ctx, lengths, fresh, 2, 128, 32, seed=prompt, dtype=dtype, spare=1, tail=3)
+    c.store()
+    prompts(c, 8)
+
+
+def test_fp32_sums_do_not_drift(ctx):
+    """Over 1024 keys of ordinary scores the outputs are no further off than those of fp32 products and sums, a quarter to spare
+    (sums that are cut off instead of rounded were twice as far)."""
+    torch.backends.cuda.matmul.allow_tf32 = False
+    n, length, heads, hd = 16, 1024, 32, 128
+    for seed in range(3):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        loud = lambda: 1.0 + 3.0 * (torch.rand(heads, hd, generator=gen, device="cuda") < 0.05)
+        k, v = (torch.randn(n * length, heads, hd, generator=gen, device="cuda") * loud() for _ in range(2))
+        q = 1.5 * torch.randn(n, heads, hd, generator=gen, device="cuda")
+        cache = cs.KVCache(n * length // 64, 64, heads, hd, rope_theta=0.0, ctx=ctx)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        lens, pages = ints([length] * n), ints(rng_pages(seed, n, length // 64))
+        whole, last = ints([length * i for i in range(n + 1)]), ints(list(range(n + 1)))
+        batch = lambda f, t: cs.KVBatch(n, t, f.data_ptr(), lens.data_ptr(), pages.data_ptr(), length // 64)
+        out, hk, hv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        torch.cuda.synchronize()
+        cache.append(batch(whole, n * length), k.data_ptr(), v.data_ptr(), 0, rotate=False)
+        cache.read(batch(whole, n * length), hk.data_ptr(), hv.data_ptr())
+        cache.attention(batch(last, n), q.data_ptr(), 0, heads, out.data_ptr())
+        ctx.synchronize()
+
+        def attend(x):
+            kk, vv = (a.to(x).view(n, length, heads, hd).transpose(1, 2) for a in (hk, hv))
+            s = torch.matmul(kk, q.to(x)[..., None])[..., 0] / hd ** 0.5
+            e = torch.exp(s - s.amax(-1, keepdim=True))
+            return (torch.matmul(e[:, :, None], vv)[:, :, 0] / e.sum(-1, keepdim=True)).to(torch.float64)
+
+        want = attend(torch.float64)
+        own, plain = (float((a.to(torch.float64) - want).norm() / want.norm()) for a in (out, attend(torch.float32)))
+        assert own <= 1.25 * plain, (own, plain)
+        cache.close()
+
+
+def rng_pages(seed, n, per):
+    return np.random.default_rng(seed).permutation(n * per).reshape(n, per).tolist()
