@@ -7,8 +7,8 @@
 // when the maximum grows. A logit may be among the alternatives only if it reaches a bound that the k-th best cannot be below:
 // the least, over the CTA's W warps, of the ceil(k / W)-th greatest of the lanes' maxima so far, taken after the first
 // round and whenever the logits seen have doubled. What reaches it is put aside, some hundred pieces of a row,
-// and ranked at the end (2048 rows of 151936 in bf16: 101 us without alternatives, 133 to 146 with 20; 156 with lists kept in
-// order on the way). A row where more do than there is room for (rising order) is read again with the
+// and ranked at the end (2048 rows of 151936 in bf16: 101 us without alternatives, 132 with 20 - 140 to 146 in a long run of calls,
+// where the power cap holds the clock at 1.87 GHz -, 156 with lists kept in order on the way). A row where more do than there is room for (rising order) is read again with the
 // bound it ended with, into sorted lists. Keys are (logit, index), so results do not depend on who comes first. Few rows
 // are cut over the CTAs of a cluster, whose leader joins them. What bounds it: the logits' bytes, and behind them the
 // exponentials (one a logit, sixteen a clock and SM: 0.7 of the memory's time for 16-bit logits).
@@ -430,12 +430,18 @@ void launch_logprobs(csdr_context* ctx, int dtype, const LogprobArgs& a) {
     LaunchScope ls(ctx, KC_LOGPROB);
     with_dtype(dtype, [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        // four CTAs of 256 threads an SM (three: 140 us instead of 133 for 2048 rows of 151936); where a row is cut because
-        // there are few, 512
+        // Few rows are cut over two, four or eight CTAs of 512 threads, while every CTA has an SM of its own; up to a row an SM in
+        // two, where a part is worth a second CTA on the SM, which is eight loads a thread; more rows are not cut and go by four
+        // CTAs of 256 an SM (three: 140 us instead of 133 for 2048 rows of 151936 in bf16). Rows of fp32 logits, us uncut and in
+        // two, four, eight parts:
+        //   of 151936   10 rows 13.4, 7.6, 5.5, 5.1;  37: 13.6, 7.7, 7.7, 8.0;  74: 27, 11, 13, 15;  148: 29.5, 16.9, 23, 26;
+        //               296: 35, 32, 39, 50;  592: 55, 62, 71, 93 (bf16, 20 alternatives: 148 rows 22, 19, 30, 46; 296: 28, 35, 52, 84)
+        //   of 32000    10 rows 4.6, 4.3, 3.6, 3.7;  74: 4.9, 4.3, 6.2, 8.2;  148: 5.1, 5.1, 8.7, 13 (bf16, 20 alternatives: 9.1, 10.3)
         uint32_t ranks = 1;
         while (ranks < 8u && static_cast<uint64_t>(a.rows) * ranks * 2u <= static_cast<uint64_t>(ctx->sm_count) &&
                a.vocab / (ranks * 2u) >= 512u * Vec<T>::N)
             ranks *= 2u;
+        if (ranks == 1u && a.rows <= static_cast<uint32_t>(ctx->sm_count) && a.vocab / 2u >= 8u * 512u * Vec<T>::N) ranks = 2;
         const dim3 grid(a.rows * ranks);
         if (ranks == 1u) {
             if (a.top) launch_op(ctx, logprob_kernel<T, true, 256>, grid, 256, 0, 1, a);

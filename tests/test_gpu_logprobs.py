@@ -159,3 +159,20 @@ def test_on_a_stream_of_its_own_captured_and_replayed(rows, vocab):
             assert torch.equal(ids.long(), order)
     del g
     own.close()
+
+
+@pytest.mark.parametrize("dtype,vocab", [("f32", 33000), ("bf16", 70001)])
+@pytest.mark.parametrize("top", [0, 7])
+def test_rows_around_a_row_an_sm(ctx, dtype, vocab, top):
+    """From rows cut in four parts over rows cut in two to rows that are not cut: each row's answer is the same."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    rng = np.random.default_rng(vocab)
+    x = torch.tensor(rng.normal(0, 3, (sms + 1, vocab)), dtype=torch.float32).to(DTYPES[dtype][0])
+    targets = rng.integers(0, vocab, sms + 1)
+    every = run(x, targets, top, ctx)
+    check(every, x, targets, top)
+    for rows in (sms, sms // 2 + 1, sms // 2, sms // 4 + 1, sms // 4):
+        got = run(x[:rows], targets[:rows], top, ctx)
+        check(got, x[:rows], targets[:rows], top)
+        for a, b in zip(got, every):
+            np.testing.assert_allclose(a, b[:rows], rtol=2.0 ** -20, atol=2e-5)
