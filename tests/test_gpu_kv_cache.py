@@ -791,3 +791,68 @@ def test_fp32_sums_do_not_drift(ctx):
 
 def rng_pages(seed, n, per):
     return np.random.default_rng(seed).permutation(n * per).reshape(n, per).tolist()
+
+
+@pytest.mark.parametrize("dtype,hd,fresh", [("f32", 128, 1), ("f32", 64, 260), ("f16", 128, 60), ("bf16", 128, 60), ("bf16", 256, 3)])
+def test_pages_and_layers_past_32_bits(ctx, dtype, hd, fresh):
+    """Two layers of more than 4 GB each, pages at their ends."""
+    kvh, page = 8, 256
+    each = kvh * page // 16 * 18 * hd
+    n_pages = (1 << 32) // each + 40
+    c = Case(ctx, [700, 300], [fresh, min(fresh, 300)], kvh, hd, page, seed=9, dtype=dtype)
+    c.cache.close()
+    c.cache = cs.KVCache(n_pages, page, kvh, hd, layers=2, rope_theta=THETA, ctx=ctx)
+    assert c.cache.nbytes > 2 << 32
+    c.pages = np.where(c.pages >= 0, c.pages + n_pages - c.n_pages, -1).astype(np.int32)
+    c.store(layer=1)
+    qs = [c.values((f, 4 * kvh, hd)) for f in c.fresh]
+    out = c.attend(c.rows(qs), 4 * kvh, layer=1)
+    k, v = c.held()
+    at = 0
+    for s, (n, f) in enumerate(zip(c.lengths, c.fresh)):
+        pos = n - f + np.arange(f)
+        want = ref.attention(qs[s].to(torch.float64).numpy(), k[s], v[s], pos, hd ** -0.5)
+        close(out[at:at + f], want, c.tdtype, np.abs(v[s]).max(), bound_of(c, c.fresh, 4 * kvh, hd, qs[s], k[s], v[s], pos, hd ** -0.5))
+        at += f
+    b = c.batch([700, 300], [700, 300])
+    ko, vo = (torch.empty(1000, kvh, hd, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    c.cache.read(b, ko.data_ptr(), vo.data_ptr(), layer=1)
+    ctx.synchronize()
+    np.testing.assert_array_equal(ko.cpu().numpy(), np.concatenate(k).astype(np.float32))
+    np.testing.assert_array_equal(vo.cpu().numpy(), np.concatenate(v).astype(np.float32))
+    c.cache.read(b, ko.data_ptr(), vo.data_ptr(), layer=0)
+    ctx.synchronize()
+    assert (ko == 0).all() and (vo == 0).all()
+    c.cache.close()
+
+
+@pytest.mark.parametrize("dtype,group", [("f32", 2), ("bf16", 2), ("bf16", 64)])
+def test_strides_past_32_bits(ctx, dtype, group):
+    """Rows of q, k, v and the results 2^31 elements apart."""
+    hd, rows, stride = 64, 3, (1 << 31) + 16
+    c = Case(ctx, [40 + rows], [rows], 1, hd, 16, seed=10, dtype=dtype)
+    wide = torch.empty((rows - 1) * stride + (2 * group + 4) * hd, dtype=c.tdtype, device="cuda")
+    es = wide.element_size()
+    part = lambda at, heads: torch.as_strided(wide, (rows, heads, hd), (stride, hd, 1), at * hd)
+    b = c.batch([40], [40])
+    old_k, old_v = (t[0][:40].cuda() for t in (c.k, c.v))
+    new = [c.values((rows, h, hd)) for h in (group, 1, 1)]
+    for at, t in zip((0, group, group + 1), new):
+        part(at, t.shape[1]).copy_(t.cuda())
+    part(group + 2, group).fill_(7.0)
+    torch.cuda.synchronize()
+    c.cache.append(b, old_k.data_ptr(), old_v.data_ptr(), c.dtype, rotate=False)
+    b = c.batch([40 + rows], [rows])
+    p = wide.data_ptr()
+    c.cache.append(b, p + group * hd * es, p + (group + 1) * hd * es, c.dtype, kv_stride=stride, rotate=False, q_ptr=p, q_stride=stride,
+                   q_heads=group, q_out_ptr=p, q_out_stride=stride)
+    c.cache.attention(b, p, c.dtype, group, p + (group + 2) * hd * es, q_stride=stride, out_stride=stride)
+    ctx.synchronize()
+    k, v = (ref.held(torch.cat([t[0][:40], x]).to(torch.float64).numpy()) for t, x in ((c.k, new[1]), (c.v, new[2])))
+    q = new[0].to(torch.float64).numpy()
+    assert torch.equal(part(0, group).cpu(), new[0])
+    pos = 40 + np.arange(rows)
+    close(part(group + 2, group), ref.attention(q, k, v, pos, hd ** -0.5), c.tdtype, np.abs(v).max(),
+          bound_of(c, [rows], group, hd, new[0], k, v, pos, hd ** -0.5))
+    c.cache.close()

@@ -176,3 +176,15 @@ def test_rows_around_a_row_an_sm(ctx, dtype, vocab, top):
         check(got, x[:rows], targets[:rows], top)
         for a, b in zip(got, every):
             np.testing.assert_allclose(a, b[:rows], rtol=2.0 ** -20, atol=2e-5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_past_32_bits(ctx, dtype):
+    rows, vocab, stride = 3, 50001, (1 << 31) + 8
+    rng = np.random.default_rng(7)
+    x = torch.tensor(rng.normal(0, 3, (rows, vocab)), dtype=torch.float32).to(DTYPES[dtype][0])
+    room = torch.empty((rows - 1) * stride + vocab, dtype=x.dtype, device="cuda")
+    wide = torch.as_strided(room, (rows, vocab), (stride, 1))
+    wide.copy_(x.cuda())
+    targets = rng.integers(0, vocab, rows)
+    check(run(wide, targets, 20, ctx), x, targets, 20)

@@ -396,3 +396,25 @@ def test_waits_that_are_given_up(fmt, rows, cols, batch, copies):
         np.testing.assert_array_equal(run(w, x, 1, rows, own), want)
     w.close()
     own.close()
+
+
+def test_results_past_32_bits(ctx):
+    """More than 2^32 results, either way round."""
+    rows, cols, batch = 40001, 64, 110_003
+    rng = np.random.default_rng(20)
+    payload, dense = ref.q4_weight(rng, rows, cols, "q4_0")
+    w = cs.Q4Weight.from_payload(payload, "q4_0", rows, cols, ctx)
+    x = torch.tensor(rng.normal(0, 1, (batch, cols)), dtype=torch.float32)
+    toks = np.unique(np.concatenate([rng.integers(0, batch, 200), [0, 1, batch - 2, batch - 1, (1 << 32) // rows, (1 << 32) // rows + 1]]))
+    picked = np.unique(np.concatenate([rng.integers(0, rows, 200), [0, rows - 1, (1 << 32) // batch, (1 << 32) // batch + 1]]))
+    y = torch.empty(batch * rows, device="cuda")
+    for layout in (0, 1):
+        xd = (x if layout else x.t()).contiguous().cuda()
+        y.fill_(7.0)
+        torch.cuda.synchronize()
+        w.matmul_device(xd.data_ptr(), 0, layout, batch, y.data_ptr(), layout)
+        ctx.synchronize()
+        got = y.view(batch, rows) if layout else y.view(rows, batch).t()
+        check(got[torch.tensor(toks, device="cuda")].to(torch.float64).cpu().numpy(), x[toks], dense)
+        check(got[:, torch.tensor(picked, device="cuda")].to(torch.float64).cpu().numpy(), x, dense[picked])
+    w.close()
