@@ -107,7 +107,7 @@ struct Rows {
             const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : kTop;
             // the scale's sign goes with q: the largest score / factor is the largest score
             const float up = copysignf(power_of_two(kTop - e), p.a.scale);
-            factor[h] = fmaxf(fabsf(p.a.scale) * 1.4426950408889634f * power_of_two(min(e - kTop + kCodeShift, 127)), FLT_MIN);
+            factor[h] = factor_of(p.a.scale, e - kTop + kCodeShift, 100);      // scores / factor are below 2^22
 #pragma unroll
             for (uint32_t g = 0; g < G; ++g) sum_q[h][g] = 0.0f;
 #pragma unroll

@@ -19,6 +19,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// |scale| log2 e 2^n, what a row's products are multiplied by to be exponents of two. At least a normal number (nothing that is
+// smaller tells keys apart), and at most 2^most, so that no score passes fp32: there the least difference of two products decides.
+__device__ __forceinline__ float factor_of(float scale, int n, int most) {
+    const int first = min(n, 127);
+    const float f = fabsf(scale) * __int_as_float((first + 127) << 23) * (1.4426950408889634f * __int_as_float((n - first + 127) << 23));
+    return fminf(fmaxf(f, FLT_MIN), __int_as_float((most + 127) << 23));
+}
+
 struct AttnParams {
     KvView kv;
     KvBatchView b;

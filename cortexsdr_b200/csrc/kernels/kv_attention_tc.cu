@@ -252,7 +252,7 @@ kv_attention_tc_kernel(AttnParams p) {
                 // 2^e above the largest |q|; the scale's sign goes with q
                 const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : 15;
                 const float up = copysignf(power_of_two(15 - e), p.a.scale);
-                factor = fmaxf(fabsf(p.a.scale) * 1.4426950408889634f * power_of_two(e - 15), FLT_MIN);
+                factor = factor_of(p.a.scale, e - 15, 80);      // products are below 2^38
 #pragma unroll
                 for (uint32_t c = 0; c < HD / 8u; ++c) {
                     float v[8];

@@ -856,3 +856,27 @@ def test_strides_past_32_bits(ctx, dtype, group):
     close(part(group + 2, group), ref.attention(q, k, v, pos, hd ** -0.5), c.tdtype, np.abs(v).max(),
           bound_of(c, [rows], group, hd, new[0], k, v, pos, hd ** -0.5))
     c.cache.close()
+
+
+@pytest.mark.parametrize("dtype,fresh", [("f32", 1), ("f32", 260), ("bf16", 1), ("bf16", 60)])
+def test_queries_of_the_greatest_magnitude(ctx, dtype, fresh):
+    """Queries up to the type's largest number, with a scale that brings scores back to where they tell keys apart."""
+    c = Case(ctx, [300], [fresh], 2, 128, 32, seed=11, dtype=dtype)
+    c.store()
+    k, v = c.held()
+    pos = 300 - fresh + np.arange(fresh)
+    for top in (2.0 ** 122, 2.0 ** 125, 3e38):
+        q = c.values((fresh, 8, 128)).to(torch.float64)
+        scale = float(np.float32(float(q.abs().max()) / top / 128 ** 0.5))
+        q = (q * (top / q.abs().max())).to(c.tdtype)
+        out = c.attend(c.rows([q]), 8, scale=scale)
+        x = q.to(torch.float64).numpy()
+        close(out, ref.attention(x, k[0], v[0], pos, scale), c.tdtype, np.abs(v[0]).max(), bound_of(c, [fresh], 8, 128, q, k[0], v[0], pos, scale))
+    # scores past fp32: the greatest alone weighs
+    q = torch.sign(c.values((fresh, 8, 128)).to(torch.float64)) * 3e38
+    out = c.attend(c.rows([q.to(c.tdtype)]), 8)
+    x = q.to(c.tdtype).to(torch.float64).numpy()
+    if fresh == 1:
+        close(out, ref.attention(x, k[0], v[0], pos, 128 ** -0.5), c.tdtype, np.abs(v[0]).max())
+    assert torch.isfinite(out).all()
+    c.cache.close()
