@@ -104,7 +104,7 @@ struct Rows {
             // 2^e above the largest |q|: q 2^(top - e) < 2^15 (and sixteen times that), exact but for the last bits of what is
             // 2^-20 of the largest
             constexpr int kTop = kFine ? 15 : 11;
-            const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : kTop;
+            const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -110), 128) : kTop;      // 2^125 is the most that powers below go to
             // the scale's sign goes with q: the largest score / factor is the largest score
             const float up = copysignf(power_of_two(kTop - e), p.a.scale);
             factor[h] = factor_of(p.a.scale, e - kTop + kCodeShift, 100);      // scores / factor are below 2^22

@@ -250,7 +250,7 @@ kv_attention_tc_kernel(AttnParams p) {
 #pragma unroll
                     for (uint32_t i = 0; i < 8u; ++i) big = fmaxf(big, fabsf(op_widen(reinterpret_cast<const T*>(&raw[c])[i])));
                 // 2^e above the largest |q|; the scale's sign goes with q
-                const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -80), 128) : 15;
+                const int e = big > 0.0f && big < INFINITY ? min(max(ilogbf(big) + 1, -110), 128) : 15;
                 const float up = copysignf(power_of_two(15 - e), p.a.scale);
                 factor = factor_of(p.a.scale, e - 15, 80);      // products are below 2^38
 #pragma unroll

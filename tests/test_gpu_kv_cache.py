@@ -880,3 +880,20 @@ def test_queries_of_the_greatest_magnitude(ctx, dtype, fresh):
         close(out, ref.attention(x, k[0], v[0], pos, 128 ** -0.5), c.tdtype, np.abs(v[0]).max())
     assert torch.isfinite(out).all()
     c.cache.close()
+
+
+@pytest.mark.parametrize("dtype,fresh", [("f32", 1), ("f32", 260), ("bf16", 1), ("bf16", 60)])
+def test_queries_of_the_least_magnitude(ctx, dtype, fresh):
+    """Queries down to numbers that are not normal, with a scale that brings scores up to where they tell keys apart."""
+    c = Case(ctx, [300], [fresh], 2, 128, 32, seed=12, dtype=dtype)
+    c.store()
+    k, v = c.held()
+    pos = 300 - fresh + np.arange(fresh)
+    for top in (2.0 ** -80, 2.0 ** -100, 2.0 ** -115, 2.0 ** -123):
+        q = c.values((fresh, 8, 128)).to(torch.float64)
+        scale = float(np.float32(float(q.abs().max()) / top / 128 ** 0.5))
+        q = (q * (top / q.abs().max())).to(c.tdtype)
+        out = c.attend(c.rows([q]), 8, scale=scale)
+        x = q.to(torch.float64).numpy()
+        close(out, ref.attention(x, k[0], v[0], pos, scale), c.tdtype, np.abs(v[0]).max(), bound_of(c, [fresh], 8, 128, q, k[0], v[0], pos, scale))
+    c.cache.close()
