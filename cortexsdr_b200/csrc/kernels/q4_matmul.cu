@@ -158,8 +158,8 @@ __device__ __forceinline__ void stage(const Q4Params& p, uint32_t u0, uint32_t u
         if (kScaled) {
 #pragma unroll
             for (uint32_t o = kLanes / 2u; o; o >>= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-            // what is not finite stays as it is; 2^-100 counts as the smallest
-            if (big != 0u && big < 0x7F800000u) ex = max(static_cast<int>(big >> 23) - 127, -100);
+            // what is not finite stays as it is; 2^-112 counts as the smallest (from there every fp32 number is an fp16 one, or two)
+            if (big != 0u && big < 0x7F800000u) ex = max(static_cast<int>(big >> 23) - 127, -112);
         }
         const float up = power_of_two(14 - ex);
         float sum_hi = 0.0f, sum_lo = 0.0f;
@@ -198,8 +198,9 @@ __device__ __forceinline__ void stage(const Q4Params& p, uint32_t u0, uint32_t u
             }
             if (e % kLanes == 0u) {
                 float* backs = reinterpret_cast<float*>(mine + S::kBacksAt);
-                backs[column] = power_of_two(ex - 14);
-                if constexpr (SPLIT) backs[column + 4u] = power_of_two(ex - 14);
+                const float back = power_of_two(FMT ? ex - 14 : ex);      // the last 2^4 of q4_0's codes at the very end
+                backs[column] = back;
+                if constexpr (SPLIT) backs[column + 4u] = back;
             }
         }
     }
@@ -425,7 +426,7 @@ q4_matmul_kernel(Q4Params p) {
 #pragma unroll
                 for (uint32_t i = 0; i < 2u; ++i) {
                     if (tok + i >= n_tok) continue;
-                    constexpr float kCodes = FMT ? 1.0f : 1u << kCodeShift;
+                    constexpr float kCodes = FMT ? 1.0f : 1u << (kCodeShift - 14);
 #pragma unroll
                     for (uint32_t h = 0; h < 2u; ++h) {
                         const uint32_t e = (tok + i) * kRowsBlock + row + 8u * h, run = e / 32u, owner = run % ranks;

@@ -418,3 +418,22 @@ def test_results_past_32_bits(ctx):
         check(got[torch.tensor(toks, device="cuda")].to(torch.float64).cpu().numpy(), x[toks], dense)
         check(got[:, torch.tensor(picked, device="cuda")].to(torch.float64).cpu().numpy(), x, dense[picked])
     w.close()
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("largest", [2.0 ** -123, 2.0 ** -113, 2.0 ** -105, 2.0 ** 126])
+def test_activations_at_the_ends_of_their_range(ctx, fmt, dtype, largest):
+    """check()'s bound, and for results that are not normal fp32 numbers their last bit, 2^-149, for every partial sum (16 of
+    units and ranks) and for every sixteenth of it where a partial sum is kept 2^4 smaller."""
+    rng = np.random.default_rng(21)
+    payload, dense = ref.q4_weight(rng, 48, 768, fmt)
+    w = cs.Q4Weight.from_payload(payload, fmt, 48, 768, ctx)
+    x = torch.tensor(rng.normal(0, 1, (3, 768)))
+    x = (x / x.abs().max() * largest / (64 if largest > 1 else 1)).to(DTYPES[dtype][0])      # (sums of the largest stay finite)
+    y = run(w, x, 1, 48, ctx)
+    xx = x.to(torch.float64).numpy()
+    want, room = xx @ dense.T, np.abs(xx) @ np.abs(dense).T
+    assert np.isfinite(want.astype(np.float32)).all() and (want != 0).all()
+    assert (np.abs(y - want) <= 2.0 ** -19 * room + 16 * 16 * 2.0 ** -149).all()
+    w.close()
