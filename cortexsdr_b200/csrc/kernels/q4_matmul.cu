@@ -71,8 +71,8 @@ q4_relay_kernel(const uint8_t* __restrict__ in, Q4View w, uint8_t* __restrict__ 
 
 // The product. Weights are the rows of mma.m16n8k16 (their codes as subnormals, codes4.cuh), tokens its columns: eight
 // 16-bit tokens, or four fp32 ones as fp16 roundings and what these left (22 bits). Each group of 32 columns is two
-// products, whose sums in fp32 then meet the group's step; the 8 of q4_0 and the minima of q4_k come off through the
-// activations' own sums over the group.
+// products, whose sums in fp32 then meet the group's step. The 8 of q4_0 comes off the codes (exactly: a weight of nothing adds
+// nothing, however loud its activation), the minima of q4_k through the activations' own sums over the group.
 //
 // A one-token product must read the weights at the rate of the memory, and has no reuse to hide anything behind: a warp
 // owns sixteen rows and streams its units through registers, several ahead. Few rows do not fill the GPU that way, so the
@@ -96,9 +96,9 @@ template <int FMT, int NT, bool SPLIT>
 struct Q4Shape {
     static constexpr uint32_t kTokens = NT * (SPLIT ? 4u : 8u), kColumns = NT * 8u;
     static constexpr uint32_t kUnitCols = FMT ? 256u : 128u, kGroups = kUnitCols / 32u;
-    // of a unit: activations as fragments [group][column][t], the group sums that its columns need [group][column], and the powers
+    // of a unit: activations as fragments [group][column][t], of q4_k the sums that meet the minima [group][column], and the powers
     // of two that products are times as large [column]
-    static constexpr uint32_t kSumsAt = kGroups * kColumns * 64u, kBacksAt = kSumsAt + kGroups * kColumns * 4u;
+    static constexpr uint32_t kSumsAt = kGroups * kColumns * 64u, kBacksAt = kSumsAt + (FMT ? kGroups * kColumns * 4u : 0u);
     static constexpr uint32_t kStageBytes = kBacksAt + kColumns * 4u;
     // partial results of all ranks (runs of 32, so up to a run a rank more than there are), twice
     static constexpr uint32_t kSums = kRowsBlock * kTokens + 8u * 32u, kSumBytes = 2u * kSums * 4u;
@@ -162,7 +162,7 @@ __device__ __forceinline__ void stage(const Q4Params& p, uint32_t u0, uint32_t u
             if (big != 0u && big < 0x7F800000u) ex = max(static_cast<int>(big >> 23) - 127, -112);
         }
         const float up = power_of_two(14 - ex);
-        float sum_hi = 0.0f, sum_lo = 0.0f;
+        float sum_hi = 0.0f, sum_lo = 0.0f;      // for q4_k
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
@@ -177,24 +177,24 @@ __device__ __forceinline__ void stage(const Q4Params& p, uint32_t u0, uint32_t u
                 sum_hi += x + z;      // fp16 holds them as they are
             }
         }
-        sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 1);
-        sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 2);
-        if constexpr (SPLIT) {
+        if constexpr (FMT) {
+            sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 1);
+            sum_hi += __shfl_xor_sync(0xFFFFFFFFu, sum_hi, 2);
+        }
+        if constexpr (FMT && SPLIT) {
             sum_lo += __shfl_xor_sync(0xFFFFFFFFu, sum_lo, 1);
             sum_lo += __shfl_xor_sync(0xFFFFFFFFu, sum_lo, 2);
         }
         if (there) {
-            // q4_0: what the 8 of every code adds to the product; q4_k: the sum that the minimum meets
-            constexpr float kTake = FMT ? 1.0f : -8.0f / (1u << kCodeShift);
             const uint32_t column = SPLIT ? tok / 4u * 8u + tok % 4u : tok, at = gr * S::kColumns + column;
             uint8_t* mine = to + static_cast<size_t>(unit) * S::kStageBytes;
             uint4* frags = reinterpret_cast<uint4*>(mine);
-            float* sums = reinterpret_cast<float*>(mine + S::kSumsAt);
             frags[at * 4u + piece] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             if constexpr (SPLIT) frags[(at + 4u) * 4u + piece] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            if (piece == 0u) {
-                sums[at] = sum_hi * kTake;
-                if constexpr (SPLIT) sums[at + 4u] = sum_lo * kTake;
+            if (FMT && piece == 0u) {
+                float* sums = reinterpret_cast<float*>(mine + S::kSumsAt);
+                sums[at] = sum_hi;
+                if constexpr (SPLIT) sums[at + 4u] = sum_lo;
             }
             if (e % kLanes == 0u) {
                 float* backs = reinterpret_cast<float*>(mine + S::kBacksAt);
@@ -349,6 +349,13 @@ q4_matmul_kernel(Q4Params p) {
                             uint32_t a[4], b[4];
                             widen_codes<true>(word_of(w.codes[gr / 2u], (gr & 1u) * 2u), a);
                             widen_codes<true>(word_of(w.codes[gr / 2u], (gr & 1u) * 2u + 1u), b);
+                            if constexpr (FMT == 0) {
+#pragma unroll
+                                for (uint32_t j = 0; j < 4u; ++j) {
+                                    a[j] = less_eight(a[j]);
+                                    b[j] = less_eight(b[j]);
+                                }
+                            }
                             float sA, sB, mA = 0.0f, mB = 0.0f;
                             if constexpr (FMT == 0) {
                                 const float2 x = halves(word_of(w.steps[0], gr / 2u)), z = halves(word_of(w.steps[0], 2u + gr / 2u));
@@ -367,17 +374,11 @@ q4_matmul_kernel(Q4Params p) {
 #pragma unroll
                             for (uint32_t n = 0; n < NT; ++n) {
                                 const uint4 f = *(reinterpret_cast<const uint4*>(staged) + (gr * S::kColumns + n * 8u + g) * 4u + t);
-                                const float2 s = *reinterpret_cast<const float2*>(staged + S::kSumsAt + (gr * S::kColumns + n * 8u + 2u * t) * 4u);
                                 float c[4];
-                                if constexpr (FMT == 0) {
-                                    c[0] = c[2] = s.x;
-                                    c[1] = c[3] = s.y;
-                                    mma16816(c, a[0], b[0], a[1], b[1], f.x, f.y);
-                                } else {
-                                    mma16816_first(c, a[0], b[0], a[1], b[1], f.x, f.y);
-                                }
+                                mma16816_first(c, a[0], b[0], a[1], b[1], f.x, f.y);
                                 mma16816(c, a[2], b[2], a[3], b[3], f.z, f.w);
                                 if constexpr (FMT) {
+                                    const float2 s = *reinterpret_cast<const float2*>(staged + S::kSumsAt + (gr * S::kColumns + n * 8u + 2u * t) * 4u);
                                     z[n][0] = fmaf(mA, s.x, z[n][0]);
                                     z[n][2] = fmaf(mB, s.x, z[n][2]);
                                     if constexpr (!ONE) {
@@ -456,7 +457,7 @@ q4_matmul_kernel(Q4Params p) {
 struct Sizes {
     uint32_t tokens, stage_bytes, sum_bytes, groups;
     constexpr Sizes(bool split, int format, uint32_t nt)
-        : tokens(nt * (split ? 4u : 8u)), stage_bytes(q4_unit_cols(format) / 32u * nt * 8u * 68u + nt * 32u),
+        : tokens(nt * (split ? 4u : 8u)), stage_bytes(q4_unit_cols(format) / 32u * nt * 8u * (format ? 68u : 64u) + nt * 32u),
           sum_bytes(2u * (kRowsBlock * tokens + 8u * 32u) * 4u), groups(q4_unit_cols(format) / 32u) {}
     // units whose activations fit beside the partial results, with n CTAs an SM
     uint32_t staged(uint32_t n) const { return ((n == 2u ? 104u : 208u) * 1024u - sum_bytes) / stage_bytes; }
