@@ -58,7 +58,7 @@ int csdr_kv_cache_create(csdr_context* ctx, uint32_t n_layers, uint32_t n_pages,
     return guard([&] {
         require_ctx(ctx);
         if (!out) throw Error(CSDR_ERR_INVALID_ARG, "out is null");
-        if (!n_layers || !n_pages || !kv_heads || n_pages > 0x7FFFFFFFu)
+        if (!n_layers || !n_pages || !kv_heads || n_pages > 0x7FFFFFFFu || kv_heads > 65535u)      // as q_heads
             throw Error(CSDR_ERR_INVALID_ARG, "cache: zero or out-of-range field");
         if (page_tokens < kKvBlock || page_tokens > 4096u || (page_tokens & (page_tokens - 1u)))
             throw Error(CSDR_ERR_INVALID_ARG, "cache: page_tokens must be a power of two from 16 to 4096");

@@ -504,7 +504,7 @@ CSDR_API int csdr_decoder_step_device_async(csdr_decoder* d, const int32_t* toke
  * number of sequences through page tables. Each group of 64 values of a head is held as 4-bit codes with
  * an fp16 minimum and an fp16 step: minimum + step * code, step = (max - min) / 15 (4.5 bits a value with
  * head_dim 64, 128 or 256; 0.28 of an fp16 cache). A group that holds a value that is not finite reads
- * back as NaN; values past 65504 saturate. rope_theta at least 1: the rotary embedding that
+ * back as NaN; values past 65504 saturate. At most 65535 heads. rope_theta at least 1: the rotary embedding that
  * csdr_kv_cache_append_device_async applies on request; 0 or less: none. */
 CSDR_API int csdr_kv_cache_create(csdr_context* ctx, uint32_t n_layers, uint32_t n_pages,
                                   uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim,

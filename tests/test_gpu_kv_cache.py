@@ -897,3 +897,10 @@ def test_queries_of_the_least_magnitude(ctx, dtype, fresh):
         x = q.to(torch.float64).numpy()
         close(out, ref.attention(x, k[0], v[0], pos, scale), c.tdtype, np.abs(v[0]).max(), bound_of(c, [fresh], 8, 128, q, k[0], v[0], pos, scale))
     c.cache.close()
+
+
+def test_refuses_more_heads_than_queries_can_have(ctx):
+    """One page of the smallest: what would fit the device, but no call could attend over."""
+    with pytest.raises(ValueError, match="out-of-range"):
+        cs.KVCache(1, 16, 65536, 64, ctx=ctx)
+    cs.KVCache(1, 16, 65535, 64, ctx=ctx).close()
