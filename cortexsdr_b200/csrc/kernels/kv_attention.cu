@@ -730,6 +730,9 @@ void launch_rows(csdr_context* ctx, uint64_t rows, AttnParams& p) {
     //   fp32   49, 72, 203, 680 and 51, 81, 212, 647 (heads of 256: 74, 119, 388, 1358 and 96, 141, 401, 1286)
     //   fp16   43, 64, 177, 585 and 57, 75, 147, 363
     //   bf16   41, 58, 160, 526 and, on tcgen05, 51, 53, 76, 164 (fp16 outputs are eight times as fine and keep their codes)
+    // One form for all sequences of a call, whatever they have: a captured call does not know. Single tokens beside a prompt cost
+    // more than in a call of their own: 31 over 8192 keys and 2048 rows of a prompt 515 (fp32), 543 (fp16), 364 (bf16), as two calls
+    // 486, 309, 191; 31 over 1024 and 512 rows of a prompt 74, 61, 57, as two calls 85, 83, 72.
     constexpr bool kWide = std::is_same<T, float>::value || HD > 128;
     if (rows < (kWide ? 1024u : std::is_same<T, __half>::value ? 192u : 96u)) {
         launch<T, HD, true, 1>(ctx, p);

@@ -10,11 +10,12 @@
 // that the matrix unit does not wait for the exponentials (a warp of its own for that would leave every thread 96 registers
 // instead of 128). Two CTAs an SM fill what is left. Work is cut as there (kv_attention.cuh).
 //
-// 3 sequences of 2048 with 512 new tokens, 32 query heads over 8 of 128: 114 us, 332 TFLOP/s (by warps 245 us). The products
+// 3 sequences of up to 2048 with 512 new tokens, 32 query heads over 8 of 128: 114 us, 332 TFLOP/s (by warps 245 us). The products
 // are 42 of it (one of 64 columns takes 75 cycles, of 128 columns 121: 1080 a block); a warp widens its part of a block in 1400
 // cycles and has a row's weights in 960. A block passes through the three one after the other, and two CTAs overlap them only
-// in part. Tried and slower: 256 rows a CTA
-// (129 us: one CTA's phases have nobody beside them), keys published before values (122 us).
+// in part: a CTA has a block every 7200 cycles (31 blocks each at 1.965 GHz), of which these are 3440. The rest are the waits
+// between the roles, and what 128 registers a thread do not hold (heads of 128: 560 bytes of spills, 640 of reloads). Tried and
+// slower: 256 rows a CTA (129 us: one CTA's phases have nobody beside them), keys published before values (122 us).
 #include "codes4.cuh"
 #include "kv_attention.cuh"
 

@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t meta_offset(uint32_t tok, uint32_t d, uint32
 }
 
 // cos and sin of position * freq, to fp32's precision: the angle is reduced by multiples of pi / 2 in 64 bits (Cody
-// and Waite: pi / 2 as a 33-bit head, whose multiples are exact, and the rest), then Taylor series, 1e-9 at pi / 4.
+// and Waite: pi / 2 as a 33-bit head, whose multiples are exact, and the rest), then Taylor series, 1.8e-9 at pi / 4.
 __device__ __forceinline__ float2 turn(int32_t pos, double freq) {
     const double a = static_cast<double>(pos) * freq, k = rint(a * 0.63661977236758134);
     const double x = fma(k, -6.077100506506192e-11, fma(k, -1.5707963267341256, a)), z = x * x;

@@ -10,8 +10,8 @@ namespace csdr {
 
 // How a weight lies on the device: units of sixteen rows and kCols columns, a row tile's units one behind the
 // other. A unit: codes, for each pair of 32-column groups and each lane (g = lane / 4, t = lane % 4) the words
-// (row g, group 0), (row g + 8, group 0), (row g, group 1), (row g + 8, group 1), column 8 t + n of the
-// group in bits 4n; then for g < 8 the steps of rows g and g + 8:
+// (row g, group 0), (row g + 8, group 0), (row g, group 1), (row g + 8, group 1), columns 8 t + 0 .. 3 of the
+// group in a word's low half, + 4 .. 7 in its high half (pack_codes, codes4.cuh); then for g < 8 the steps of rows g and g + 8:
 //   q4_0   128 columns; fp16 steps [g][row g, row g + 8][4 groups]
 //   q4_k   256 columns; 6-bit (step, minimum) as bytes [g][row][8 groups], then fp16 (d, dmin) [g][row]
 // so that a lane finds what its matrix fragments take in 128-bit pieces and a row tile is read front to

@@ -55,8 +55,8 @@ enum {
 };
 
 enum { CSDR_DTYPE_F32 = 0, CSDR_DTYPE_BF16 = 1,
-       CSDR_KV_Q4 = 16 /* csdr_decoder_config.kv_dtype only */,
        CSDR_DTYPE_F16 = 2 /* KV caches and the operators that say so; elsewhere activations are fp32 or bf16 */ };
+enum { CSDR_KV_Q4 = 16 /* no element type: csdr_decoder_config.kv_dtype for the 4-bit cache */ };
 enum { CSDR_LAYOUT_FEATURE_MAJOR = 0, CSDR_LAYOUT_TOKEN_MAJOR = 1 };
 enum { CSDR_KIND_HSDR = 0, CSDR_KIND_HSDC = 1 };
 
@@ -510,6 +510,7 @@ CSDR_API int csdr_kv_cache_create(csdr_context* ctx, uint32_t n_layers, uint32_t
                                   uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim,
                                   float rope_theta, csdr_kv_cache** out);
 CSDR_API int csdr_kv_cache_destroy(csdr_kv_cache* cache);
+/* Of its pages. Beside them a cache has the workspace of its attention calls, 20 MB with heads of 64, else 40. */
 CSDR_API int csdr_kv_cache_bytes(const csdr_kv_cache* cache, size_t* bytes);
 
 /* A ragged batch of new tokens, all arrays on the device. Sequence s has rows first_dev[s] to
@@ -528,7 +529,7 @@ typedef struct {
 
 /* Stores the new tokens' keys and values (n_tokens x kv_heads x head_dim; kv_stride elements between the
  * rows of either, 0: dense; dtype: CSDR_DTYPE_F32, _BF16 or _F16). rotate != 0: keys, and queries where given
- * (q_dev, q_stride, q_heads -> q_out_dev, q_out_stride; q_out may be q itself), are rotated by their position
+ * (q_dev, q_stride, q_heads -> q_out_dev, q_out_stride; q_out may be q itself, and overlaps nothing else), are rotated by their position
  * as the decoder rotates them (adjacent pairs, api/cortex_sdk.cpp:1363-1423), angles in 64 bits; else
  * queries are copied. Tokens must have slots of their own. Asynchronous on the cache's context. */
 CSDR_API int csdr_kv_cache_append_device_async(csdr_kv_cache* cache, uint32_t layer,
@@ -544,9 +545,11 @@ CSDR_API int csdr_kv_cache_read_device_async(csdr_kv_cache* cache, uint32_t laye
  * out = softmax(scale * q k^T) v (multi_head_attention, kernels/attention_kernels.cpp:26-113), a new token
  * seeing every token up to its own position. q and out: n_tokens x q_heads x head_dim of `dtype`, strides
  * as above; out must not overlap q; scale 0: 1 / sqrt(head_dim). A token that sees nothing gets zeros.
- * Scores, weights and sums in fp32; of bf16 prompts (heads of 64 or 128, 96 query rows and more of a kv head a
- * sequence on average) keys, values and weights are operands in fp16, 2^-11 of themselves, and sums fp32. Calls on one cache
- * share its workspace: they run one after the other, graphs that were captured from them too. */
+ * Scores, weights and sums in fp32, operands to 22 bits; of 16-bit rows sums lose four bits. Of bf16 rows and of fp16 prompts (heads
+ * of 64 or 128, 192 query rows and more of a kv head a sequence on average, over all sequences and rows of the call) a weight
+ * times a value's step is one operand in fp16, 2^-12 of itself; of bf16 prompts (96 and more) keys, values and weights are,
+ * 2^-11 of themselves. Calls on one cache share its workspace: they run one after the other, graphs that were captured from them
+ * too. */
 CSDR_API int csdr_kv_cache_attention_device_async(csdr_kv_cache* cache, uint32_t layer,
                                                   const csdr_kv_batch* batch, const void* q_dev,
                                                   size_t q_stride, int dtype, uint32_t q_heads, float scale,
@@ -559,9 +562,9 @@ CSDR_API int csdr_kv_cache_attention_device_async(csdr_kv_cache* cache, uint32_t
 CSDR_API int csdr_q4_create(csdr_context* ctx, const char* format, const void* payload, size_t nbytes,
                             uint32_t rows, uint32_t cols, csdr_q4_weight** out);
 CSDR_API int csdr_q4_destroy(csdr_q4_weight* weight);
-/* y = W x (+ bias), fp32 out; dtypes (CSDR_DTYPE_F16 too) and layouts as csdr_matmul_device_async. Products and sums
- * are those of fp32 activations; an activation that is not finite leaves its token's results not finite. y must not
- * overlap x. Products of several tokens share scratch of the context: they run one after the other, graphs that were
+/* y = W x (+ bias), fp32 out; dtypes (CSDR_DTYPE_F16 too) and layouts as csdr_matmul_device_async. An activation is held
+ * to 2^-22 of itself and 2^-39 of the largest of its 128 columns (q4_k: 256), sums are fp32: results are within 2^-19 of
+ * sum |x w| for widths to 2^14. One that is not finite leaves its token's results not finite. y must not overlap x. Products of several tokens share scratch of the context: they run one after the other, graphs that were
  * captured from them too. Asynchronous on the context's stream. */
 CSDR_API int csdr_q4_matmul_device_async(csdr_context* ctx, const csdr_q4_weight* weight,
                                          const void* x_dev, int x_dtype, int x_layout, size_t batch,
