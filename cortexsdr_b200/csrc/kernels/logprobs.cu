@@ -7,11 +7,11 @@
 // when the maximum grows. A logit may be among the alternatives only if it reaches a bound that the k-th best cannot be below:
 // the least, over the CTA's W warps, of the ceil(k / W)-th greatest of the lanes' maxima so far, taken after the first
 // round and whenever the logits seen have doubled. What reaches it is put aside, some hundred pieces of a row,
-// and ranked at the end (2048 rows of 151936 in bf16: 101 us without alternatives, 132 with 20 - 140 to 146 in a long run of calls,
-// where the power cap holds the clock at 1.87 GHz -, 156 with lists kept in order on the way). A row where more do than there is room for (rising order) is read again with the
-// bound it ended with, into sorted lists. Keys are (logit, index), so results do not depend on who comes first. Few rows
-// are cut over the CTAs of a cluster, whose leader joins them. What bounds it: the logits' bytes, and behind them the
-// exponentials (one a logit, sixteen a clock and SM: 0.7 of the memory's time for 16-bit logits).
+// and ranked at the end (2048 rows of 151936 in bf16: 101 us without alternatives, 132 with 20, 156 with lists kept in order on the
+// way; in a long run of calls 140 to 146, where the power cap holds the clock at 1.87 GHz). A row where more do than there is room
+// for (rising order) is read again with the bound it ended with, into sorted lists. Keys are (logit, index), so results do not depend
+// on who comes first. Few rows are cut over the CTAs of a cluster, whose leader joins them. What bounds it: the logits' bytes, and
+// behind them the exponentials (one a logit, sixteen a clock and SM: 0.7 of the memory's time for 16-bit logits).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -61,7 +61,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_
         if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
     return false;
 }
-// A kernel's first wait: without a limit it is given up whatever it finds (CSDR_WAIT_GIVE_UP).
+// Where a kernel's first wait is: without a limit it is given up whatever it finds (CSDR_WAIT_GIVE_UP).
 __device__ __forceinline__ bool mbar_wait_first(uint32_t bar, uint32_t parity, uint32_t limit) {
     return mbar_wait(bar, parity, limit) && limit != 0u;
 }

@@ -463,7 +463,8 @@ struct Sizes {
     uint32_t staged(uint32_t n) const { return ((n == 2u ? 104u : 208u) * 1024u - sum_bytes) / stage_bytes; }
 };
 
-// Clusters of r CTAs that are resident at once, n CTAs an SM (GPCs do not divide by every r).
+// Clusters of r CTAs that are resident at once, n CTAs an SM (GPCs do not divide by every r); none where r do not fit one.
+constexpr uint32_t kNoCluster = 0xFFFFFFFFu;
 uint32_t resident(csdr_context* ctx, uint32_t n, uint32_t r) {
     uint32_t& known = ctx->q4_resident[n - 1u][r - 1u];
     if (!known && r == 1u) known = static_cast<uint32_t>(ctx->sm_count) * n;
@@ -483,9 +484,9 @@ uint32_t resident(csdr_context* ctx, uint32_t n, uint32_t r) {
         cfg.numAttrs = 1;
         int clusters = 0;
         CSDR_CUDA(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
-        known = static_cast<uint32_t>(std::max(clusters, 1));
+        known = clusters > 0 ? static_cast<uint32_t>(clusters) : kNoCluster;
     }
-    return known;
+    return known == kNoCluster ? 0u : known;
 }
 
 // Token tiles a launch whose fragments are made ahead: what 16 MB hold.
@@ -518,7 +519,9 @@ Cut cut_of(csdr_context* ctx, const Q4View& w, bool split, size_t batch, bool ma
         const float unit = (nt == 1u ? 0.5f : nt == 2u ? 0.8f : 1.7f) * (w.format ? 3.0f : 1.0f);
         for (uint32_t n = 2; n >= 1u; --n)
             for (uint32_t r = 1; r <= 8u && r <= w.n_units; ++r) {
-                const uint32_t fit = resident(ctx, n, r), units = (w.n_units + r - 1u) / r, fits = sz.staged(n);
+                const uint32_t fit = resident(ctx, n, r);
+                if (!fit) continue;
+                const uint32_t units = (w.n_units + r - 1u) / r, fits = sz.staged(n);
                 const uint32_t most = std::min(blocks, std::max(1u, static_cast<uint32_t>(ctx->sm_count) * n / r));
                 const uint32_t fewer = std::min<uint32_t>(most, std::max<uint32_t>(1u, static_cast<uint32_t>(ctx->sm_count * n / r / tiles)));
                 const float items = static_cast<float>((units * std::min<size_t>(batch, sz.tokens) * sz.groups * 4u + kThreads - 1u) / kThreads);
